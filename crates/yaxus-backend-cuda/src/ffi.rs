@@ -130,6 +130,10 @@ extern "C" {
     pub fn yx_add_assign(ctx: *mut yx_ctx, a_dev: *mut f32, b_dev: *const f32, n: usize) -> c_int;
     pub fn yx_select_rows(ctx: *mut yx_ctx, x_dev: *const f32, src_rows: u32, cols: u32, rows_host: *const u32, n: u32, out_dev: *mut f32) -> c_int;
     pub fn yx_argmax_rows(ctx: *mut yx_ctx, logits_dev: *const f32, rows: u32, cols: u32, out_host: *mut u32) -> c_int;
+    // ---- from hidden states to log probabilities
+    pub fn yx_matmul_epilogue(ctx: *mut yx_ctx, x_dev: *const c_void, x_dtype: c_int, w_bf16_dev: *const c_void, bias_dev: *const f32, activation: c_int, residual_dev: *const c_void, rows: u32, n: u32, k: u32, out_dev: *mut c_void, out_dtype: c_int) -> c_int;
+    pub fn yx_logprob_rows(ctx: *mut yx_ctx, logits_dev: *const c_void, dtype: c_int, rows: u32, cols: u32, stride: usize, ids_host: *const u32, n_ids: u32, n_top: u32, logprob_dev: *mut f32, entropy_dev: *mut f32, top_ids_dev: *mut u32, top_logprob_dev: *mut f32) -> c_int;
+    pub fn yx_matmul_logprobs(ctx: *mut yx_ctx, x_dev: *const c_void, x_dtype: c_int, w_bf16_dev: *const c_void, rows: u32, n: u32, k: u32, ids_host: *const u32, logprob_dev: *mut f32, entropy_dev: *mut f32) -> c_int;
     // ---- attention without allocation
     pub fn yx_attend_static(ctx: *mut yx_ctx, kv: *mut yx_kv, layer: c_int, q_dev: *const c_void, q_dtype: c_int, hq: c_int, window: i64, out_dev: *mut c_void, out_dtype: c_int) -> c_int;
 }

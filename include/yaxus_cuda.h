@@ -261,6 +261,49 @@ int yx_argmax_rows(yx_ctx *ctx, const float *logits_dev, uint32_t rows, uint32_t
 int yx_attend_static(yx_ctx *ctx, yx_kv *kv, int layer, const void *q_dev, int q_dtype, int hq, int64_t window,
                      void *out_dev, int out_dtype);
 
+/* ---- From hidden states to log probabilities (no counterpart in the reference) ------------------
+ * What a served model needs beside the trait's operators: projections with a bias, an activation or
+ * a residual, and the log probabilities that a serving API reports with its tokens.  All of them
+ * enqueue on the context's stream and wait for nothing.  Scratch grows with the largest call so far
+ * and is never given back before yx_ctx_destroy, so a recorded call stays valid whatever calls
+ * follow it; a call that would have to allocate while its stream is being captured is refused (make
+ * one of its size before).  Calls of one context, recorded ones included, share that scratch:
+ * replay them in the order of one stream. */
+
+enum yx_activation {
+    YX_ACT_NONE = 0,
+    YX_ACT_RELU = 1,
+    YX_ACT_GELU = 2,        /* y (1 + erf(y / sqrt 2)) / 2 */
+    YX_ACT_GELU_TANH = 3,   /* y (1 + tanh(sqrt(2 / pi) (y + 0.044715 y^3))) / 2 */
+    YX_ACT_SILU = 4         /* y / (1 + exp(-y)) */
+};
+
+/* out [rows, n] = act(x [rows, k] . w [n, k]^T + bias) + residual.  x of `x_dtype`, taken exactly (no
+ * rounding to w's type); w bf16; bias f32 [n] or null; residual [rows, n] of `out_dtype` or null.  Sums
+ * and epilogue are f32, rounded once to `out_dtype`.  out may be the residual itself (x += ...) and may
+ * lie over x; over w, over the bias or over part of the residual it is refused. */
+int yx_matmul_epilogue(yx_ctx *ctx, const void *x_dev, int x_dtype, const void *w_bf16_dev, const float *bias_dev,
+                       int activation, const void *residual_dev, uint32_t rows, uint32_t n, uint32_t k, void *out_dev,
+                       int out_dtype);
+
+/* Log probabilities under the softmax of each row of logits [rows, cols] of `dtype`, rows `stride`
+ * elements apart (stride >= cols; cols is the vocabulary, what lies between is not read).
+ *   logprob  [rows, n_ids]:  log p of the row's given tokens, ids_host [rows, n_ids] (copied at once)
+ *   entropy  [rows]:         -sum p log p, in nats
+ *   top_ids, top_logprob [rows, n_top]: the most probable tokens, largest first, equal logits by token
+ * Each may be null (logprob with n_ids 0, the top pair with n_top 0); n_top <= YX_TOP_MAX and <= cols.
+ * A logit that is no number counts as -inf, as in yx_argmax_rows, and +inf as the largest f32.  A row
+ * with nothing above -inf has log probabilities -inf and entropy 0. */
+#define YX_TOP_MAX 32
+int yx_logprob_rows(yx_ctx *ctx, const void *logits_dev, int dtype, uint32_t rows, uint32_t cols, size_t stride,
+                    const uint32_t *ids_host, uint32_t n_ids, uint32_t n_top, float *logprob_dev, float *entropy_dev,
+                    uint32_t *top_ids_dev, float *top_logprob_dev);
+
+/* yx_logprob_rows of the logits x [rows, k] . w [n, k]^T, one given token a row, without the logits:
+ * logprob [rows] of ids_host [rows], entropy [rows] or null.  x and w as for yx_matmul_epilogue. */
+int yx_matmul_logprobs(yx_ctx *ctx, const void *x_dev, int x_dtype, const void *w_bf16_dev, uint32_t rows, uint32_t n,
+                       uint32_t k, const uint32_t *ids_host, float *logprob_dev, float *entropy_dev);
+
 #ifdef __cplusplus
 }
 #endif

@@ -10,7 +10,7 @@ from .kvcache import KvCache, PassMeta, slot  # noqa: F401
 
 def __getattr__(name):
     # CudaBackend needs torch; import it lazily so that the host-side pieces work without it.
-    if name in ("CudaBackend", "LayerMeta", "Rope", "Kv", "BackendError"):
+    if name in ("CudaBackend", "LayerMeta", "Rope", "Kv", "LogProbs", "BackendError"):
         from . import backend
         return getattr(backend, name)
     raise AttributeError(name)

@@ -16,6 +16,8 @@ YX_OK, YX_ERR_INVALID, YX_ERR_CUDA, YX_ERR_OOM, YX_ERR_STATE, YX_ERR_DEVICE, YX_
 F32, F16, BF16 = 0, 1, 2
 PAGE = 128
 HEAD_DIM = 128
+ACTIVATIONS = {None: 0, "none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}   # yx_activation
+TOP_MAX = 32                                    # most alternatives yx_logprob_rows gives
 STATIC_SPLITS, STATIC_MAX_ROW_HEADS = 8, 1024   # yx_attend_static's built-in scratch
 PROBE_ITEM_WORDS = 41
 
@@ -81,6 +83,11 @@ SIGNATURES = {
     "yx_add_assign": (c_int, [c_void_p, c_void_p, c_void_p, c_size_t]),
     "yx_select_rows": (c_int, [c_void_p, c_void_p, c_uint32, c_uint32, c_void_p, c_uint32, c_void_p]),
     "yx_argmax_rows": (c_int, [c_void_p, c_void_p, c_uint32, c_uint32, c_void_p]),
+    "yx_matmul_epilogue": (c_int, [c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p, c_uint32, c_uint32, c_uint32,
+                                   c_void_p, c_int]),
+    "yx_logprob_rows": (c_int, [c_void_p, c_void_p, c_int, c_uint32, c_uint32, c_size_t, c_void_p, c_uint32, c_uint32, c_void_p,
+                                c_void_p, c_void_p, c_void_p]),
+    "yx_matmul_logprobs": (c_int, [c_void_p, c_void_p, c_int, c_void_p, c_uint32, c_uint32, c_uint32, c_void_p, c_void_p, c_void_p]),
     "yx_attend_static": (c_int, [c_void_p, c_void_p, c_int, c_void_p, c_int, c_int, c_int64, c_void_p, c_int]),
     "yx_attend_partial": (c_int, [c_void_p, c_void_p, c_int, c_void_p, c_int, c_int, c_int64, c_uint64, c_uint64,
                                   c_void_p, c_void_p, c_void_p]),

@@ -9,7 +9,7 @@ own device memory and the stream; every computation is a kernel of the C library
 """
 import ctypes
 from dataclasses import dataclass, field
-from typing import List, Optional, Sequence
+from typing import List, NamedTuple, Optional, Sequence
 
 import numpy as np
 import torch
@@ -75,6 +75,14 @@ class Kv:
             pass
 
 
+class LogProbs(NamedTuple):
+    """What `logprob_rows` and `matmul_logprobs` give, on the device; None where it was not asked for."""
+    logprob: Optional[torch.Tensor]            # of the given tokens, in their shape
+    entropy: Optional[torch.Tensor] = None     # [rows], in nats
+    top_ids: Optional[torch.Tensor] = None     # [rows, top] int32, most probable first
+    top_logprob: Optional[torch.Tensor] = None
+
+
 # Addresses go to the C ABI as plain integers: at decode sizes an operator's kernel takes no longer than
 # its call, and making a ctypes object for every argument (2 us for a numpy array's) was a tenth of it.
 def _ptr(t: Optional[torch.Tensor]):
@@ -83,6 +91,14 @@ def _ptr(t: Optional[torch.Tensor]):
 
 def _u32(a) -> np.ndarray:
     return np.ascontiguousarray(a, dtype=np.uint32)
+
+
+def _token_ids(a) -> np.ndarray:
+    a = np.asarray(a)
+    assert a.dtype.kind in "iu" or a.size == 0, "token ids are whole numbers"
+    if a.dtype != np.uint32:   # (a negative or a huge one must not wrap around into the vocabulary)
+        assert a.size == 0 or (a.min() >= 0 and a.max() <= 0xffffffff), "a token id is outside the vocabulary"
+    return _u32(a)
 
 
 def _u32p(a: np.ndarray) -> int:
@@ -300,6 +316,60 @@ class CudaBackend:
         if rc != _lib.YX_OK:
             raise BackendError(rc, self.last_error())
         return out
+
+    # ---- from hidden states to log probabilities ------------------------------------------
+    def _here(self, t: torch.Tensor) -> bool:
+        return t.get_device() == self.device.index   # (-1 for a tensor in host memory)
+
+    def _check_product(self, x: torch.Tensor, w: torch.Tensor) -> None:
+        assert self._here(x) and x.dim() == 2 and x.dtype in _YX_DTYPE and x.is_contiguous()
+        assert self._here(w) and w.dim() == 2 and w.dtype == torch.bfloat16 and w.is_contiguous()
+        assert x.shape[1] == w.shape[1], "matmul inner dim"
+
+    def matmul_epilogue(self, x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = None, activation: Optional[str] = None,
+                        residual: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
+                        out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+        """act(x [T, K] . w [N, K]^T + bias) + residual, for x and result f32 or 16-bit and w a bf16 matrix.  `activation`:
+        "relu", "gelu", "gelu_tanh", "silu" or None.  `out` may be the residual.  The result's type is `out`'s, else
+        `out_dtype`, else the residual's, else f32."""
+        assert activation in _lib.ACTIVATIONS, "unknown activation"
+        self._check_product(x, w)
+        shape = (x.shape[0], w.shape[0])
+        if out is None:
+            out = torch.empty(shape, dtype=out_dtype or (torch.float32 if residual is None else residual.dtype), device=self.device)
+        assert self._here(out) and out.shape == shape and out.dtype in _YX_DTYPE and out.is_contiguous()
+        assert bias is None or (self._here(bias) and bias.dtype == torch.float32 and bias.shape == shape[1:] and bias.is_contiguous())
+        assert residual is None or (self._here(residual) and residual.dtype == out.dtype and residual.shape == shape and residual.is_contiguous())
+        self._L.yx_matmul_epilogue(self._ctx, _ptr(x), _YX_DTYPE[x.dtype], _ptr(w), _ptr(bias), _lib.ACTIVATIONS[activation],
+                                   _ptr(residual), x.shape[0], w.shape[0], w.shape[1], _ptr(out), _YX_DTYPE[out.dtype])
+        return out
+
+    def logprob_rows(self, logits: torch.Tensor, ids=None, top: int = 0, entropy: bool = False) -> LogProbs:
+        """Log probabilities under the softmax of each row of `logits` (f32 or 16-bit; rows may lie further apart than they
+        are long): of the given tokens `ids` ([rows] or [rows, n], on the host), the entropy, the `top` most probable."""
+        assert self._here(logits) and logits.dim() == 2 and logits.dtype in _YX_DTYPE and (logits.shape[1] <= 1 or logits.stride(1) == 1)
+        rows, cols = logits.shape
+        stride = logits.stride(0) if rows > 1 else cols
+        idx = None if ids is None else _token_ids(ids)
+        assert idx is None or (idx.ndim in (1, 2) and idx.shape[0] == rows), "one row of ids for each row of logits"
+        new = lambda *shape, dtype=torch.float32: torch.empty(shape, dtype=dtype, device=self.device)   # noqa: E731
+        n_ids = 0 if idx is None else idx.size // max(rows, 1)
+        r = LogProbs(new(*idx.shape) if n_ids else None, new(rows) if entropy else None,
+                     new(rows, top, dtype=torch.int32) if top else None, new(rows, top) if top else None)
+        self._L.yx_logprob_rows(self._ctx, _ptr(logits), _YX_DTYPE[logits.dtype], rows, cols, stride, _u32p(idx) if n_ids else None, n_ids,
+                                top, _ptr(r.logprob), _ptr(r.entropy), _ptr(r.top_ids), _ptr(r.top_logprob))
+        return r
+
+    def matmul_logprobs(self, x: torch.Tensor, w: torch.Tensor, ids, entropy: bool = True) -> LogProbs:
+        """`logprob_rows(x . w^T, ids)` for one given token a row, without the logits ever being stored."""
+        self._check_product(x, w)
+        idx = _token_ids(ids)
+        assert idx.shape == (x.shape[0],), "one id for each row"
+        r = LogProbs(torch.empty(x.shape[0], dtype=torch.float32, device=self.device),
+                     torch.empty(x.shape[0], dtype=torch.float32, device=self.device) if entropy else None)
+        self._L.yx_matmul_logprobs(self._ctx, _ptr(x), _YX_DTYPE[x.dtype], _ptr(w), x.shape[0], w.shape[0], w.shape[1], _u32p(idx),
+                                   _ptr(r.logprob), _ptr(r.entropy))
+        return r
 
     def attention(self, qkv: torch.Tensor, q_norm: torch.Tensor, k_norm: torch.Tensor, kv: Kv, hq: int, eps: float,
                   layer: LayerMeta) -> torch.Tensor:

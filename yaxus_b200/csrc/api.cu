@@ -50,6 +50,26 @@ int ensure_buffer(yx_ctx *ctx, void **buf, size_t *cap, size_t bytes) {
     return YX_OK;
 }
 
+int grow(yx_ctx *ctx, yx_ctx::Grown &buf, size_t bytes) {
+    if (bytes <= buf.cap && buf.dev) return YX_OK;
+    cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+    if (int rc = check_cuda(ctx, cudaStreamIsCapturing(ctx->stream, &capture), "cudaStreamIsCapturing")) return rc;
+    if (capture != cudaStreamCaptureStatusNone)
+        return fail(ctx, YX_ERR_STATE, "scratch would have to grow while the stream is being captured: make a call of this size first");
+    const size_t want = std::max<size_t>(bytes + bytes / 2, 4096);
+    void *p = nullptr;
+    if (int rc = check_cuda(ctx, cudaMalloc(&p, want), "cudaMalloc (workspace)")) return rc;
+    try {
+        if (buf.dev) ctx->outgrown.push_back(buf.dev);
+    } catch (const std::bad_alloc &) {
+        cudaFree(p);
+        return fail(ctx, YX_ERR_OOM, "out of host memory");
+    }
+    buf.dev = (char *)p;
+    buf.cap = want;
+    return YX_OK;
+}
+
 // The reference writes pass metadata through its command stream so that it lands after the
 // kernels of earlier passes (crates/yaxus-backend-gpu/src/dev/wgpu/mod.rs:284-294).  Here a
 // ring of pinned buffers does the same: the caller's arrays are copied at once, the
@@ -602,6 +622,9 @@ void yx_ctx_destroy(yx_ctx *ctx) {
     if (ctx->idx_dev) cudaFree(ctx->idx_dev);
     if (ctx->pick_counters) cudaFree(ctx->pick_counters);
     if (ctx->pick_host) cudaFreeHost(ctx->pick_host);
+    for (yx_ctx::Grown *b : {&ctx->lp_ids, &ctx->lp_logits, &ctx->ep_rows})
+        if (b->dev) cudaFree(b->dev);
+    for (void *p : ctx->outgrown) cudaFree(p);
     if (ctx->gather_buf) cudaFree(ctx->gather_buf);
     if (ctx->dev_status) cudaFreeHost(ctx->dev_status);
     for (auto &e : ctx->prof_events)

@@ -1,0 +1,125 @@
+// Matrix products that end in something other than themselves: bias, activation and residual (yx_matmul_epilogue), or
+// the log probabilities of a softmax over the product's columns (yx_matmul_logprobs).  No counterpart in the reference,
+// whose models have projections without bias and a gated MLP; the products are those of yx_matmul.
+#include <algorithm>
+
+#include "yx_epilogue.cuh"
+
+namespace yx {
+namespace {
+
+using namespace dev;
+
+// Any shape: a warp per output, pass rows in the grid's y extent.
+__global__ void matmul_epilogue_any_kernel(const void *__restrict__ x, int x_dtype, const __nv_bfloat16 *__restrict__ w, uint32_t N, uint32_t K,
+                                           const Epilogue e, void *out) {
+    const uint32_t n = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5), t = blockIdx.y, lane = threadIdx.x & 31;
+    if (n >= N) return;
+    float s = 0.0f;
+    for (uint32_t k = lane; k < K; k += 32) s += __bfloat162float(w[(size_t)n * K + k]) * load_as_f32(x, x_dtype, (size_t)t * K + k);
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
+    if (lane != 0) return;
+    const size_t at = (size_t)t * N + n;
+    float y = activate(e.bias ? s + e.bias[n] : s, e.act);
+    if (e.residual) y += load_as_f32(e.residual, e.out_dtype, at);
+    store_from_f32(out, e.out_dtype, at, y);
+}
+
+size_t size_of(int dtype) { return dtype == YX_F32 ? 4 : 2; }
+bool valid(int dtype) { return dtype == YX_F32 || dtype == YX_F16 || dtype == YX_BF16; }
+bool overlap(const void *a, size_t an, const void *b, size_t bn) {
+    return a && b && (uintptr_t)a < (uintptr_t)b + bn && (uintptr_t)b < (uintptr_t)a + an;
+}
+
+bool aligned(const void *p, size_t size) { return ((uintptr_t)p & (size - 1)) == 0; }
+
+struct Guard {
+    int prev = -1;
+    explicit Guard(int dev) {
+        cudaGetDevice(&prev);
+        if (prev != dev) cudaSetDevice(dev);
+        else prev = -1;
+    }
+    ~Guard() {
+        if (prev >= 0) cudaSetDevice(prev);
+    }
+};
+
+int matmul_any(yx_ctx *ctx, const void *x, int x_dtype, const void *w, uint32_t T, uint32_t N, uint32_t K, const Epilogue &e, void *out) {
+    const size_t xs = size_of(x_dtype), os = size_of(e.out_dtype);
+    for (uint32_t t0 = 0; t0 < T; t0 += 65535u) {   // (the y extent's end)
+        Epilogue part = e;
+        if (e.residual) part.residual = (const char *)e.residual + (size_t)t0 * N * os;
+        matmul_epilogue_any_kernel<<<dim3((N - 1) / 8 + 1, std::min(T - t0, 65535u)), 256, 0, ctx->stream>>>(
+            (const char *)x + (size_t)t0 * K * xs, x_dtype, (const __nv_bfloat16 *)w, N, K, part, (char *)out + (size_t)t0 * N * os);
+        ctx->launches++;
+        ctx->last_launch = yx_ctx::LAST_OTHER;
+        if (int rc = check_cuda(ctx, cudaGetLastError(), "matmul kernel (any shape)")) return rc;
+    }
+    return YX_OK;
+}
+
+}  // namespace
+}  // namespace yx
+
+using namespace yx;
+
+extern "C" {
+
+int yx_matmul_epilogue(yx_ctx *ctx, const void *x_dev, int x_dtype, const void *w_bf16_dev, const float *bias_dev, int activation,
+                       const void *residual_dev, uint32_t rows, uint32_t n, uint32_t k, void *out_dev, int out_dtype) {
+    if (!ctx) return YX_ERR_INVALID;
+    if (ctx->status != YX_OK) return ctx->status;
+    if (!valid(x_dtype) || !valid(out_dtype)) return fail(ctx, YX_ERR_INVALID, "matmul_epilogue: bad dtype");
+    if (activation < YX_ACT_NONE || activation > YX_ACT_SILU) return fail(ctx, YX_ERR_INVALID, "matmul_epilogue: unknown activation");
+    if (rows == 0 || n == 0) return YX_OK;
+    if (!x_dev || !w_bf16_dev || !out_dev || k == 0) return fail(ctx, YX_ERR_INVALID, "matmul_epilogue: null tensor or empty inner dimension");
+    if (!aligned(x_dev, size_of(x_dtype)) || !aligned(w_bf16_dev, 2) || !aligned(bias_dev, 4) || !aligned(residual_dev, size_of(out_dtype)) ||
+        !aligned(out_dev, size_of(out_dtype)))
+        return fail(ctx, YX_ERR_INVALID, "matmul_epilogue: a tensor off its type's alignment");
+    const size_t x_bytes = (size_t)rows * k * size_of(x_dtype), out_bytes = (size_t)rows * n * size_of(out_dtype);
+    if (overlap(out_dev, out_bytes, w_bf16_dev, (size_t)n * k * 2) || overlap(out_dev, out_bytes, bias_dev, (size_t)n * 4))
+        return fail(ctx, YX_ERR_INVALID, "matmul_epilogue: the result lies over the weight or the bias");
+    if (out_dev != residual_dev && overlap(out_dev, out_bytes, residual_dev, out_bytes))
+        return fail(ctx, YX_ERR_INVALID, "matmul_epilogue: the result lies over part of the residual");
+    Guard guard(ctx->device);
+    // Other CTAs still read the rows when a result is written: a result over its own rows takes them from a copy.
+    if (overlap(out_dev, out_bytes, x_dev, x_bytes)) {
+        if (int rc = grow(ctx, ctx->ep_rows, x_bytes)) return rc;
+        if (int rc = check_cuda(ctx, cudaMemcpyAsync(ctx->ep_rows.dev, x_dev, x_bytes, cudaMemcpyDeviceToDevice, ctx->stream), "matmul_epilogue: rows under the result"))
+            return rc;
+        x_dev = ctx->ep_rows.dev;
+    }
+    const Epilogue e{bias_dev, residual_dev, activation, out_dtype};
+    return matmul_any(ctx, x_dev, x_dtype, w_bf16_dev, rows, n, k, e, out_dev);
+}
+
+int yx_matmul_logprobs(yx_ctx *ctx, const void *x_dev, int x_dtype, const void *w_bf16_dev, uint32_t rows, uint32_t n, uint32_t k,
+                       const uint32_t *ids_host, float *logprob_dev, float *entropy_dev) {
+    if (!ctx) return YX_ERR_INVALID;
+    if (ctx->status != YX_OK) return ctx->status;
+    if (!valid(x_dtype)) return fail(ctx, YX_ERR_INVALID, "matmul_logprobs: bad dtype");
+    if (rows == 0) return YX_OK;
+    if (!x_dev || !w_bf16_dev || !ids_host || !logprob_dev || n == 0 || k == 0)
+        return fail(ctx, YX_ERR_INVALID, "matmul_logprobs: null tensor, no columns or empty inner dimension");
+    if (!aligned(x_dev, size_of(x_dtype)) || !aligned(w_bf16_dev, 2) || !aligned(logprob_dev, 4) || !aligned(entropy_dev, 4))
+        return fail(ctx, YX_ERR_INVALID, "matmul_logprobs: a tensor off its type's alignment");
+    for (uint32_t r = 0; r < rows; r++)
+        if (ids_host[r] >= n) return fail(ctx, YX_ERR_INVALID, "matmul_logprobs: a token id is outside the vocabulary");
+    Guard guard(ctx->device);
+    // Logits of as many rows as 64 MB hold, then their log probabilities.
+    const uint32_t step = (uint32_t)std::max<size_t>(1, std::min<size_t>(rows, ((size_t)64 << 20) / ((size_t)n * 4)));
+    if (int rc = grow(ctx, ctx->lp_logits, (size_t)step * n * 4)) return rc;
+    const Epilogue e{nullptr, nullptr, YX_ACT_NONE, YX_F32};
+    for (uint32_t r = 0; r < rows; r += step) {
+        const uint32_t m = std::min(step, rows - r);
+        if (int rc = matmul_any(ctx, (const char *)x_dev + (size_t)r * k * size_of(x_dtype), x_dtype, w_bf16_dev, m, n, k, e, ctx->lp_logits.dev)) return rc;
+        if (int rc = launch_logprob_rows(ctx, ctx->lp_logits.dev, YX_F32, m, n, n, ids_host + r, 1, 0, logprob_dev + r,
+                                         entropy_dev ? entropy_dev + r : nullptr, nullptr, nullptr))
+            return rc;
+    }
+    return YX_OK;
+}
+
+}  // extern "C"

@@ -358,6 +358,15 @@ struct yx_ctx {
     uint32_t *pick_host = nullptr;         // argmax: the result, pinned and mapped
     size_t pick_cap = 0;                   // rows both are made for
 
+    // The operators behind the hidden states (logprobs.cu, matmul_epi.cu).  Grown by `grow`: buffers that were
+    // outgrown are kept, because a recorded call may still name them.
+    struct Grown {
+        char *dev = nullptr;
+        size_t cap = 0;
+    };
+    Grown lp_ids, lp_logits, ep_rows;      // given tokens; logits of a few rows at a time; pass rows copied or in parts
+    std::vector<void *> outgrown;
+
     // multi-GPU
     ncclComm *comm = nullptr;
     int n_ranks = 1, rank = 0;
@@ -374,11 +383,18 @@ int check_cuda(yx_ctx *ctx, cudaError_t e, const char *what);
 // Stream-ordered upload of `bytes` from pageable host memory through the pinned ring.
 int upload_ordered(yx_ctx *ctx, void *dst_dev, const void *src_host, size_t bytes);
 int ensure_buffer(yx_ctx *ctx, void **buf, size_t *cap, size_t bytes);
+// The same for buffers that recorded calls may name: an outgrown one lives until the context ends, and growing while the
+// stream is being captured is an error of its own instead of a broken capture.
+int grow(yx_ctx *ctx, yx_ctx::Grown &buf, size_t bytes);
 // yx_attend over the keys [key_lo, key_hi) only: what one rank alone has to do for yx_attend_allgather.
 int attend_key_range(yx_ctx *ctx, yx_kv *kv, int layer, const void *q, int q_dtype, int hq, int64_t window, uint64_t key_lo,
                      uint64_t key_hi, void *out, int out_dtype);
 // out = x . w^T on the tensor cores for many rows (matmul_tc.cu says what it takes).
 int launch_matmul_tc(yx_ctx *ctx, const float *x, const void *w, uint32_t T, uint32_t N, uint32_t K, bool glu, float *out);
+
+// The statistics of softmax rows: logprobs.cu.
+int launch_logprob_rows(yx_ctx *ctx, const void *logits, int dtype, uint32_t rows, uint32_t cols, size_t stride, const uint32_t *ids_host,
+                        uint32_t n_ids, uint32_t n_top, float *logprob, float *entropy, uint32_t *top_ids, float *top_logprob);
 
 // Kernel launchers (each returns a yx_error and counts its launches in ctx->launches).
 int launch_append(yx_ctx *ctx, yx_kv *kv, int layer, const void *k_rows, const void *v_rows, int src_dtype);
