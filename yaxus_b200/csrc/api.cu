@@ -56,7 +56,7 @@ int grow(yx_ctx *ctx, yx_ctx::Grown &buf, size_t bytes) {
     if (int rc = check_cuda(ctx, cudaStreamIsCapturing(ctx->stream, &capture), "cudaStreamIsCapturing")) return rc;
     if (capture != cudaStreamCaptureStatusNone)
         return fail(ctx, YX_ERR_STATE, "scratch would have to grow while the stream is being captured: make a call of this size first");
-    const size_t want = std::max<size_t>(bytes + bytes / 2, 4096);
+    const size_t want = std::max<size_t>(buf.dev ? bytes + bytes / 2 : bytes, 4096);
     void *p = nullptr;
     if (int rc = check_cuda(ctx, cudaMalloc(&p, want), "cudaMalloc (workspace)")) return rc;
     try {
@@ -140,6 +140,7 @@ int fold_device_status(yx_ctx *ctx) {
         // A kernel that gave up may have left arrival counters (fused merge, shared matmul tiles) non-zero.
         if (ctx->counters) cudaMemsetAsync(ctx->counters, 0, ctx->counters_cap, ctx->stream);
         if (ctx->mm_counters) cudaMemsetAsync(ctx->mm_counters, 0, ctx->mm_counters_cap, ctx->stream);
+        if (ctx->ep_counters.dev) cudaMemsetAsync(ctx->ep_counters.dev, 0, ctx->ep_counters.cap, ctx->stream);
         return fail(ctx, YX_ERR_DEVICE,
                     "a kernel reported a failed check: code " + std::to_string(s.code) + " at " +
                         std::to_string(s.where) + " (" + std::to_string(s.a) + ", " + std::to_string(s.b) + ")" +
@@ -622,7 +623,7 @@ void yx_ctx_destroy(yx_ctx *ctx) {
     if (ctx->idx_dev) cudaFree(ctx->idx_dev);
     if (ctx->pick_counters) cudaFree(ctx->pick_counters);
     if (ctx->pick_host) cudaFreeHost(ctx->pick_host);
-    for (yx_ctx::Grown *b : {&ctx->lp_ids, &ctx->lp_logits, &ctx->ep_rows})
+    for (yx_ctx::Grown *b : {&ctx->lp_ids, &ctx->lp_logits, &ctx->lp_stats, &ctx->ep_rows, &ctx->ep_part, &ctx->ep_counters})
         if (b->dev) cudaFree(b->dev);
     for (void *p : ctx->outgrown) cudaFree(p);
     if (ctx->gather_buf) cudaFree(ctx->gather_buf);

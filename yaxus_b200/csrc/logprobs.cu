@@ -33,6 +33,13 @@ __device__ __forceinline__ float key_logit(uint64_t k) {
     return __uint_as_float(b & 0x80000000u ? b & 0x7fffffffu : ~b);
 }
 
+__device__ __forceinline__ RowStats merge_warp(RowStats r) {
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1)
+        r = merge(r, RowStats{__shfl_xor_sync(0xffffffffu, r.m, d), __shfl_xor_sync(0xffffffffu, r.s, d), __shfl_xor_sync(0xffffffffu, r.t, d)});
+    return r;
+}
+
 struct RowsArgs {
     const void *logits;
     int dtype;
@@ -53,9 +60,7 @@ __global__ void __launch_bounds__(256) logprob_rows_kernel(const RowsArgs a) {
     const size_t row = blockIdx.x, base = row * a.stride;
     RowStats r = no_stats();
     for (uint32_t c = threadIdx.x; c < a.cols; c += blockDim.x) r = merge(r, RowStats{clean(load_as_f32(a.logits, a.dtype, base + c)), 1.0f, 0.0f});
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1)
-        r = merge(r, RowStats{__shfl_xor_sync(0xffffffffu, r.m, d), __shfl_xor_sync(0xffffffffu, r.s, d), __shfl_xor_sync(0xffffffffu, r.t, d)});
+    r = merge_warp(r);
     if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = r;
     __syncthreads();
     r = part[0];
@@ -84,6 +89,28 @@ __global__ void __launch_bounds__(256) logprob_rows_kernel(const RowsArgs a) {
     }
 }
 
+// The statistics of a row's blocks of columns, merged; one CTA a row.
+__global__ void __launch_bounds__(128) logprob_blocks_kernel(const float4 *__restrict__ stats, uint32_t blocks, const float *__restrict__ picked,
+                                                             float *__restrict__ logprob, float *__restrict__ out_entropy) {
+    __shared__ RowStats part[4];
+    dependent_entry();
+    const size_t row = blockIdx.x;
+    RowStats r = no_stats();
+    for (uint32_t b = threadIdx.x; b < blocks; b += blockDim.x) {
+        const float4 f = stats[row * blocks + b];
+        r = merge(r, RowStats{f.x, f.y, f.z});
+    }
+    r = merge_warp(r);
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = r;
+    __syncthreads();
+    if (threadIdx.x != 0) return;
+    r = merge(merge(part[0], part[1]), merge(part[2], part[3]));
+    logprob[row] = log_prob(picked[row], r.m, logf(r.s));
+    if (out_entropy) out_entropy[row] = entropy(r);
+}
+
+}  // namespace
+
 int put_ids(yx_ctx *ctx, const uint32_t *host, size_t n, const uint32_t **out) {
     if (int rc = grow(ctx, ctx->lp_ids, n * 4)) return rc;
     *out = (const uint32_t *)ctx->lp_ids.dev;
@@ -97,7 +124,10 @@ int put_ids(yx_ctx *ctx, const uint32_t *host, size_t n, const uint32_t **out) {
     return YX_OK;
 }
 
-}  // namespace
+int launch_logprob_blocks(yx_ctx *ctx, const void *stats, uint32_t blocks, const float *picked, uint32_t rows, float *logprob, float *entropy) {
+    ctx->last_launch = yx_ctx::LAST_OTHER;
+    return launch_dependent(ctx, "logprob_blocks kernel launch", logprob_blocks_kernel, dim3(rows), dim3(128), 0, (const float4 *)stats, blocks, picked, logprob, entropy);
+}
 
 int launch_logprob_rows(yx_ctx *ctx, const void *logits, int dtype, uint32_t rows, uint32_t cols, size_t stride, const uint32_t *ids_host,
                         uint32_t n_ids, uint32_t n_top, float *logprob, float *entropy, uint32_t *top_ids, float *top_logprob) {

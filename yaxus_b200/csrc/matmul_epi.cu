@@ -46,18 +46,30 @@ struct Guard {
     }
 };
 
-int matmul_any(yx_ctx *ctx, const void *x, int x_dtype, const void *w, uint32_t T, uint32_t N, uint32_t K, const Epilogue &e, void *out) {
-    const size_t xs = size_of(x_dtype), os = size_of(e.out_dtype);
-    for (uint32_t t0 = 0; t0 < T; t0 += 65535u) {   // (the y extent's end)
-        Epilogue part = e;
-        if (e.residual) part.residual = (const char *)e.residual + (size_t)t0 * N * os;
-        matmul_epilogue_any_kernel<<<dim3((N - 1) / 8 + 1, std::min(T - t0, 65535u)), 256, 0, ctx->stream>>>(
-            (const char *)x + (size_t)t0 * K * xs, x_dtype, (const __nv_bfloat16 *)w, N, K, part, (char *)out + (size_t)t0 * N * os);
+int matmul_any(yx_ctx *ctx, const Product &p, int x_dtype) {
+    const size_t xs = size_of(x_dtype), os = size_of(p.e.out_dtype);
+    for (uint32_t t0 = 0; t0 < p.T; t0 += 65535u) {   // (the y extent's end)
+        Epilogue e = p.e;
+        if (e.residual) e.residual = (const char *)e.residual + (size_t)t0 * p.N * os;
+        matmul_epilogue_any_kernel<<<dim3((p.N - 1) / 8 + 1, std::min(p.T - t0, 65535u)), 256, 0, ctx->stream>>>(
+            (const char *)p.x + (size_t)t0 * p.K * xs, x_dtype, (const __nv_bfloat16 *)p.w, p.N, p.K, e, (char *)p.out + (size_t)t0 * p.N * os);
         ctx->launches++;
         ctx->last_launch = yx_ctx::LAST_OTHER;
         if (int rc = check_cuda(ctx, cudaGetLastError(), "matmul kernel (any shape)")) return rc;
     }
     return YX_OK;
+}
+
+Product product(const void *x, int x_dtype, const void *w, uint32_t T, uint32_t N, uint32_t K) {
+    Product p{};
+    p.x = x;
+    p.w = w;
+    p.T = T;
+    p.N = N;
+    p.K = K;
+    p.parts = x_dtype == YX_BF16 ? 1 : x_dtype == YX_F16 ? 2 : 3;
+    p.e.out_dtype = YX_F32;
+    return p;
 }
 
 }  // namespace
@@ -84,15 +96,19 @@ int yx_matmul_epilogue(yx_ctx *ctx, const void *x_dev, int x_dtype, const void *
     if (out_dev != residual_dev && overlap(out_dev, out_bytes, residual_dev, out_bytes))
         return fail(ctx, YX_ERR_INVALID, "matmul_epilogue: the result lies over part of the residual");
     Guard guard(ctx->device);
+    Product p = product(x_dev, x_dtype, w_bf16_dev, rows, n, k);
+    p.out = out_dev;
+    p.e = Epilogue{bias_dev, residual_dev, activation, out_dtype};
+    const bool tensor = exact_tc_takes(p);
     // Other CTAs still read the rows when a result is written: a result over its own rows takes them from a copy.
-    if (overlap(out_dev, out_bytes, x_dev, x_bytes)) {
+    if ((!tensor || exact_tc_reads_rows_late(p)) && overlap(out_dev, out_bytes, x_dev, x_bytes)) {
         if (int rc = grow(ctx, ctx->ep_rows, x_bytes)) return rc;
         if (int rc = check_cuda(ctx, cudaMemcpyAsync(ctx->ep_rows.dev, x_dev, x_bytes, cudaMemcpyDeviceToDevice, ctx->stream), "matmul_epilogue: rows under the result"))
             return rc;
-        x_dev = ctx->ep_rows.dev;
+        ctx->last_launch = yx_ctx::LAST_OTHER;
+        p.x = ctx->ep_rows.dev;
     }
-    const Epilogue e{bias_dev, residual_dev, activation, out_dtype};
-    return matmul_any(ctx, x_dev, x_dtype, w_bf16_dev, rows, n, k, e, out_dev);
+    return tensor ? launch_matmul_epilogue_tc(ctx, p) : matmul_any(ctx, p, x_dtype);
 }
 
 int yx_matmul_logprobs(yx_ctx *ctx, const void *x_dev, int x_dtype, const void *w_bf16_dev, uint32_t rows, uint32_t n, uint32_t k,
@@ -108,15 +124,30 @@ int yx_matmul_logprobs(yx_ctx *ctx, const void *x_dev, int x_dtype, const void *
     for (uint32_t r = 0; r < rows; r++)
         if (ids_host[r] >= n) return fail(ctx, YX_ERR_INVALID, "matmul_logprobs: a token id is outside the vocabulary");
     Guard guard(ctx->device);
+    Product p = product(x_dev, x_dtype, w_bf16_dev, rows, n, k);
+    if (exact_tc_takes(p)) {
+        p.blocks = logprobs_block(p);
+        // (the statistics, then the given tokens' logits)
+        const size_t stats = (size_t)rows * p.blocks * 16;
+        if (int rc = grow(ctx, ctx->lp_stats, stats + (size_t)rows * 4)) return rc;
+        p.stats = ctx->lp_stats.dev;
+        p.picked = (float *)(ctx->lp_stats.dev + stats);
+        p.ids_host = ids_host;
+        if (rows > 32)
+            if (int rc = put_ids(ctx, ids_host, rows, &p.ids_dev)) return rc;
+        if (int rc = launch_matmul_logprobs_tc(ctx, p)) return rc;
+        return launch_logprob_blocks(ctx, p.stats, p.blocks, p.picked, rows, logprob_dev, entropy_dev);
+    }
     // Logits of as many rows as 64 MB hold, then their log probabilities.
     const uint32_t step = (uint32_t)std::max<size_t>(1, std::min<size_t>(rows, ((size_t)64 << 20) / ((size_t)n * 4)));
     if (int rc = grow(ctx, ctx->lp_logits, (size_t)step * n * 4)) return rc;
-    const Epilogue e{nullptr, nullptr, YX_ACT_NONE, YX_F32};
+    p.out = ctx->lp_logits.dev;
     for (uint32_t r = 0; r < rows; r += step) {
-        const uint32_t m = std::min(step, rows - r);
-        if (int rc = matmul_any(ctx, (const char *)x_dev + (size_t)r * k * size_of(x_dtype), x_dtype, w_bf16_dev, m, n, k, e, ctx->lp_logits.dev)) return rc;
-        if (int rc = launch_logprob_rows(ctx, ctx->lp_logits.dev, YX_F32, m, n, n, ids_host + r, 1, 0, logprob_dev + r,
-                                         entropy_dev ? entropy_dev + r : nullptr, nullptr, nullptr))
+        p.x = (const char *)x_dev + (size_t)r * k * size_of(x_dtype);
+        p.T = std::min(step, rows - r);
+        if (int rc = matmul_any(ctx, p, x_dtype)) return rc;
+        if (int rc = launch_logprob_rows(ctx, p.out, YX_F32, p.T, n, n, ids_host + r, 1, 0, logprob_dev + r, entropy_dev ? entropy_dev + r : nullptr,
+                                         nullptr, nullptr))
             return rc;
     }
     return YX_OK;

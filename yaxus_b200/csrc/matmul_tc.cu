@@ -29,6 +29,7 @@
 
 #include <algorithm>
 
+#include "yx_epilogue.cuh"
 #include "yx_tcgen05.cuh"
 
 namespace yx {
@@ -59,10 +60,29 @@ constexpr uint32_t TC_SMEM_BUDGET = 220 * 1024;
 // 80 rows pays 19 us of 399 for chains of eight in place of 16.
 constexpr uint32_t TC_CHAIN = 16, TC_FIRST_CHAIN = 32, TC_SHORT_CHAIN = 8, TC_CUT_CHAIN = 6, TC_LEAST_CHAIN = 4;
 constexpr int TC_MAX_BUFS = 4;
+// The same for rows taken exactly (EPILOGUE, LOGPROBS), by their parts, and for results of 16 bits, which keep none of it.
+constexpr uint32_t EXACT_CHAIN[3] = {12, 6, 3}, NARROW_CHAIN = 32;
 constexpr uint32_t GLU_GROUP = 16;          // gate and up rows alternate in a tile sixteen by sixteen: a warp holds both
+
+// What becomes of a product.
+//  PLAIN, GLU: f32 rows in two bf16 parts (yx_matmul, yx_matmul_glu).
+//  EPILOGUE: bias, activation and residual; LOGPROBS: softmax statistics of 128 columns at a time.  Both take the rows exactly, in
+//  as many bf16 parts as their type has bits for: bf16 one, f16 (11 bits) two, f32 (24 bits) three.
+enum Kind { PLAIN, GLU, EPILOGUE, LOGPROBS };
+constexpr int kind_parts(int kind, int parts) { return kind < EPILOGUE ? 2 : parts; }
+
+// Where the LOGPROBS kinds leave the statistics of a pass row t over 128 columns: [T][blocks] of (m, s, t, -), and the
+// logit of the row's given token.
+struct StatsOut {
+    float4 *stats;
+    uint32_t blocks;
+    float *picked;          // [T]
+};
 
 struct PairArgs {
     uint32_t T, cols;                 // pass rows; columns of the result
+    uint32_t parts;                   // bf16 parts of a pass row (EPILOGUE, LOGPROBS)
+    bool early_w;                     // what wrote the weights is complete when this kernel starts
     uint32_t bt, t_tiles;             // pass rows of a tile (multiple of 32), tiles of them
     uint32_t ksteps;
     uint32_t pairs;                   // CTA pairs of the grid
@@ -72,6 +92,9 @@ struct PairArgs {
     uint32_t bufs, buf_columns;       // accumulators in tensor memory
     uint32_t chain, long_first;       // k steps summed in one of them; whether a piece begins with more
     float *out;
+    Epilogue e;                       // EPILOGUE (`out` is of its type)
+    StatsOut so;                      // LOGPROBS
+    const uint32_t *ids;              // LOGPROBS: given tokens [T]
     float *part;                      // [2 * rest_pairs shares][2 CTAs][bt][128]
     uint32_t *counters;               // [tiles left over][2 CTAs], zero between launches
     yx_dev_status *status;
@@ -141,6 +164,103 @@ __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
 }
 
+// N results of this lane's column, pass rows from t0 on: bias, activation, residual.
+template <int N>
+__device__ __forceinline__ void finish_rows(const Epilogue &e, void *out, uint32_t T, uint32_t cols, const float (&v)[N], uint32_t t0, uint32_t col) {
+    if (col >= cols) return;
+    const float bias = e.bias ? e.bias[col] : 0.0f;
+    constexpr int H = N < 16 ? N : 16;   // (residuals in flight)
+#pragma unroll
+    for (int h = 0; h < N; h += H) {
+        const size_t at = (size_t)(t0 + h) * cols + col;
+        float y[H], r[H];
+        if (e.residual) {
+#pragma unroll
+            for (int i = 0; i < H; i++) r[i] = t0 + h + i < T ? load_as_f32(e.residual, e.out_dtype, at + (size_t)i * cols) : 0.0f;
+        }
+#pragma unroll
+        for (int i = 0; i < H; i++) y[i] = v[h + i] + bias;
+        if (e.act != YX_ACT_NONE) {
+#pragma unroll
+            for (int i = 0; i < H; i += 4) *(float4 *)(y + i) = activate4(make_float4(y[i], y[i + 1], y[i + 2], y[i + 3]), e.act);
+        }
+        if (e.residual) {
+#pragma unroll
+            for (int i = 0; i < H; i++) y[i] += r[i];
+        }
+#pragma unroll
+        for (int i = 0; i < H; i++)
+            if (t0 + h + i < T) store_from_f32(out, e.out_dtype, at + (size_t)i * cols, y[i]);
+    }
+}
+
+// ---- softmax statistics of a warp's 32 columns for each of its pass rows --------------------------------
+//
+// A lane holds a column; the sums run over columns.  Sixteen pass rows at a time change places with the columns
+// through 2 KiB of shared memory (16-byte chunks of a pass row's 128 bytes at chunk ^ (row & 7): no bank is met twice
+// either way), after which a lane has half a pass row's columns: 2.5 shared-memory accesses for a logit's eight or so
+// instructions, where summing across lanes would take three shuffles for each.
+constexpr int STATS_SCRATCH = 16 * 32;   // floats a warp
+
+// Statistics of pass rows 0..15 of v over this warp's 32 columns, in lanes r and r + 16 for row r.  `want`: the row's given
+// token, counted from the warp's first column (past 31: not here); `logit`: set to its logit.
+template <int N>
+__device__ __forceinline__ RowStats stats_of_16(const float (&v)[N], int first, bool column, float *scratch, int lane, uint32_t want, float &logit) {
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < (N < 16 ? N : 16); i++) scratch[i * 32 + (((lane >> 2) ^ (i & 7)) << 2) + (lane & 3)] = column ? v[first + i] : -INFINITY;
+    __syncwarp();
+    const int r = lane & 15;
+    float q[16];
+#pragma unroll
+    for (int c = 0; c < 4; c++) *(float4 *)(q + 4 * c) = *(const float4 *)(scratch + r * 32 + ((((lane >> 4) * 4 + c) ^ (r & 7)) << 2));
+    if (want < 32u) logit = scratch[r * 32 + (((want >> 2) ^ (r & 7)) << 2) + (want & 3)];
+    RowStats st{q[0], 0.0f, 0.0f};
+#pragma unroll
+    for (int i = 1; i < 16; i++) st.m = fmaxf(st.m, q[i]);
+    if (!(st.m < INFINITY)) {   // an infinity (or nothing but no numbers)
+#pragma unroll
+        for (int i = 0; i < 16; i++) q[i] = clean(q[i]);
+        st.m = clean(st.m);
+    }
+#pragma unroll
+    for (int i = 0; i < 16; i++) {
+        const float d = distance(q[i], st.m), e = fast_exp2(d * LOG2_E);
+        st.s += e;
+        st.t += e * d;
+    }
+    return merge(st, RowStats{__shfl_xor_sync(0xffffffffu, st.m, 16), __shfl_xor_sync(0xffffffffu, st.s, 16), __shfl_xor_sync(0xffffffffu, st.t, 16)});
+}
+
+// Up to 32 pass rows from t0 on: each warp's 32 columns, then the four warps of a barrier together.  `turn` counts the
+// group's calls: the warps' results go to two buffers in turn, so that one barrier a call is enough.  Warp `turn` mod
+// four merges and writes.
+template <int N>
+__device__ __forceinline__ void stats_rows(const StatsOut &so, uint32_t T, uint32_t cols, const float (&v)[N], uint32_t t0, uint32_t row, uint32_t block,
+                                           const uint32_t *ids, float *scratch, float4 (*results)[4][32], uint32_t &turn, int barrier, int warp, int lane) {
+    const uint32_t t = t0 + lane;
+    const uint32_t want = lane < N && t < T ? ids[t] - (row - lane) : 0xffffffffu;
+    float logit = 0.0f;
+    RowStats st = stats_of_16(v, 0, row < cols, scratch, lane, lane < 16 ? want : 0xffffffffu, logit);
+    if constexpr (N > 16) {
+        const RowStats hi = stats_of_16(v, 16, row < cols, scratch, lane, lane < 16 ? 0xffffffffu : want, logit);
+        if (lane >= 16) st = hi;
+    }
+    if (want < 32u) so.picked[t] = logit;
+    results[turn & 1][warp & 3][lane] = make_float4(st.m, st.s, st.t, 0.0f);
+    asm volatile("bar.sync %0, 128;" ::"r"(barrier) : "memory");
+    if ((turn & 3) == (uint32_t)(warp & 3) && lane < N && t < T) {
+        RowStats all = no_stats();
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float4 f = results[turn & 1][i][lane];
+            all = merge(all, RowStats{f.x, f.y, f.z});
+        }
+        so.stats[(size_t)t * so.blocks + block] = make_float4(all.m, all.s, all.t, 0.0f);
+    }
+    turn++;
+}
+
 // 32 pass rows from `t0` on of this lane's weight row.
 template <bool GLU>
 __device__ __forceinline__ void store_rows(const PairArgs &a, const float (&v)[32], uint32_t t0, uint32_t row, int lane) {
@@ -172,7 +292,7 @@ __device__ __forceinline__ void store_rows(const PairArgs &a, const float (&v)[3
 // CHUNKS: 64-row chunks of a tile, what an epilogue thread keeps in registers (two for up to
 // 128 pass rows, three for up to 192: before the chains of eight above, steps of 80 and of 311 rows took 391 and 453 us with
 // room for four, 382 and 437 so; with them 399 and 440).
-template <bool GLU, int CHUNKS>
+template <int KIND, int CHUNKS>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TC_THREADS, 1)
 matmul_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap x_map, const PairArgs a) {
     extern __shared__ __align__(1024) unsigned char smem[];
@@ -180,9 +300,12 @@ matmul_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_const
     __shared__ uint32_t tmem_base_s;
     __shared__ int abort_flag;
     __shared__ int last_s;
+    __shared__ __align__(16) float stats_scratch[KIND == LOGPROBS ? 8 * STATS_SCRATCH : 4];
+    __shared__ float4 stats_results[KIND == LOGPROBS ? 2 : 1][2][4][KIND == LOGPROBS ? 32 : 1];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = blockIdx.x & 1u, pair = blockIdx.x >> 1;
-    const uint32_t S = a.stages, x_bytes = a.bt * 128u, stage_bytes = W_BYTES + x_bytes;   // x: bt / 2 rows, high and low part
+    const uint32_t parts = KIND < EPILOGUE ? 2u : a.parts;
+    const uint32_t S = a.stages, x_bytes = parts * a.bt * 64u, stage_bytes = W_BYTES + x_bytes;   // x: bt / 2 rows, the high part first
     const uint32_t base = smem_u32(smem);
     const uint32_t b_full = smem_u32(bar_store), b_empty = b_full + 8 * TC_MAX_STAGES;
     const uint32_t b_acc_full = b_empty + 8 * TC_MAX_STAGES, b_acc_empty = b_acc_full + 8 * TC_MAX_BUFS;
@@ -220,7 +343,7 @@ matmul_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_const
         auto load_w = [&](uint32_t s, const Piece &p, uint32_t k) {
             const uint32_t m0 = (p.tile / a.t_tiles) * TC_M + rank * 128u;
             if (rank == 0) mbar_expect_tx(b_full + 8 * s, 2 * stage_bytes);
-            tma_load_4d_pair(base + s * stage_bytes, &w_map, (int)(k * TC_KSTEP), GLU ? 0 : (int)m0, 0, GLU ? (int)(m0 / (2 * GLU_GROUP)) : 0,
+            tma_load_4d_pair(base + s * stage_bytes, &w_map, (int)(k * TC_KSTEP), KIND == GLU ? 0 : (int)m0, 0, KIND == GLU ? (int)(m0 / (2 * GLU_GROUP)) : 0,
                              full0 + 8 * s);
         };
         auto load_x = [&](uint32_t s, const Piece &p, uint32_t k) {
@@ -228,9 +351,10 @@ matmul_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_const
             tma_load_3d_pair(base + s * stage_bytes + W_BYTES, &x_map, (int)(k * TC_KSTEP), (int)t0, 0, full0 + 8 * s);
         };
         // The kernel ahead (the split of the activations) let this one start only after its own wait, so nothing
-        // that may still run writes the weights: the ring's first weights are on their way before the wait.
+        // that may still run writes the weights: the ring's first weights are on their way before the wait.  (Rows that are
+        // bf16 already have no split ahead of them.)
         uint32_t ahead = 0;
-        {
+        if (KIND < EPILOGUE || a.early_w) {
             Walk walk(a, pair);
             Piece p;
             while (ahead < S && walk.next(a, pair, p))
@@ -272,11 +396,14 @@ matmul_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_const
                     mbar_wait(b_full + 8 * s, phase, abortp, a.status, 503);
                     if (*abortp) break;
                     tc_fence_after();
-                    const uint32_t w_lo = desc_lo(base + s * stage_bytes, 0), h_lo = w_lo + W_BYTES / 16, l_lo = h_lo + x_bytes / 32;
+                    const uint32_t w_lo = desc_lo(base + s * stage_bytes, 0), h_lo = w_lo + W_BYTES / 16;
 #pragma unroll
                     for (uint32_t kk = 0; kk < 4; kk++) umma2_ss_lo(acc, w_lo + 2 * kk, h_lo + 2 * kk, idesc, k > k0 || kk > 0);
+                    for (uint32_t part = 1; part < parts; part++) {
+                        const uint32_t l_lo = h_lo + part * (a.bt * 4u);
 #pragma unroll
-                    for (uint32_t kk = 0; kk < 4; kk++) umma2_ss_lo(acc, w_lo + 2 * kk, l_lo + 2 * kk, idesc, 1);
+                        for (uint32_t kk = 0; kk < 4; kk++) umma2_ss_lo(acc, w_lo + 2 * kk, l_lo + 2 * kk, idesc, 1);
+                    }
                     umma2_commit(b_empty + 8 * s);
                     if (++s == S) {
                         s = 0;
@@ -292,6 +419,14 @@ matmul_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_const
         Walk walk(a, pair);
         Piece p;
         AccTurn turn;
+        uint32_t stats_turn = 0;
+        auto finish = [&](const float (&v)[32], uint32_t t, uint32_t row) {
+            if constexpr (KIND < EPILOGUE) store_rows<KIND == GLU>(a, v, t, row, lane);
+            else if constexpr (KIND == EPILOGUE) finish_rows(a.e, a.out, a.T, a.cols, v, t, row);
+            else
+                stats_rows(a.so, a.T, a.cols, v, t, row, row >> 7, a.ids, stats_scratch + warp * STATS_SCRATCH, stats_results[warp >> 2], stats_turn, 2 + (warp >> 2),
+                           warp, lane);
+        };
         while (walk.next(a, pair, p)) {
             const uint32_t wr = (warp & 3) * 32 + lane;   // weight row of this CTA's 128
             const uint32_t row = (p.tile / a.t_tiles) * TC_M + rank * 128u + wr, t0 = (p.tile % a.t_tiles) * a.bt;
@@ -340,7 +475,7 @@ matmul_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_const
                 const uint32_t c = c0 + 64 * j;
                 if (c >= a.bt) break;
                 if (p.whole) {
-                    store_rows<GLU>(a, sum[j], t0 + c, row, lane);
+                    finish(sum[j], t0 + c, row);
                 } else {
                     float4 *mine = share(pair) + c / 4 * 128u;
 #pragma unroll
@@ -388,7 +523,7 @@ matmul_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_const
 #pragma unroll
                     for (int i = 0; i < 4; i++) *(float4 *)(v + 16 * h + 4 * i) = sum[i];
                 }
-                store_rows<GLU>(a, v, t0 + c, row, lane);
+                finish(v, t0 + c, row);
             }
         }
     }
@@ -427,6 +562,67 @@ __global__ void __launch_bounds__(256) split_rows_kernel(const float *__restrict
     lo[idx] = make_uint4(l[0], l[1], l[2], l[3]);
 }
 
+// The bf16 parts of eight f32 or f16 values, largest first, cut off and not rounded: each part takes the next eight bits, so
+// that PARTS of them are the value itself, and a value above the largest bf16 stays finite.
+template <int PARTS>
+__device__ __forceinline__ void cut_parts(const float (&v)[8], uint32_t (&out)[PARTS][4]) {
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        float a = v[2 * j], b = v[2 * j + 1];
+#pragma unroll
+        for (int p = 0; p < PARTS; p++) {
+            const uint32_t ha = __float_as_uint(a) & 0xffff0000u, hb = __float_as_uint(b) & 0xffff0000u;
+            out[p][j] = ha >> 16 | hb;
+            a -= __uint_as_float(ha);
+            b -= __uint_as_float(hb);
+        }
+        // What is no number, or infinite, is so in its first part alone (the bits cut off might be all that told the two
+        // apart, and infinity less itself is no number).
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const uint32_t x = __float_as_uint(v[2 * j + i]), shift = 16 * i;
+            if ((x & 0x7f800000u) != 0x7f800000u) continue;
+            const uint32_t first = (x & 0x7fffffu ? 0x7fc0u : x >> 16) << shift;
+            out[0][j] = (out[0][j] & ~(0xffffu << shift)) | first;
+#pragma unroll
+            for (int p = 1; p < PARTS; p++) out[p][j] &= ~(0xffffu << shift);
+        }
+    }
+}
+// Eight consecutive elements, at an address of 16 bytes' alignment where VEC says so, as f32.
+template <int DTYPE, bool VEC>
+__device__ __forceinline__ void load8(const void *base, size_t at, float (&v)[8]) {
+    if constexpr (!VEC) {
+#pragma unroll
+        for (int j = 0; j < 8; j++) v[j] = load_as_f32(base, DTYPE, at + j);
+    } else if constexpr (DTYPE == YX_F32) {
+        *(float4 *)v = *(const float4 *)((const float *)base + at);
+        *(float4 *)(v + 4) = *(const float4 *)((const float *)base + at + 4);
+    } else {
+        const uint4 u = *(const uint4 *)((const uint16_t *)base + at);
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const float2 f = unpack2<DTYPE == YX_BF16>(w[j]);
+            v[2 * j] = f.x;
+            v[2 * j + 1] = f.y;
+        }
+    }
+}
+// x [n] -> its PARTS bf16 parts, [PARTS][n]; eight elements a thread (n is a multiple of eight).
+template <int DTYPE, int PARTS, bool VEC>
+__global__ void __launch_bounds__(256) cut_rows_kernel(const void *__restrict__ x, size_t n, uint4 *__restrict__ out) {
+    dependent_entry();
+    const size_t idx = (size_t)blockIdx.x * blockDim.x + threadIdx.x;
+    if (idx * 8 >= n) return;
+    float v[8];
+    load8<DTYPE, VEC>(x, idx * 8, v);
+    uint32_t parts[PARTS][4];
+    cut_parts<PARTS>(v, parts);
+#pragma unroll
+    for (int p = 0; p < PARTS; p++) out[p * (n / 8) + idx] = make_uint4(parts[p][0], parts[p][1], parts[p][2], parts[p][3]);
+}
+
 // ---- passes of few rows ------------------------------------------------------------------------------------
 //
 // At most 32 pass rows: the weights stream through the chip once and everything else must stay out of their way.
@@ -455,10 +651,13 @@ constexpr uint32_t ROWS_MAX = 32;           // pass rows
 constexpr uint32_t ROWS_CHAIN = 8, ROWS_BUFS = 4;   // (and four accumulators: the tensor cores run on while an epilogue adds shares up)
 
 struct RowsArgs {
-    const float *x;
+    const void *x;
     uint32_t T, K, cols, ksteps, units, ctas, stages;
     uint32_t x_vec16;
     float *out;
+    Epilogue e;                       // EPILOGUE (`out` is of its type)
+    StatsOut so;                      // LOGPROBS
+    uint32_t ids[ROWS_MAX];           // LOGPROBS: given tokens
     float *part;          // [2 * ctas shares][TP][128]
     uint32_t *counters;   // one a tile, zero between launches
     yx_dev_status *status;
@@ -486,7 +685,16 @@ __device__ __forceinline__ void store_few(const RowsArgs &a, const float (&v)[TP
     }
 }
 
-template <int TP, bool GLU>
+// Accumulator columns of a k step's products: PARTS blocks of TP pass rows, in what an MMA of 128 weight rows takes (a
+// multiple of 16), and how far apart the accumulators lie.
+constexpr uint32_t rows_columns(int tp, int parts) { return (uint32_t)(tp * parts + 15) / 16 * 16; }
+constexpr uint32_t rows_pitch(int tp, int parts) {
+    uint32_t c = 16;
+    while (c < rows_columns(tp, parts)) c *= 2;
+    return c;
+}
+
+template <int TP, int KIND, int PARTS>
 __global__ void __launch_bounds__(ROWS_THREADS, 1)
 matmul_rows_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ RowsArgs a) {
     extern __shared__ __align__(1024) unsigned char smem[];
@@ -494,8 +702,11 @@ matmul_rows_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_const
     __shared__ uint32_t tmem_base_s;
     __shared__ int abort_flag;
     __shared__ int last_s;
-    constexpr uint32_t NB = 2 * TP, X_BYTES = NB * 128, STAGE = W_BYTES + X_BYTES;
-    constexpr uint32_t TMEM = ROWS_BUFS * NB;
+    constexpr bool GLU_TILES = KIND == GLU;
+    constexpr uint32_t NB = rows_columns(TP, PARTS), PITCH = rows_pitch(TP, PARTS), X_BYTES = NB * 128, STAGE = W_BYTES + X_BYTES;
+    constexpr uint32_t TMEM = ROWS_BUFS * PITCH;
+    __shared__ __align__(16) float stats_scratch[KIND == LOGPROBS ? 4 * STATS_SCRATCH : 4];
+    __shared__ float4 stats_results[2][4][KIND == LOGPROBS ? 32 : 1];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t S = a.stages, base = smem_u32(smem);
     const uint32_t b_full = smem_u32(bar_store), b_empty = b_full + 8 * TC_MAX_STAGES;
@@ -506,8 +717,8 @@ matmul_rows_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_const
     auto weight_rows = [&](uint32_t u, int &x, int &y, int &z) {
         const uint32_t tile = u / a.ksteps;
         x = (int)((u - tile * a.ksteps) * TC_KSTEP);
-        y = GLU ? 0 : (int)(tile * ROWS_M);
-        z = GLU ? (int)(tile * (ROWS_M / (2 * GLU_GROUP))) : 0;
+        y = GLU_TILES ? 0 : (int)(tile * ROWS_M);
+        z = GLU_TILES ? (int)(tile * (ROWS_M / (2 * GLU_GROUP))) : 0;
     };
     if (warp == 4 && lane == 0) {
         prefetch_tensormap(&w_map);
@@ -565,7 +776,7 @@ matmul_rows_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_const
             for (uint32_t u = u0; u < u1 && !*abortp; n++) {
                 if (u == piece_end) piece_end = min(u1, (u / a.ksteps + 1) * a.ksteps);
                 const uint32_t end = min(piece_end, u + ROWS_CHAIN);
-                const uint32_t buf = n % ROWS_BUFS, acc = tmem + buf * NB;
+                const uint32_t buf = n % ROWS_BUFS, acc = tmem + buf * PITCH;
                 if (n >= ROWS_BUFS) mbar_wait(b_acc_empty + 8 * buf, (n / ROWS_BUFS - 1) & 1u, abortp, a.status, 512);
                 tc_fence_after();
                 for (uint32_t first = u; u < end; u++) {
@@ -588,20 +799,38 @@ matmul_rows_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_const
         // ---- activations: every eighth step is this warp's ------------------------------------------
         for (uint32_t u = u0 + (uint32_t)(warp - ROWS_CONVERT_WARP); u < u1; u += ROWS_CONVERTERS) {
             const uint32_t it = u - u0, s = it % S, use = it / S;
-            const float *src = a.x + (size_t)(u % a.ksteps) * TC_KSTEP;
+            const uint32_t k = (u % a.ksteps) * TC_KSTEP + (lane & 7) * 8;
             constexpr int R = TP / 4;          // 16-byte operand chunks (eight k of a pass row) a lane
+            uint4 bits[R];                     // bf16 rows are operands as they are
             float v[R][8];
 #pragma unroll
             for (int r = 0; r < R; r++) {
                 const uint32_t t = r * 4 + (lane >> 3);
                 if (t >= a.T) continue;        // (rows past T only reach accumulator columns that nobody reads)
-                const float *p = src + (size_t)t * a.K + (lane & 7) * 8;
-                if (a.x_vec16) {
-                    *(float4 *)&v[r][0] = *(const float4 *)p;
-                    *(float4 *)&v[r][4] = *(const float4 *)(p + 4);
-                } else {
+                const size_t at = (size_t)t * a.K + k;
+                if constexpr (KIND < EPILOGUE) {
+                    const float *p = (const float *)a.x + at;
+                    if (a.x_vec16) {
+                        *(float4 *)&v[r][0] = *(const float4 *)p;
+                        *(float4 *)&v[r][4] = *(const float4 *)(p + 4);
+                    } else {
 #pragma unroll
-                    for (int j = 0; j < 4; j++) *(float2 *)&v[r][2 * j] = *(const float2 *)(p + 2 * j);
+                        for (int j = 0; j < 4; j++) *(float2 *)&v[r][2 * j] = *(const float2 *)(p + 2 * j);
+                    }
+                } else if (k >= a.K) {         // (K ends inside the step, at a multiple of eight)
+                    bits[r] = make_uint4(0, 0, 0, 0);
+#pragma unroll
+                    for (int j = 0; j < 8; j++) v[r][j] = 0.0f;
+                } else if constexpr (PARTS == 1) {
+                    if (a.x_vec16) {
+                        bits[r] = *(const uint4 *)((const uint16_t *)a.x + at);
+                    } else {
+                        const uint16_t *p = (const uint16_t *)a.x + at;
+                        bits[r] = make_uint4(p[0] | (uint32_t)p[1] << 16, p[2] | (uint32_t)p[3] << 16, p[4] | (uint32_t)p[5] << 16, p[6] | (uint32_t)p[7] << 16);
+                    }
+                } else {
+                    if (a.x_vec16) load8<PARTS == 2 ? YX_F16 : YX_F32, true>(a.x, at, v[r]);
+                    else load8<PARTS == 2 ? YX_F16 : YX_F32, false>(a.x, at, v[r]);
                 }
             }
             if (use > 0) mbar_wait(b_empty + 8 * s, (use - 1) & 1u, abortp, a.status, 514);
@@ -611,16 +840,25 @@ matmul_rows_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_const
             for (int r = 0; r < R; r++) {
                 const uint32_t t = r * 4 + (lane >> 3);
                 if (t >= a.T) continue;
-                uint32_t h[4], l[4];
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    h[j] = pack2<true>(v[r][2 * j], v[r][2 * j + 1]);
-                    const float2 b = unpack2<true>(h[j]);
-                    l[j] = pack2<true>(v[r][2 * j] - b.x, v[r][2 * j + 1] - b.y);
-                }
                 unsigned char *at = dst + t * 128 + (((lane & 7) ^ (t & 7)) << 4);
-                *(uint4 *)at = make_uint4(h[0], h[1], h[2], h[3]);
-                *(uint4 *)(at + TP * 128) = make_uint4(l[0], l[1], l[2], l[3]);
+                if constexpr (KIND < EPILOGUE) {
+                    uint32_t h[4], l[4];
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        h[j] = pack2<true>(v[r][2 * j], v[r][2 * j + 1]);
+                        const float2 b = unpack2<true>(h[j]);
+                        l[j] = pack2<true>(v[r][2 * j] - b.x, v[r][2 * j + 1] - b.y);
+                    }
+                    *(uint4 *)at = make_uint4(h[0], h[1], h[2], h[3]);
+                    *(uint4 *)(at + TP * 128) = make_uint4(l[0], l[1], l[2], l[3]);
+                } else if constexpr (PARTS == 1) {
+                    *(uint4 *)at = bits[r];
+                } else {
+                    uint32_t parts[PARTS][4];
+                    cut_parts<PARTS>(v[r], parts);
+#pragma unroll
+                    for (int p = 0; p < PARTS; p++) *(uint4 *)(at + p * TP * 128) = make_uint4(parts[p][0], parts[p][1], parts[p][2], parts[p][3]);
+                }
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
@@ -628,7 +866,12 @@ matmul_rows_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_const
         }
     } else {
         // ---- epilogue -------------------------------------------------------------------------
-        uint32_t n = 0;
+        uint32_t n = 0, stats_turn = 0;
+        auto finish = [&](const float (&v)[TP], uint32_t row) {
+            if constexpr (KIND < EPILOGUE) store_few<TP, KIND == GLU>(a, v, row, lane);
+            else if constexpr (KIND == EPILOGUE) finish_rows(a.e, a.out, a.T, a.cols, v, 0, row);
+            else stats_rows(a.so, a.T, a.cols, v, 0, row, row >> 7, a.ids, stats_scratch + warp * STATS_SCRATCH, stats_results, stats_turn, 2, warp, lane);
+        };
         for (uint32_t u = u0; u < u1;) {
             const uint32_t tile = u / a.ksteps, end = min(u1, (tile + 1) * a.ksteps);
             const bool whole = end - u == a.ksteps;
@@ -646,11 +889,27 @@ matmul_rows_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_const
             for (int i = 0; i < TP; i++) v[i] = 0.0f;
             for (; u < end; n++) {
                 u = min(end, u + ROWS_CHAIN);
-                const uint32_t buf = n % ROWS_BUFS, acc = tmem + buf * NB + ((uint32_t)warp << 21);
+                const uint32_t buf = n % ROWS_BUFS, acc = tmem + buf * PITCH + ((uint32_t)warp << 21);
                 mbar_wait(b_acc_full + 8 * buf, (n / ROWS_BUFS) & 1u, abortp, a.status, 515);
                 __syncwarp();   // (a wait that ran out does not stop these warps: their barriers below count all of them)
                 tc_fence_after();
-                if constexpr (TP == 8) {
+                if constexpr (PARTS != 2) {
+                    // (the parts' sums one below the other, the smallest first)
+                    float part[TP];
+#pragma unroll
+                    for (int p = PARTS - 1; p >= 0; p--) {
+#pragma unroll
+                        for (int h = 0; h < TP; h += TP < 16 ? TP : 16) {
+                            uint32_t r[16];
+                            tmem_ld16(acc + p * TP + h, r);
+                            tmem_ld_wait();
+#pragma unroll
+                            for (int i = 0; i < (TP < 16 ? TP : 16); i++) part[h + i] = p == PARTS - 1 ? __uint_as_float(r[i]) : part[h + i] + __uint_as_float(r[i]);
+                        }
+                    }
+#pragma unroll
+                    for (int i = 0; i < TP; i++) v[i] += part[i];
+                } else if constexpr (TP == 8) {
                     uint32_t r[16];
                     tmem_ld16(acc, r);
                     tmem_ld_wait();
@@ -672,7 +931,7 @@ matmul_rows_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_const
                 if (lane == 0) mbar_arrive(b_acc_empty + 8 * buf);
             }
             if (whole) {
-                store_few<TP, GLU>(a, v, row, lane);
+                finish(v, row);
                 continue;
             }
             auto share = [&](uint32_t q) { return a.part + (size_t)(2 * q + (q == q0 ? later : 0u)) * TP * 128u + wr; };
@@ -707,7 +966,7 @@ matmul_rows_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_const
 #pragma unroll
                     for (int i = 0; i < TP; i++) v[i] += w[b][i];
             }
-            store_few<TP, GLU>(a, v, row, lane);
+            finish(v, row);
         }
     }
     __syncwarp();
@@ -765,19 +1024,21 @@ int ensure_counters(yx_ctx *ctx, size_t n) {
     return check_cuda(ctx, cudaMemsetAsync(ctx->mm_counters, 0, ctx->mm_counters_cap, ctx->stream), "matmul: counters");
 }
 
+constexpr uint32_t smem_budget(int kind) { return kind == LOGPROBS ? 200 * 1024 : TC_SMEM_BUDGET; }   // (24 KiB change places there)
+
 // CTA pairs that are on the chip together (a GPC with an odd number of SMs leaves one out).
-template <bool GLU, int CHUNKS>
+template <int KIND, int CHUNKS>
 int resident_pairs(yx_ctx *ctx, int *out) {
-    int &n = ctx->mm_pairs[GLU][CHUNKS - 2];
+    int &n = ctx->mm_pairs[KIND][CHUNKS - 2];
     if (n == 0) {
-        auto *kernel = matmul_pair_kernel<GLU, CHUNKS>;
-        if (int rc = check_cuda(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, TC_SMEM_BUDGET),
+        auto *kernel = matmul_pair_kernel<KIND, CHUNKS>;
+        if (int rc = check_cuda(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_budget(KIND)),
                                 "matmul: shared memory attribute"))
             return rc;
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3((unsigned)ctx->sm_count / 2 * 2);
         cfg.blockDim = dim3(TC_THREADS);
-        cfg.dynamicSmemBytes = TC_SMEM_BUDGET;
+        cfg.dynamicSmemBytes = smem_budget(KIND);
         cudaLaunchAttribute attr[1];
         attr[0].id = cudaLaunchAttributeClusterDimension;
         attr[0].val.clusterDim.x = 2;
@@ -803,41 +1064,68 @@ uint32_t tile_rows(uint32_t T) {
 // tile: one more epilogue and one more share to add up for most pairs.  A k step takes 0.26 us and 2 ns a pass row
 // (62 GB/s into each SM, measured at 96 to 256 rows), the extra epilogue 3 us, adding up at all another 6; behind
 // whole rounds both are hidden.  A share of fewer than four k steps costs more to add up than it saves.
-uint32_t share_rest(uint32_t tiles, uint32_t ksteps, uint32_t pairs, uint32_t bt, bool hidden) {
+uint32_t share_rest(uint32_t tiles, uint32_t ksteps, uint32_t pairs, uint32_t bt, bool hidden, float row = 0.002f) {
     const uint32_t most = std::max(1u, ksteps / 4), each = std::min(pairs / tiles, most);
     const uint32_t all = std::min(pairs, tiles * most);
-    const float step = 0.26f + 0.002f * (float)bt, overrun = hidden ? 1.0f : each == 1 ? 9.0f : 3.0f;
+    const float step = 0.26f + row * (float)bt, overrun = hidden ? 1.0f : each == 1 ? 9.0f : 3.0f;
     const float even = step * (float)((ksteps + each - 1) / each), equal = step * (float)(tiles * ksteps) / (float)all;
     return even <= equal + overrun ? tiles * each : all;
 }
 
-template <bool GLU, int CHUNKS>
-int matmul_pair_rows(yx_ctx *ctx, const float *x, const void *w, uint32_t T, uint32_t N, uint32_t K, float *out) {
-    const size_t n = (size_t)T * K;
-    if (int rc = ensure_buffer(ctx, (void **)&ctx->mm_packed, &ctx->mm_packed_cap, n * 4)) return rc;
+// What a pass of more than 32 rows is given, whatever becomes of the product.
+template <int KIND, int CHUNKS>
+int plan_pairs(yx_ctx *ctx, const Product &p, PairArgs &a) {
     int pairs = 0;
-    if (int rc = resident_pairs<GLU, CHUNKS>(ctx, &pairs)) return rc;
-
-    PairArgs a{};
-    a.T = T;
-    a.cols = GLU ? N / 2 : N;
-    a.t_tiles = (T + TC_MAX_BT - 1) / TC_MAX_BT;
-    a.bt = tile_rows(T);
-    a.ksteps = K / TC_KSTEP;
-    const uint32_t tiles = ((N + TC_M - 1) / TC_M) * a.t_tiles;
+    if (int rc = resident_pairs<KIND, CHUNKS>(ctx, &pairs)) return rc;
+    a.T = p.T;
+    a.cols = KIND == GLU ? p.N / 2 : p.N;
+    a.parts = kind_parts(KIND, p.parts);
+    a.t_tiles = (p.T + TC_MAX_BT - 1) / TC_MAX_BT;
+    a.bt = tile_rows(p.T);
+    a.ksteps = (p.K + TC_KSTEP - 1) / TC_KSTEP;
+    const uint32_t tiles = ((p.N + TC_M - 1) / TC_M) * a.t_tiles;
     a.pairs = (uint32_t)pairs;
     a.rounds = tiles / a.pairs;
     a.rest_units = (tiles - a.rounds * a.pairs) * a.ksteps;
-    if (a.rest_units > 0) a.rest_pairs = share_rest(tiles - a.rounds * a.pairs, a.ksteps, a.pairs, a.bt, a.rounds > 0);
-    const uint32_t stage_bytes = W_BYTES + a.bt * 128u;
-    a.stages = std::min<uint32_t>(TC_MAX_STAGES, (TC_SMEM_BUDGET - 1024) / stage_bytes);
+    if (a.rest_units > 0) a.rest_pairs = share_rest(tiles - a.rounds * a.pairs, a.ksteps, a.pairs, a.bt, a.rounds > 0, 0.001f * (float)a.parts);
+    a.stages = std::min<uint32_t>(TC_MAX_STAGES, (smem_budget(KIND) - 1024) / (W_BYTES + a.parts * a.bt * 64u));
     a.bufs = a.bt <= 128 ? 4 : a.bt <= 160 ? 3 : 2;
     a.buf_columns = 512 / a.bufs / 32 * 32;
-    const bool large = a.bufs < TC_MAX_BUFS && a.rounds > 0 && a.ksteps >= 2 * TC_CHAIN;
-    a.chain = large ? TC_CHAIN : std::min(a.rounds > 0 ? TC_SHORT_CHAIN : TC_CUT_CHAIN, std::max(TC_LEAST_CHAIN, a.ksteps / 2));
-    a.long_first = large && a.bufs == 2;
-    a.out = out;
+    if (KIND < EPILOGUE) {
+        const bool large = a.bufs < TC_MAX_BUFS && a.rounds > 0 && a.ksteps >= 2 * TC_CHAIN;
+        a.chain = large ? TC_CHAIN : std::min(a.rounds > 0 ? TC_SHORT_CHAIN : TC_CUT_CHAIN, std::max(TC_LEAST_CHAIN, a.ksteps / 2));
+        a.long_first = large && a.bufs == 2;
+    } else {
+        a.chain = KIND == EPILOGUE && p.e.out_dtype != YX_F32 ? NARROW_CHAIN : EXACT_CHAIN[a.parts - 1];
+    }
     a.status = ctx->dev_status;
+    return YX_OK;
+}
+
+template <int KIND, int CHUNKS>
+int launch_pairs(yx_ctx *ctx, const CUtensorMap &w_map, const CUtensorMap &x_map, const PairArgs &a) {
+    const uint32_t grid = 2 * (a.rounds > 0 ? a.pairs : a.rest_pairs);
+    return launch_dependent(ctx, "matmul kernel launch", matmul_pair_kernel<KIND, CHUNKS>, dim3(grid), dim3(TC_THREADS),
+                            a.stages * (W_BYTES + a.parts * a.bt * 64u), w_map, x_map, a);
+}
+
+// The map of `parts` matrices [T, K] one behind the other: a CTA's half of a tile's rows, of every part.
+int encode_rows(yx_ctx *ctx, CUtensorMap *map, const void *x, uint32_t T, uint32_t K, uint32_t parts, uint32_t bt) {
+    const cuuint64_t dims[3] = {K, T, parts};
+    const cuuint64_t strides[2] = {(cuuint64_t)K * 2, (cuuint64_t)T * K * 2};
+    const cuuint32_t box[3] = {TC_KSTEP, bt / 2, parts};
+    return encode(ctx, map, 3, x, dims, strides, box);
+}
+
+// PLAIN and GLU.
+template <int KIND, int CHUNKS>
+int matmul_pair_rows(yx_ctx *ctx, const Product &p) {
+    const float *x = (const float *)p.x;
+    const size_t n = (size_t)p.T * p.K;
+    if (int rc = ensure_buffer(ctx, (void **)&ctx->mm_packed, &ctx->mm_packed_cap, n * 4)) return rc;
+    PairArgs a{};
+    if (int rc = plan_pairs<KIND, CHUNKS>(ctx, p, a)) return rc;
+    a.out = (float *)p.out;
     // The most any pass needs (39 MB), so that a call that is being recorded into a graph finds it whatever passes came
     // before: the shares' room does not grow with the rows (512 rows may leave no tile over, 100 rows many).
     if (int rc = ensure_buffer(ctx, (void **)&ctx->mm_part, &ctx->mm_part_cap, (size_t)a.pairs * 2 * 2 * TC_MAX_BT * 128 * sizeof(float))) return rc;
@@ -846,81 +1134,166 @@ int matmul_pair_rows(yx_ctx *ctx, const float *x, const void *w, uint32_t T, uin
     a.counters = ctx->mm_counters;
 
     CUtensorMap w_map, x_map;
-    if (int rc = encode_weights(ctx, &w_map, w, N, K, GLU)) return rc;
+    if (int rc = encode_weights(ctx, &w_map, p.w, p.N, p.K, KIND == GLU)) return rc;
     uint4 *hi = (uint4 *)ctx->mm_packed, *lo = hi + n / 8;
-    {
-        const cuuint64_t dims[3] = {K, T, 2};
-        const cuuint64_t strides[2] = {(cuuint64_t)K * 2, (cuuint64_t)T * K * 2};
-        const cuuint32_t box[3] = {TC_KSTEP, a.bt / 2, 2};
-        if (int rc = encode(ctx, &x_map, 3, hi, dims, strides, box)) return rc;
-    }
+    if (int rc = encode_rows(ctx, &x_map, hi, p.T, p.K, 2, a.bt)) return rc;
     ctx->last_launch = yx_ctx::LAST_OTHER;
     if (int rc = launch_dependent(ctx, "matmul: activation split kernel launch", ((uintptr_t)x & 15u) == 0 ? split_rows_kernel<true> : split_rows_kernel<false>,
                                   dim3((unsigned)((n / 8 + 255) / 256)), dim3(256), 0, x, n, hi, lo))
         return rc;
-    const uint32_t grid = 2 * (a.rounds > 0 ? a.pairs : a.rest_pairs);
-    return launch_dependent(ctx, "matmul kernel launch", matmul_pair_kernel<GLU, CHUNKS>, dim3(grid), dim3(TC_THREADS), a.stages * stage_bytes, w_map, x_map, a);
+    return launch_pairs<KIND, CHUNKS>(ctx, w_map, x_map, a);
 }
 
-template <int TP, bool GLU>
-int matmul_few_rows(yx_ctx *ctx, const float *x, const void *w, uint32_t T, uint32_t N, uint32_t K, float *out) {
-    constexpr uint32_t stage_bytes = W_BYTES + 2 * TP * 128, stages = std::min<uint32_t>(TC_MAX_STAGES, TC_SMEM_BUDGET / stage_bytes);
-    auto *kernel = matmul_rows_kernel<TP, GLU>;
-    bool &configured = ctx->mm_rows_configured[GLU][TP / 16];
+// The scratch of the kinds that take their rows exactly: theirs alone, at the most any pass needs, and never moved.
+int exact_scratch(yx_ctx *ctx, size_t tiles, float **part, uint32_t **counters) {
+    if (int rc = grow(ctx, ctx->ep_part, (size_t)(ctx->sm_count / 2) * 2 * 2 * TC_MAX_BT * 128 * sizeof(float))) return rc;
+    char *before = ctx->ep_counters.dev;
+    if (int rc = grow(ctx, ctx->ep_counters, std::max<size_t>(tiles, 65536) * sizeof(uint32_t))) return rc;
+    *part = (float *)ctx->ep_part.dev;
+    *counters = (uint32_t *)ctx->ep_counters.dev;
+    if (ctx->ep_counters.dev == before) return YX_OK;
+    return check_cuda(ctx, cudaMemsetAsync(ctx->ep_counters.dev, 0, ctx->ep_counters.cap, ctx->stream), "matmul: counters");
+}
+
+// EPILOGUE and LOGPROBS.
+template <int KIND, int CHUNKS>
+int exact_pair_rows(yx_ctx *ctx, const Product &p) {
+    const size_t n = (size_t)p.T * p.K;
+    PairArgs a{};
+    if (int rc = plan_pairs<KIND, CHUNKS>(ctx, p, a)) return rc;
+    a.out = (float *)p.out;
+    a.e = p.e;
+    a.so = StatsOut{(float4 *)p.stats, p.blocks, p.picked};
+    a.ids = p.ids_dev;
+    if (int rc = exact_scratch(ctx, 2 * a.pairs, &a.part, &a.counters)) return rc;
+    const void *rows = p.x;
+    if (p.parts > 1) {
+        if (int rc = grow(ctx, ctx->ep_rows, n * 2 * p.parts)) return rc;
+        rows = ctx->ep_rows.dev;
+    } else if (((uintptr_t)rows & 15u) != 0) {
+        if (int rc = grow(ctx, ctx->ep_rows, n * 2)) return rc;
+        if (int rc = check_cuda(ctx, cudaMemcpyAsync(ctx->ep_rows.dev, rows, n * 2, cudaMemcpyDeviceToDevice, ctx->stream), "matmul: unaligned rows")) return rc;
+        rows = ctx->ep_rows.dev;
+    }
+    CUtensorMap w_map, x_map;
+    if (int rc = encode_weights(ctx, &w_map, p.w, p.N, p.K, false)) return rc;
+    if (int rc = encode_rows(ctx, &x_map, rows, p.T, p.K, p.parts, a.bt)) return rc;
+    ctx->last_launch = yx_ctx::LAST_OTHER;
+    if (p.parts > 1) {
+        const bool vec = ((uintptr_t)p.x & 15u) == 0;
+        auto *kernel = p.parts == 2 ? (vec ? cut_rows_kernel<YX_F16, 2, true> : cut_rows_kernel<YX_F16, 2, false>)
+                                    : (vec ? cut_rows_kernel<YX_F32, 3, true> : cut_rows_kernel<YX_F32, 3, false>);
+        if (int rc = launch_dependent(ctx, "matmul: activation split kernel launch", kernel, dim3((unsigned)((n / 8 + 255) / 256)), dim3(256), 0, p.x, n,
+                                      (uint4 *)ctx->ep_rows.dev))
+            return rc;
+    }
+    // (with LOGPROBS the given tokens' kernel is ahead, which starts this one after its own wait too)
+    a.early_w = p.parts > 1 || KIND == LOGPROBS;
+    return launch_pairs<KIND, CHUNKS>(ctx, w_map, x_map, a);
+}
+
+template <int TP, int KIND, int PARTS>
+int matmul_few_rows(yx_ctx *ctx, const Product &p) {
+    constexpr uint32_t stage_bytes = W_BYTES + rows_columns(TP, PARTS) * 128;
+    constexpr uint32_t stages = std::min<uint32_t>(TC_MAX_STAGES, (KIND == LOGPROBS ? 210 * 1024 : TC_SMEM_BUDGET) / stage_bytes);
+    auto *kernel = matmul_rows_kernel<TP, KIND, PARTS>;
+    bool &configured = ctx->mm_rows_configured[KIND][PARTS - 1][TP / 16];
     if (!configured) {
         if (int rc = check_cuda(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, stages * stage_bytes),
                                 "matmul: shared memory attribute"))
             return rc;
         configured = true;
     }
+    const uint32_t T = p.T, N = p.N, K = p.K;
     RowsArgs a{};
-    // Other CTAs still read the rows when a tile's result is written: a result over its own rows takes them from a copy.
-    const uintptr_t x0 = (uintptr_t)x, o0 = (uintptr_t)out;
-    if (o0 < x0 + (size_t)T * K * 4 && x0 < o0 + (size_t)T * (GLU ? N / 2 : N) * 4) {
-        if (int rc = ensure_buffer(ctx, (void **)&ctx->mm_packed, &ctx->mm_packed_cap, (size_t)ROWS_MAX * K * 4)) return rc;
-        if (int rc = check_cuda(ctx, cudaMemcpyAsync(ctx->mm_packed, x, (size_t)T * K * 4, cudaMemcpyDeviceToDevice, ctx->stream), "matmul: rows under the result"))
-            return rc;
-        x = (const float *)ctx->mm_packed;
+    a.x = p.x;
+    if (KIND < EPILOGUE) {
+        // Other CTAs still read the rows when a tile's result is written: a result over its own rows takes them from a copy.
+        const uintptr_t x0 = (uintptr_t)p.x, o0 = (uintptr_t)p.out;
+        if (o0 < x0 + (size_t)T * K * 4 && x0 < o0 + (size_t)T * (KIND == GLU ? N / 2 : N) * 4) {
+            if (int rc = ensure_buffer(ctx, (void **)&ctx->mm_packed, &ctx->mm_packed_cap, (size_t)ROWS_MAX * K * 4)) return rc;
+            if (int rc = check_cuda(ctx, cudaMemcpyAsync(ctx->mm_packed, p.x, (size_t)T * K * 4, cudaMemcpyDeviceToDevice, ctx->stream), "matmul: rows under the result"))
+                return rc;
+            a.x = ctx->mm_packed;
+        }
     }
-    a.x = x;
     a.T = T;
     a.K = K;
-    a.cols = GLU ? N / 2 : N;
-    a.ksteps = K / TC_KSTEP;
+    a.cols = KIND == GLU ? N / 2 : N;
+    a.ksteps = (K + TC_KSTEP - 1) / TC_KSTEP;
     const uint32_t tiles = (N + ROWS_M - 1) / ROWS_M;
     a.units = tiles * a.ksteps;
     a.ctas = std::min((uint32_t)ctx->sm_count, std::max(1u, a.units / 2));
     a.stages = stages;
-    a.x_vec16 = ((uintptr_t)x & 15u) == 0;
-    a.out = out;
+    a.x_vec16 = ((uintptr_t)a.x & 15u) == 0;
+    a.out = (float *)p.out;
+    a.e = p.e;
+    a.so = StatsOut{(float4 *)p.stats, p.blocks, p.picked};
+    if (KIND == LOGPROBS) std::copy(p.ids_host, p.ids_host + T, a.ids);
     a.status = ctx->dev_status;
-    // (for any number of rows and any weight, as in matmul_pair_rows: one row may be followed by sixteen in a recording)
-    if (int rc = ensure_buffer(ctx, (void **)&ctx->mm_part, &ctx->mm_part_cap, (size_t)2 * ctx->sm_count * ROWS_MAX * 128 * sizeof(float))) return rc;
-    if (int rc = ensure_counters(ctx, tiles)) return rc;
-    a.part = ctx->mm_part;
-    a.counters = ctx->mm_counters;
+    if (KIND < EPILOGUE) {
+        // (for any number of rows and any weight, as in matmul_pair_rows: one row may be followed by sixteen in a recording)
+        if (int rc = ensure_buffer(ctx, (void **)&ctx->mm_part, &ctx->mm_part_cap, (size_t)2 * ctx->sm_count * ROWS_MAX * 128 * sizeof(float))) return rc;
+        if (int rc = ensure_counters(ctx, tiles)) return rc;
+        a.part = ctx->mm_part;
+        a.counters = ctx->mm_counters;
+    } else if (int rc = exact_scratch(ctx, tiles, &a.part, &a.counters)) {
+        return rc;
+    }
     CUtensorMap w_map;
-    if (int rc = encode_weights(ctx, &w_map, w, N, K, GLU)) return rc;
+    if (int rc = encode_weights(ctx, &w_map, p.w, N, K, KIND == GLU)) return rc;
     ctx->last_launch = yx_ctx::LAST_OTHER;
     return launch_dependent(ctx, "matmul kernel launch", kernel, dim3(a.ctas), dim3(ROWS_THREADS), stages * stage_bytes, w_map, a);
 }
 
-template <bool GLU>
-int matmul_tc(yx_ctx *ctx, const float *x, const void *w, uint32_t T, uint32_t N, uint32_t K, float *out) {
-    if (T <= 8) return matmul_few_rows<8, GLU>(ctx, x, w, T, N, K, out);
-    if (T <= 16) return matmul_few_rows<16, GLU>(ctx, x, w, T, N, K, out);
-    if (T <= 32) return matmul_few_rows<32, GLU>(ctx, x, w, T, N, K, out);
-    const uint32_t rows = tile_rows(T);
-    if (rows <= 128) return matmul_pair_rows<GLU, 2>(ctx, x, w, T, N, K, out);
-    if (rows <= 192) return matmul_pair_rows<GLU, 3>(ctx, x, w, T, N, K, out);
-    return matmul_pair_rows<GLU, 4>(ctx, x, w, T, N, K, out);
+template <int KIND>
+int matmul_tc(yx_ctx *ctx, const Product &p) {
+    if (p.T <= 8) return matmul_few_rows<8, KIND, 2>(ctx, p);
+    if (p.T <= 16) return matmul_few_rows<16, KIND, 2>(ctx, p);
+    if (p.T <= 32) return matmul_few_rows<32, KIND, 2>(ctx, p);
+    const uint32_t rows = tile_rows(p.T);
+    if (rows <= 128) return matmul_pair_rows<KIND, 2>(ctx, p);
+    if (rows <= 192) return matmul_pair_rows<KIND, 3>(ctx, p);
+    return matmul_pair_rows<KIND, 4>(ctx, p);
+}
+
+template <int KIND, int PARTS>
+int exact_few_rows(yx_ctx *ctx, const Product &p) {
+    // (eight columns of one part are fewer than an MMA takes)
+    if constexpr (PARTS > 1)
+        if (p.T <= 8) return matmul_few_rows<8, KIND, PARTS>(ctx, p);
+    if (p.T <= 16) return matmul_few_rows<16, KIND, PARTS>(ctx, p);
+    return matmul_few_rows<32, KIND, PARTS>(ctx, p);
+}
+template <int KIND>
+int exact_tc(yx_ctx *ctx, const Product &p) {
+    if (p.T <= ROWS_MAX)
+        return p.parts == 1 ? exact_few_rows<KIND, 1>(ctx, p) : p.parts == 2 ? exact_few_rows<KIND, 2>(ctx, p) : exact_few_rows<KIND, 3>(ctx, p);
+    const uint32_t rows = tile_rows(p.T);
+    if (rows <= 128) return exact_pair_rows<KIND, 2>(ctx, p);
+    if (rows <= 192) return exact_pair_rows<KIND, 3>(ctx, p);
+    return exact_pair_rows<KIND, 4>(ctx, p);
 }
 
 }  // namespace
 
 // Takes K a multiple of 128, w 16-byte aligned, x 8-byte aligned; with `glu`, a multiple of 16 result columns.
 int launch_matmul_tc(yx_ctx *ctx, const float *x, const void *w, uint32_t T, uint32_t N, uint32_t K, bool glu, float *out) {
-    return glu ? matmul_tc<true>(ctx, x, w, T, N, K, out) : matmul_tc<false>(ctx, x, w, T, N, K, out);
+    Product p{};
+    p.x = x;
+    p.w = w;
+    p.T = T;
+    p.N = N;
+    p.K = K;
+    p.parts = 2;
+    p.out = out;
+    return glu ? matmul_tc<GLU>(ctx, p) : matmul_tc<PLAIN>(ctx, p);
 }
+
+bool exact_tc_takes(const Product &p) { return p.K % 8 == 0 && ((uintptr_t)p.w & 15u) == 0; }
+bool exact_tc_reads_rows_late(const Product &p) { return p.T <= ROWS_MAX || p.parts == 1; }
+uint32_t logprobs_block(const Product &p) { return p.T <= ROWS_MAX ? (p.N + ROWS_M - 1) / ROWS_M : 2 * ((p.N + TC_M - 1) / TC_M); }
+int launch_matmul_epilogue_tc(yx_ctx *ctx, const Product &p) { return exact_tc<EPILOGUE>(ctx, p); }
+int launch_matmul_logprobs_tc(yx_ctx *ctx, const Product &p) { return exact_tc<LOGPROBS>(ctx, p); }
 
 }  // namespace yx

@@ -8,14 +8,6 @@
 
 namespace yx {
 
-// out = act(sum + bias) + residual, in f32, rounded once to the output's type.
-struct Epilogue {
-    const float *bias;      // [cols] or null
-    const void *residual;   // [rows, cols] of the output's type or null; may be the output itself
-    int act;                // yx_activation
-    int out_dtype;          // yx_dtype
-};
-
 namespace dev {
 
 __device__ __forceinline__ float load_as_f32(const void *p, int dtype, size_t i) {
@@ -38,6 +30,12 @@ __device__ __forceinline__ float activate(float y, int act) {
     case YX_ACT_SILU: return y / (1.0f + expf(-y));
     default: return y;
     }
+}
+
+// (out of line: a tile's epilogue is unrolled over up to 128 results, and five activations in each would not fit the
+// instruction cache; four at a time, the call costs less than the exponentials)
+static __device__ __noinline__ float4 activate4(float4 y, int act) {
+    return make_float4(activate(y.x, act), activate(y.y, act), activate(y.z, act), activate(y.w, act));
 }
 
 // A softmax's statistics over some of a row's logits l: the largest m, s = sum exp(l - m), t = sum exp(l - m) (l - m).

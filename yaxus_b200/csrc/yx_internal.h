@@ -350,8 +350,8 @@ struct yx_ctx {
     size_t mm_sums_cap = 0;
     uint32_t *mm_counters = nullptr;       // arrivals at the matmul tiles several CTAs share; zero between launches
     size_t mm_counters_cap = 0;
-    bool mm_rows_configured[2][3] = {};    // opt-in to large shared memory of the few-row matmul kernels
-    int mm_pairs[2][3] = {};               // CTA pairs of the matmul kernel (plain or GLU, by the tile's size) that fit the chip together
+    bool mm_rows_configured[4][3][3] = {}; // opt-in to large shared memory of the few-row matmul kernels
+    int mm_pairs[4][3] = {};               // CTA pairs of the matmul kernel (by its kind and the tile's size) that fit the chip together
     uint32_t *idx_dev = nullptr;           // token ids / row indices / argmax parts of the model operators
     size_t idx_cap = 0;
     uint32_t *pick_counters = nullptr;     // argmax: arrivals per row, zero between launches
@@ -364,7 +364,8 @@ struct yx_ctx {
         char *dev = nullptr;
         size_t cap = 0;
     };
-    Grown lp_ids, lp_logits, ep_rows;      // given tokens; logits of a few rows at a time; pass rows copied or in parts
+    Grown lp_ids, lp_logits, lp_stats;     // given tokens; logits of a few rows at a time; statistics by blocks of columns
+    Grown ep_rows, ep_part, ep_counters;   // pass rows copied or in parts; sums of shared tiles, and arrivals there (zero between launches)
     std::vector<void *> outgrown;
 
     // multi-GPU
@@ -389,10 +390,38 @@ int grow(yx_ctx *ctx, yx_ctx::Grown &buf, size_t bytes);
 // yx_attend over the keys [key_lo, key_hi) only: what one rank alone has to do for yx_attend_allgather.
 int attend_key_range(yx_ctx *ctx, yx_kv *kv, int layer, const void *q, int q_dtype, int hq, int64_t window, uint64_t key_lo,
                      uint64_t key_hi, void *out, int out_dtype);
+// out = act(sum + bias) + residual, in f32, rounded once to the output's type.
+struct Epilogue {
+    const float *bias;       // [cols] or null
+    const void *residual;    // [rows, cols] of the output's type or null; may be the output itself
+    int act;                 // yx_activation
+    int out_dtype;           // yx_dtype
+};
 // out = x . w^T on the tensor cores for many rows (matmul_tc.cu says what it takes).
 int launch_matmul_tc(yx_ctx *ctx, const float *x, const void *w, uint32_t T, uint32_t N, uint32_t K, bool glu, float *out);
 
-// The statistics of softmax rows: logprobs.cu.
+// A product whose rows are taken exactly, and what becomes of it (matmul_tc.cu).  `parts`: bf16 parts of a row's value.
+struct Product {
+    const void *x, *w;
+    uint32_t T, N, K;
+    int parts;
+    void *out;
+    Epilogue e;              // yx_matmul_epilogue
+    void *stats;             // yx_matmul_logprobs: float4 [T][blocks], blocks = logprobs_block(p)
+    uint32_t blocks;
+    float *picked;           // logits of the given tokens [T]
+    const uint32_t *ids_dev, *ids_host;   // for more than 32 rows; for fewer
+};
+bool exact_tc_takes(const Product &p);
+// Whether the kernel that writes the result is also the one that reads the rows.
+bool exact_tc_reads_rows_late(const Product &p);
+uint32_t logprobs_block(const Product &p);
+int launch_matmul_epilogue_tc(yx_ctx *ctx, const Product &p);
+int launch_matmul_logprobs_tc(yx_ctx *ctx, const Product &p);
+
+// The statistics of softmax rows: logprobs.cu.  put_ids brings `n` given tokens to the device (ctx->lp_ids).
+int put_ids(yx_ctx *ctx, const uint32_t *host, size_t n, const uint32_t **out);
+int launch_logprob_blocks(yx_ctx *ctx, const void *stats, uint32_t blocks, const float *picked, uint32_t rows, float *logprob, float *entropy);
 int launch_logprob_rows(yx_ctx *ctx, const void *logits, int dtype, uint32_t rows, uint32_t cols, size_t stride, const uint32_t *ids_host,
                         uint32_t n_ids, uint32_t n_top, float *logprob, float *entropy, uint32_t *top_ids, float *top_logprob);
 
