@@ -623,7 +623,7 @@ void yx_ctx_destroy(yx_ctx *ctx) {
     if (ctx->idx_dev) cudaFree(ctx->idx_dev);
     if (ctx->pick_counters) cudaFree(ctx->pick_counters);
     if (ctx->pick_host) cudaFreeHost(ctx->pick_host);
-    for (yx_ctx::Grown *b : {&ctx->lp_ids, &ctx->lp_logits, &ctx->lp_stats, &ctx->ep_rows, &ctx->ep_part, &ctx->ep_counters})
+    for (yx_ctx::Grown *b : {&ctx->lp_ids, &ctx->lp_logits, &ctx->lp_stats, &ctx->lp_parts, &ctx->ep_rows, &ctx->ep_part, &ctx->ep_counters})
         if (b->dev) cudaFree(b->dev);
     for (void *p : ctx->outgrown) cudaFree(p);
     if (ctx->gather_buf) cudaFree(ctx->gather_buf);

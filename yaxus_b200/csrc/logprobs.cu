@@ -40,51 +40,314 @@ __device__ __forceinline__ RowStats merge_warp(RowStats r) {
     return r;
 }
 
+// ---- rows of logits ---------------------------------------------------------------------------------------
+//
+// One pass over the logits.  A row is cut into parts, a CTA each (one part where there are rows enough to fill the chip), and a
+// part into tiles of 16 logits a thread, the next tile's loads in flight while one is worked on.  A thread keeps the
+// statistics (m, s, t) of what it has seen and moves m only when a tile exceeds it.
+//
+// The best tokens: whatever exceeds the n-th best found so far goes to a list in shared memory, and the list is cut back
+// to its n best, in order, when it has grown.  The first tile has no n-th best: the n-th largest of 32 groups' largest serves
+// (n numbers are at least that, one of each group), which some n to 4 n logits pass.  Keys of logit and token are all
+// different, so that a row of equal logits passes no more.  The parts' lists and statistics meet in the row's last CTA.
+constexpr int THREADS = 256, WARPS = THREADS / 32;
+constexpr int PER_THREAD = 16;                              // logits of a tile
+constexpr int TILE = THREADS * PER_THREAD;
+constexpr uint32_t MAX_PARTS = 128;                         // of a row: TILE of their best tokens
+constexpr uint32_t MAX_SHARED = 2048;                       // parts of all rows that have more than one
+constexpr int LIST_AGAIN = 64;                              // threads that have added to the list, after which it is cut back
+constexpr uint32_t IDS_PARAM = 512;                         // given tokens that ride in kernel-parameter space
+static_assert(MAX_PARTS * YX_TOP_MAX <= TILE, "the last CTA holds the parts' best tokens as one tile");
+
 struct RowsArgs {
     const void *logits;
-    int dtype;
-    uint32_t cols;
+    uint32_t cols, parts, n_ids, n_top;
     size_t stride;
-    const uint32_t *ids;
-    uint32_t n_ids, n_top;
+    const uint32_t *ids_dev;                                // null: ids
     float *logprob, *entropy;
     uint32_t *top_ids;
     float *top_logprob;
+    float4 *part_stats;                                     // [rows][parts]
+    uint64_t *part_best;                                    // [rows][parts][n_top]
+    uint32_t *arrived;                                      // [rows], zero between launches
+    uint32_t ids[IDS_PARAM];
 };
 
-// One CTA a row: the statistics in one pass, then a pass for every alternative.
-__global__ void __launch_bounds__(256) logprob_rows_kernel(const RowsArgs a) {
-    __shared__ RowStats part[8];
-    __shared__ uint64_t best[2][8];
-    dependent_entry();
-    const size_t row = blockIdx.x, base = row * a.stride;
-    RowStats r = no_stats();
-    for (uint32_t c = threadIdx.x; c < a.cols; c += blockDim.x) r = merge(r, RowStats{clean(load_as_f32(a.logits, a.dtype, base + c)), 1.0f, 0.0f});
-    r = merge_warp(r);
-    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = r;
+struct List {
+    uint64_t key[YX_TOP_MAX + (LIST_AGAIN + THREADS) * PER_THREAD];   // the best, what has come since, and one more tile
+    uint64_t group[WARPS][32];
+    uint64_t warp_best[2][WARPS];
+    uint32_t count;
+};
+
+// The n-th largest of 32 groups' largest keys; a group is a lane of every warp.  All threads get it.
+__device__ __forceinline__ uint64_t nth_of_groups(List &list, uint64_t best, uint32_t n) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    list.group[warp][lane] = best;
     __syncthreads();
-    r = part[0];
-    for (int i = 1; i < 8; i++) r = merge(r, part[i]);
-    const float log_s = logf(r.s);
-    for (uint32_t i = threadIdx.x; i < a.n_ids; i += blockDim.x)
-        a.logprob[row * a.n_ids + i] = log_prob(load_as_f32(a.logits, a.dtype, base + a.ids[row * a.n_ids + i]), r.m, log_s);
-    if (threadIdx.x == 0 && a.entropy) a.entropy[row] = entropy(r);
-    uint64_t below = ~0ull;
-    for (uint32_t k = 0; k < a.n_top; k++) {
-        uint64_t b = 0;
-        for (uint32_t c = threadIdx.x; c < a.cols; c += blockDim.x) {
-            const uint64_t key = key_of(load_as_f32(a.logits, a.dtype, base + c), c);
-            if (key < below && key > b) b = key;
+    uint64_t g = list.group[0][lane];
+#pragma unroll
+    for (int w = 1; w < WARPS; w++) g = max(g, list.group[w][lane]);
+    uint32_t larger = 0;
+#pragma unroll 8
+    for (int i = 0; i < 32; i++) {
+        const uint64_t other = __shfl_sync(0xffffffffu, g, i);
+        larger += other > g || (other == g && i < lane);   // (groups without a token share key 0)
+    }
+    return __shfl_sync(0xffffffffu, g, __ffs(__ballot_sync(0xffffffffu, larger == n - 1)) - 1);
+}
+
+// Adds this thread's key to the list if `in`; all lanes of a warp call it together.
+__device__ __forceinline__ void add_to_list(List &list, bool in, uint64_t key) {
+    const uint32_t mask = __ballot_sync(0xffffffffu, in);
+    if (mask == 0) return;
+    const int lane = threadIdx.x & 31;
+    uint32_t at = 0;
+    if (lane == 0) at = atomicAdd(&list.count, (uint32_t)__popc(mask));
+    at = __shfl_sync(0xffffffffu, at, 0) + __popc(mask & ((1u << lane) - 1));
+    if (in) list.key[at] = key;
+}
+
+// Cuts the list back to its n best, in order; after a barrier, and ends in one.  Returns how many there are.
+__device__ __forceinline__ uint32_t cut_list(List &list, uint32_t n) {
+    const uint32_t count = list.count;
+    if (count <= 2 * THREADS) {
+        // A key's place is the number of keys above it.
+        uint64_t key[2];
+        uint32_t place[2] = {0, 0};
+#pragma unroll
+        for (int j = 0; j < 2; j++) key[j] = threadIdx.x + j * THREADS < count ? list.key[threadIdx.x + j * THREADS] : 0;
+        for (uint32_t i = 0; i < count; i++) {
+            const uint64_t other = list.key[i];
+#pragma unroll
+            for (int j = 0; j < 2; j++) place[j] += other > key[j];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < 2; j++)
+            if (key[j] != 0 && place[j] < n) list.key[place[j]] = key[j];
+    } else {
+        // (a row whose logits rise: nearly all of a tile is on the list)
+        uint64_t below = ~0ull, mine = 0;
+        for (uint32_t k = 0; k < n; k++) {
+            uint64_t b = 0;
+            for (uint32_t i = threadIdx.x; i < count; i += THREADS) {
+                const uint64_t key = list.key[i];
+                if (key < below && key > b) b = key;
+            }
+#pragma unroll
+            for (int d = 16; d > 0; d >>= 1) b = max(b, __shfl_xor_sync(0xffffffffu, b, d));
+            if ((threadIdx.x & 31) == 0) list.warp_best[k & 1][threadIdx.x >> 5] = b;
+            __syncthreads();
+            b = list.warp_best[k & 1][0];
+#pragma unroll
+            for (int w = 1; w < WARPS; w++) b = max(b, list.warp_best[k & 1][w]);
+            below = b;
+            if (threadIdx.x == k) mine = b;
+        }
+        __syncthreads();
+        if (threadIdx.x < n) list.key[threadIdx.x] = mine;
+    }
+    if (threadIdx.x == 0) list.count = min(count, n);
+    __syncthreads();
+    return min(count, n);
+}
+
+// The statistics of all of the CTA's threads, in all of them; `scratch` is the caller's alone.
+__device__ __forceinline__ RowStats merge_cta(RowStats r, RowStats *scratch) {
+    r = merge_warp(r);
+    if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = r;
+    __syncthreads();
+    r = scratch[0];
+#pragma unroll
+    for (int i = 1; i < WARPS; i++) r = merge(r, scratch[i]);
+    return r;
+}
+
+template <int DTYPE>
+struct Tile {
+    static constexpr int WIDE = DTYPE == YX_F32 ? 4 : 8;   // logits in 16 bytes
+    static constexpr int VECS = PER_THREAD / WIDE;
+    uint4 v[VECS];
+
+    // Vectors first, first + THREADS, ... of a row whose logit 0 is element `shift` of vector 0; what lies before the row, behind
+    // it, or at or behind vector `end` counts as forbidden.
+    __device__ __forceinline__ void load(const char *base, uint32_t shift, uint32_t cols, uint64_t first, uint64_t end) {
+#pragma unroll
+        for (int i = 0; i < VECS; i++) {
+            const uint64_t vec = first + (uint64_t)i * THREADS, c = vec * WIDE;
+            constexpr uint32_t none = DTYPE == YX_F32 ? 0xff800000u : DTYPE == YX_F16 ? 0xfc00fc00u : 0xff80ff80u;
+            v[i] = make_uint4(none, none, none, none);
+            if (vec >= end) continue;
+            if (c >= shift && c + WIDE <= (uint64_t)shift + cols) {
+                v[i] = __ldcs((const uint4 *)(base + vec * 16));
+            } else {
+                uint32_t w[4] = {none, none, none, none};
+#pragma unroll
+                for (int e = 0; e < WIDE; e++) {
+                    if (c + e < shift || c + e >= (uint64_t)shift + cols) continue;
+                    if constexpr (DTYPE == YX_F32) w[e] = *(const uint32_t *)(base + vec * 16 + e * 4);
+                    else w[e / 2] = (w[e / 2] & (e & 1 ? 0xffffu : 0xffff0000u)) | (uint32_t)*(const uint16_t *)(base + vec * 16 + e * 2) << (e & 1 ? 16 : 0);
+                }
+                v[i] = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+        }
+    }
+    __device__ __forceinline__ void unpack(float (&x)[PER_THREAD]) const {
+#pragma unroll
+        for (int i = 0; i < VECS; i++) {
+            const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                if constexpr (DTYPE == YX_F32) {
+                    x[4 * i + e] = __uint_as_float(w[e]);
+                } else {
+                    const float2 f = unpack2<DTYPE == YX_BF16>(w[e]);
+                    x[8 * i + 2 * e] = f.x;
+                    x[8 * i + 2 * e + 1] = f.y;
+                }
+            }
+        }
+    }
+    // The token of element j; past any vocabulary before the row and at or behind vector `end`.
+    static __device__ __forceinline__ uint32_t token(uint64_t first, int j, uint32_t shift, uint64_t end) {
+        const uint64_t vec = first + (uint64_t)(j / WIDE) * THREADS;
+        return vec < end ? (uint32_t)(vec * WIDE) + j % WIDE - shift : 0xffffffffu;
+    }
+};
+
+template <int DTYPE, bool TOP>
+__global__ void __launch_bounds__(THREADS, 4) logprob_rows_kernel(const __grid_constant__ RowsArgs a) {
+    __shared__ List list;
+    __shared__ RowStats scratch[2][WARPS];
+    __shared__ bool last;
+    using T = Tile<DTYPE>;
+    dependent_entry();
+    const uint32_t row = blockIdx.x / a.parts, part = blockIdx.x - row * a.parts;
+    constexpr int ES = DTYPE == YX_F32 ? 4 : 2;
+    const char *logits = (const char *)a.logits + (size_t)row * a.stride * ES;
+    const uint32_t shift = (uint32_t)((uintptr_t)logits & 15u) / ES;
+    const char *base = logits - shift * ES;
+    const uint64_t vecs = ((uint64_t)shift + a.cols + T::WIDE - 1) / T::WIDE;
+    const uint64_t v0 = vecs * part / a.parts, v1 = vecs * (part + 1) / a.parts;
+    if (TOP && threadIdx.x == 0) list.count = 0;
+
+    RowStats r = no_stats();
+    float least = -INFINITY;   // the n-th best logit found, once there are n
+    int added = 0;
+    T next;
+    next.load(base, shift, a.cols, v0 + threadIdx.x, v1);
+    for (uint64_t v = v0; v < v1; v += T::VECS * THREADS) {
+        const T tile = next;
+        next.load(base, shift, a.cols, v + T::VECS * THREADS + threadIdx.x, v1);
+        float x[PER_THREAD];
+        tile.unpack(x);
+        float most = x[0];
+#pragma unroll
+        for (int j = 1; j < PER_THREAD; j++) most = fmaxf(most, x[j]);
+        if (most > r.m) {
+            if (most == INFINITY) {
+#pragma unroll
+                for (int j = 0; j < PER_THREAD; j++) x[j] = clean(x[j]);
+                most = clean(most);
+            }
+            const float d = distance(r.m, most), c = fast_exp2(d * LOG2_E);
+            r.t = c * (r.t + d * r.s);
+            r.s *= c;
+            r.m = most;
         }
 #pragma unroll
-        for (int d = 16; d > 0; d >>= 1) b = max(b, __shfl_xor_sync(0xffffffffu, b, d));
-        if ((threadIdx.x & 31) == 0) best[k & 1][threadIdx.x >> 5] = b;
+        for (int j = 0; j < PER_THREAD; j++) {
+            const float d = distance(x[j], r.m), e = fast_exp2(d * LOG2_E);
+            r.s += e;
+            r.t += e * d;
+        }
+        if constexpr (TOP) {
+            if (v == v0) {
+                uint64_t best = 0;
+#pragma unroll
+                for (int j = PER_THREAD - 1; j >= 0; j--) {
+                    const uint32_t token = T::token(v + threadIdx.x, j, shift, v1);
+                    if (token < a.cols) best = max(best, key_of(x[j], token));
+                }
+                const uint64_t least_key = nth_of_groups(list, best, a.n_top);
+#pragma unroll
+                for (int j = 0; j < PER_THREAD; j++) {
+                    const uint32_t token = T::token(v + threadIdx.x, j, shift, v1);
+                    const uint64_t key = token < a.cols ? key_of(x[j], token) : 0;
+                    add_to_list(list, key != 0 && key >= least_key, key);
+                }
+            } else if (__any_sync(0xffffffffu, most > least)) {
+                // (tokens come in order: an equal one later is no better)
+#pragma unroll
+                for (int j = 0; j < PER_THREAD; j++) add_to_list(list, x[j] > least, key_of(x[j], T::token(v + threadIdx.x, j, shift, v1)));
+            }
+            // (counted by the barrier itself: the list's own count may be moving again when the last thread reads it)
+            added += __syncthreads_count(v == v0 || most > least);
+            if (added > LIST_AGAIN) {
+                added = 0;
+                if (cut_list(list, a.n_top) == a.n_top) least = key_logit(list.key[a.n_top - 1]);
+                __syncthreads();
+            }
+        }
+    }
+    uint32_t found = 0;
+    if constexpr (TOP) {
         __syncthreads();
-        for (int i = 0; i < 8; i++) b = max(b, best[k & 1][i]);
-        below = b;
+        found = cut_list(list, a.n_top);
+    }
+    r = merge_cta(r, scratch[0]);
+    if (a.parts > 1) {
+        const size_t mine = (size_t)row * a.parts + part;
+        if constexpr (TOP)
+            if (threadIdx.x < a.n_top) __stcg(a.part_best + mine * a.n_top + threadIdx.x, threadIdx.x < found ? list.key[threadIdx.x] : 0ull);
+        if (threadIdx.x == 0) __stcg(a.part_stats + mine, make_float4(r.m, r.s, r.t, 0.0f));
+        __threadfence();
+        __syncthreads();
         if (threadIdx.x == 0) {
-            a.top_ids[row * a.n_top + k] = key_token(b);
-            a.top_logprob[row * a.n_top + k] = log_prob(key_logit(b), r.m, log_s);
+            last = atomicAdd(a.arrived + row, 1u) + 1 == a.parts;
+            if (last) a.arrived[row] = 0u;
+        }
+        __syncthreads();
+        if (!last) return;
+        __threadfence();
+        r = no_stats();
+        if (threadIdx.x < a.parts) {
+            const float4 f = __ldcg(a.part_stats + (size_t)row * a.parts + threadIdx.x);
+            r = RowStats{f.x, f.y, f.z};
+        }
+        if constexpr (TOP) {
+            const uint32_t keys = a.parts * a.n_top;
+            const uint64_t *from = a.part_best + (size_t)row * keys;
+            uint64_t key[PER_THREAD], best = 0;
+#pragma unroll
+            for (int j = 0; j < PER_THREAD; j++) {
+                const uint32_t i = threadIdx.x + j * THREADS;
+                key[j] = i < keys ? __ldcg(from + i) : 0;
+                best = max(best, key[j]);
+            }
+            if (threadIdx.x == 0) list.count = 0;
+            const uint64_t least_key = nth_of_groups(list, best, a.n_top);
+#pragma unroll
+            for (int j = 0; j < PER_THREAD; j++) {
+                if (j * THREADS >= keys) break;
+                add_to_list(list, key[j] != 0 && key[j] >= least_key, key[j]);
+            }
+            __syncthreads();
+            cut_list(list, a.n_top);
+        }
+        r = merge_cta(r, scratch[1]);
+    }
+    const float log_s = logf(r.s);
+    const uint32_t *ids = a.ids_dev ? a.ids_dev : a.ids;
+    for (uint32_t i = threadIdx.x; i < a.n_ids; i += THREADS)
+        a.logprob[(size_t)row * a.n_ids + i] = log_prob(load_as_f32(logits, DTYPE, ids[(size_t)row * a.n_ids + i]), r.m, log_s);
+    if (threadIdx.x == 0 && a.entropy) a.entropy[row] = entropy(r);
+    if constexpr (TOP) {
+        if (threadIdx.x < a.n_top) {
+            const uint64_t key = list.key[threadIdx.x];
+            a.top_ids[(size_t)row * a.n_top + threadIdx.x] = key_token(key);
+            a.top_logprob[(size_t)row * a.n_top + threadIdx.x] = log_prob(key_logit(key), r.m, log_s);
         }
     }
 }
@@ -131,11 +394,40 @@ int launch_logprob_blocks(yx_ctx *ctx, const void *stats, uint32_t blocks, const
 
 int launch_logprob_rows(yx_ctx *ctx, const void *logits, int dtype, uint32_t rows, uint32_t cols, size_t stride, const uint32_t *ids_host,
                         uint32_t n_ids, uint32_t n_top, float *logprob, float *entropy, uint32_t *top_ids, float *top_logprob) {
-    RowsArgs a{logits, dtype, cols, stride, nullptr, n_ids, n_top, logprob, entropy, top_ids, top_logprob};
-    if (n_ids > 0)
-        if (int rc = put_ids(ctx, ids_host, (size_t)rows * n_ids, &a.ids)) return rc;
+    RowsArgs a;
+    a.logits = logits;
+    a.cols = cols;
+    a.stride = stride;
+    a.n_ids = n_ids;
+    a.n_top = n_top;
+    a.ids_dev = nullptr;
+    a.logprob = logprob;
+    a.entropy = entropy;
+    a.top_ids = top_ids;
+    a.top_logprob = top_logprob;
+    // Rows that fill the chip by themselves are a CTA each; fewer are cut into parts of a tile or more.
+    const uint32_t tiles = (uint32_t)(((uint64_t)cols + TILE - 1) / TILE), want = 4 * (uint32_t)ctx->sm_count;
+    a.parts = rows >= want / 2 ? 1 : std::min({tiles, MAX_PARTS, (want + rows - 1) / rows, MAX_SHARED / rows});
+    // (at the most any call needs, for recordings)
+    const size_t stats = MAX_SHARED * sizeof(float4), best = (size_t)MAX_SHARED * YX_TOP_MAX * sizeof(uint64_t);
+    char *before = ctx->lp_parts.dev;
+    if (int rc = grow(ctx, ctx->lp_parts, stats + best + MAX_SHARED * sizeof(uint32_t))) return rc;
+    a.part_stats = (float4 *)ctx->lp_parts.dev;
+    a.part_best = (uint64_t *)(ctx->lp_parts.dev + stats);
+    a.arrived = (uint32_t *)(ctx->lp_parts.dev + stats + best);
+    if (ctx->lp_parts.dev != before)
+        if (int rc = check_cuda(ctx, cudaMemsetAsync(a.arrived, 0, MAX_SHARED * sizeof(uint32_t), ctx->stream), "logprob_rows: counters")) return rc;
+    const size_t given = (size_t)rows * n_ids;
+    if (given > IDS_PARAM) {
+        if (int rc = put_ids(ctx, ids_host, given, &a.ids_dev)) return rc;
+    } else if (given > 0) {
+        memcpy(a.ids, ids_host, given * 4);
+    }
     ctx->last_launch = yx_ctx::LAST_OTHER;
-    return launch_dependent(ctx, "logprob_rows kernel launch", logprob_rows_kernel, dim3(rows), dim3(256), 0, a);
+    auto go = [&](auto kernel) { return launch_dependent(ctx, "logprob_rows kernel launch", kernel, dim3(rows * a.parts), dim3(THREADS), 0, a); };
+    if (dtype == YX_F32) return n_top > 0 ? go(logprob_rows_kernel<YX_F32, true>) : go(logprob_rows_kernel<YX_F32, false>);
+    if (dtype == YX_F16) return n_top > 0 ? go(logprob_rows_kernel<YX_F16, true>) : go(logprob_rows_kernel<YX_F16, false>);
+    return n_top > 0 ? go(logprob_rows_kernel<YX_BF16, true>) : go(logprob_rows_kernel<YX_BF16, false>);
 }
 
 }  // namespace yx
@@ -151,7 +443,7 @@ extern "C" int yx_logprob_rows(yx_ctx *ctx, const void *logits_dev, int dtype, u
     if (rows == 0) return YX_OK;
     if (!logits_dev || cols == 0) return fail(ctx, YX_ERR_INVALID, "logprob_rows: null tensor or no columns");
     if (stride < cols) return fail(ctx, YX_ERR_INVALID, "logprob_rows: rows lie over one another");
-    if (rows > 0x7fffffffu) return fail(ctx, YX_ERR_INVALID, "logprob_rows: too many rows");
+    if (rows > 0x7fffffffu || cols > 0x7fffffffu) return fail(ctx, YX_ERR_INVALID, "logprob_rows: more than 2^31 rows or columns");
     if (((uintptr_t)logits_dev & (dtype == YX_F32 ? 3u : 1u)) != 0 ||
         (((uintptr_t)logprob_dev | (uintptr_t)entropy_dev | (uintptr_t)top_ids_dev | (uintptr_t)top_logprob_dev) & 3u) != 0)
         return fail(ctx, YX_ERR_INVALID, "logprob_rows: a tensor off its type's alignment");

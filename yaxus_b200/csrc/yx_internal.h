@@ -365,6 +365,7 @@ struct yx_ctx {
         size_t cap = 0;
     };
     Grown lp_ids, lp_logits, lp_stats;     // given tokens; logits of a few rows at a time; statistics by blocks of columns
+    Grown lp_parts;                        // parts of rows of logits, and arrivals there (zero between launches)
     Grown ep_rows, ep_part, ep_counters;   // pass rows copied or in parts; sums of shared tiles, and arrivals there (zero between launches)
     std::vector<void *> outgrown;
 
