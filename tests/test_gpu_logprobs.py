@@ -144,6 +144,21 @@ def test_orders(backend, rows):
         check(x, np.full((rows, 1), cols - 1), 32, r)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,cols", [(1, 60000), (300, 60000), (300, 500001), (2, 2000000)])
+def test_large_ones_in_a_few_places(backend, dtype, rows, cols):
+    # what is largest lies in every 32nd group of 16 bytes, so that one group of threads holds more than the list takes
+    c = torch.arange(cols, device="cuda")
+    wide = 4 if dtype == torch.float32 else 8
+    row = torch.where(c // wide % 32 == 3, 5.0 + (c % 1009) * 0.01, (c % 7) * 0.1).to(dtype)
+    x = row[None].expand(rows, cols).contiguous()
+    ids = np.full((rows, 1), 12)
+    r = backend.logprob_rows(x, ids, top=32, entropy=True)
+    backend.sync()
+    for i in range(0, rows, 100):     # (rows of an odd length begin at other alignments, and are summed in other orders)
+        check(x[i:i + 100], ids[i:i + 100], 32, type(r)(*(t[i:i + 100] for t in r)))
+
+
 def test_large_numbers(backend):
     x = torch.zeros(6, 5000, device="cuda")
     x[0, 17] = INF                      # counts as the largest f32

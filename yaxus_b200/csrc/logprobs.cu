@@ -44,18 +44,20 @@ __device__ __forceinline__ RowStats merge_warp(RowStats r) {
 //
 // One pass over the logits.  A row is cut into parts, a CTA each (one part where there are rows enough to fill the chip), and a
 // part into tiles of 16 logits a thread, the next tile's loads in flight while one is worked on.  A thread keeps the
-// statistics (m, s, t) of what it has seen and moves m only when a tile exceeds it.
+// statistics (m, s, t) of what it has seen and moves m only when a tile exceeds it, and there notes which token it was.
 //
-// The best tokens: whatever exceeds the n-th best found so far goes to a list in shared memory, and the list is cut back
-// to its n best, in order, when it has grown.  The first tile has no n-th best: the n-th largest of 32 groups' largest serves
-// (n numbers are at least that, one of each group), which some n to 4 n logits pass.  Keys of logit and token are all
-// different, so that a row of equal logits passes no more.  The parts' lists and statistics meet in the row's last CTA.
+// The n best tokens of a part come from that: of 32 groups of threads, the n-th largest of the groups' best is a bound that n
+// tokens reach, and only the n or so threads whose best reaches it can hold others that do.  Their logits are read once
+// more, a warp to a thread's, and what reaches the bound (n to some 4 n tokens) is put in order.  Keys of logit and token
+// are all different, so that equal logits reach it no more often.  (With a list that grew as the logits went by, and a
+// barrier a tile for it, 2048 rows of 50257 took 170 us for five tokens and 82 without.)  The parts' tokens and statistics
+// meet in the row's last CTA.
 constexpr int THREADS = 256, WARPS = THREADS / 32;
 constexpr int PER_THREAD = 16;                              // logits of a tile
 constexpr int TILE = THREADS * PER_THREAD;
-constexpr uint32_t MAX_PARTS = 128;                         // of a row: TILE of their best tokens
+constexpr uint32_t MAX_PARTS = 128;                         // of a row
 constexpr uint32_t MAX_SHARED = 2048;                       // parts of all rows that have more than one
-constexpr int LIST_AGAIN = 64;                              // threads that have added to the list, after which it is cut back
+constexpr uint32_t LIST = 2 * THREADS;                      // tokens put in order by counting
 constexpr uint32_t IDS_PARAM = 512;                         // given tokens that ride in kernel-parameter space
 static_assert(MAX_PARTS * YX_TOP_MAX <= TILE, "the last CTA holds the parts' best tokens as one tile");
 
@@ -68,26 +70,27 @@ struct RowsArgs {
     uint32_t *top_ids;
     float *top_logprob;
     float4 *part_stats;                                     // [rows][parts]
-    uint64_t *part_best;                                    // [rows][parts][n_top]
+    uint64_t *part_best;                                    // [rows][n_top][parts]
     uint32_t *arrived;                                      // [rows], zero between launches
     uint32_t ids[IDS_PARAM];
 };
 
-struct List {
-    uint64_t key[YX_TOP_MAX + (LIST_AGAIN + THREADS) * PER_THREAD];   // the best, what has come since, and one more tile
+struct Best {
+    uint64_t key[LIST];
     uint64_t group[WARPS][32];
     uint64_t warp_best[2][WARPS];
-    uint32_t count;
+    uint32_t count, threads;
+    uint32_t thread[THREADS];
 };
 
-// The n-th largest of 32 groups' largest keys; a group is a lane of every warp.  All threads get it.
-__device__ __forceinline__ uint64_t nth_of_groups(List &list, uint64_t best, uint32_t n) {
+// The n-th largest of 32 groups' largest keys; a group is a lane of every warp.  All threads get it, after one barrier.
+__device__ __forceinline__ uint64_t nth_of_groups(Best &b, uint64_t best, uint32_t n) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    list.group[warp][lane] = best;
+    b.group[warp][lane] = best;
     __syncthreads();
-    uint64_t g = list.group[0][lane];
+    uint64_t g = b.group[0][lane];
 #pragma unroll
-    for (int w = 1; w < WARPS; w++) g = max(g, list.group[w][lane]);
+    for (int w = 1; w < WARPS; w++) g = max(g, b.group[w][lane]);
     uint32_t larger = 0;
 #pragma unroll 8
     for (int i = 0; i < 32; i++) {
@@ -97,60 +100,62 @@ __device__ __forceinline__ uint64_t nth_of_groups(List &list, uint64_t best, uin
     return __shfl_sync(0xffffffffu, g, __ffs(__ballot_sync(0xffffffffu, larger == n - 1)) - 1);
 }
 
-// Adds this thread's key to the list if `in`; all lanes of a warp call it together.
-__device__ __forceinline__ void add_to_list(List &list, bool in, uint64_t key) {
+// Adds this thread's key to the list if `in`; all lanes of a warp call it together.  The list's end is not passed, but
+// counted on.
+__device__ __forceinline__ void add_to_list(Best &b, bool in, uint64_t key) {
     const uint32_t mask = __ballot_sync(0xffffffffu, in);
     if (mask == 0) return;
     const int lane = threadIdx.x & 31;
     uint32_t at = 0;
-    if (lane == 0) at = atomicAdd(&list.count, (uint32_t)__popc(mask));
+    if (lane == 0) at = atomicAdd(&b.count, (uint32_t)__popc(mask));
     at = __shfl_sync(0xffffffffu, at, 0) + __popc(mask & ((1u << lane) - 1));
-    if (in) list.key[at] = key;
+    if (in && at < LIST) b.key[at] = key;
 }
 
-// Cuts the list back to its n best, in order; after a barrier, and ends in one.  Returns how many there are.
-__device__ __forceinline__ uint32_t cut_list(List &list, uint32_t n) {
-    const uint32_t count = list.count;
-    if (count <= 2 * THREADS) {
+// The n best of the list, in order, to its front; after a barrier, and ends in one.  If more than LIST have been added, the n
+// best of `source(0 .. size - 1)` instead, a pass over all of it for each (rows made for it: most of the largest logits in one
+// of 32 places of every 128 or 256).
+template <typename F>
+__device__ __forceinline__ void order_list(Best &b, uint32_t n, uint64_t size, F source) {
+    const uint32_t count = b.count;
+    if (count <= LIST) {
         // A key's place is the number of keys above it.
         uint64_t key[2];
         uint32_t place[2] = {0, 0};
 #pragma unroll
-        for (int j = 0; j < 2; j++) key[j] = threadIdx.x + j * THREADS < count ? list.key[threadIdx.x + j * THREADS] : 0;
-        for (uint32_t i = 0; i < count; i++) {
-            const uint64_t other = list.key[i];
+        for (int j = 0; j < 2; j++) key[j] = threadIdx.x + j * THREADS < count ? b.key[threadIdx.x + j * THREADS] : 0;
+        if (threadIdx.x < count) {
+#pragma unroll 4
+            for (uint32_t i = 0; i < count; i++) {
+                const uint64_t other = b.key[i];
 #pragma unroll
-            for (int j = 0; j < 2; j++) place[j] += other > key[j];
+                for (int j = 0; j < 2; j++) place[j] += other > key[j];
+            }
         }
         __syncthreads();
 #pragma unroll
         for (int j = 0; j < 2; j++)
-            if (key[j] != 0 && place[j] < n) list.key[place[j]] = key[j];
+            if (key[j] != 0 && place[j] < n) b.key[place[j]] = key[j];
     } else {
-        // (a row whose logits rise: nearly all of a tile is on the list)
         uint64_t below = ~0ull, mine = 0;
         for (uint32_t k = 0; k < n; k++) {
-            uint64_t b = 0;
-            for (uint32_t i = threadIdx.x; i < count; i += THREADS) {
-                const uint64_t key = list.key[i];
-                if (key < below && key > b) b = key;
+            uint64_t best = 0;
+            for (uint64_t i = threadIdx.x; i < size; i += THREADS) {
+                const uint64_t key = source(i);
+                if (key < below && key > best) best = key;
             }
 #pragma unroll
-            for (int d = 16; d > 0; d >>= 1) b = max(b, __shfl_xor_sync(0xffffffffu, b, d));
-            if ((threadIdx.x & 31) == 0) list.warp_best[k & 1][threadIdx.x >> 5] = b;
+            for (int d = 16; d > 0; d >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, d));
+            if ((threadIdx.x & 31) == 0) b.warp_best[k & 1][threadIdx.x >> 5] = best;
             __syncthreads();
-            b = list.warp_best[k & 1][0];
 #pragma unroll
-            for (int w = 1; w < WARPS; w++) b = max(b, list.warp_best[k & 1][w]);
-            below = b;
-            if (threadIdx.x == k) mine = b;
+            for (int w = 0; w < WARPS; w++) best = max(best, b.warp_best[k & 1][w]);
+            below = best;
+            if (threadIdx.x == k) mine = best;
         }
-        __syncthreads();
-        if (threadIdx.x < n) list.key[threadIdx.x] = mine;
+        if (threadIdx.x < n) b.key[threadIdx.x] = mine;   // (all have read the list's count; nobody reads its keys)
     }
-    if (threadIdx.x == 0) list.count = min(count, n);
     __syncthreads();
-    return min(count, n);
 }
 
 // The statistics of all of the CTA's threads, in all of them; `scratch` is the caller's alone.
@@ -164,18 +169,18 @@ __device__ __forceinline__ RowStats merge_cta(RowStats r, RowStats *scratch) {
     return r;
 }
 
-template <int DTYPE>
+template <int DTYPE, int N = PER_THREAD>
 struct Tile {
     static constexpr int WIDE = DTYPE == YX_F32 ? 4 : 8;   // logits in 16 bytes
-    static constexpr int VECS = PER_THREAD / WIDE;
+    static constexpr int VECS = N / WIDE;
     uint4 v[VECS];
 
-    // Vectors first, first + THREADS, ... of a row whose logit 0 is element `shift` of vector 0; what lies before the row, behind
+    // Vectors first, first + step, ... of a row whose logit 0 is element `shift` of vector 0; what lies before the row, behind
     // it, or at or behind vector `end` counts as forbidden.
-    __device__ __forceinline__ void load(const char *base, uint32_t shift, uint32_t cols, uint64_t first, uint64_t end) {
+    __device__ __forceinline__ void load(const char *base, uint32_t shift, uint32_t cols, uint64_t first, uint32_t step, uint64_t end) {
 #pragma unroll
         for (int i = 0; i < VECS; i++) {
-            const uint64_t vec = first + (uint64_t)i * THREADS, c = vec * WIDE;
+            const uint64_t vec = first + (uint64_t)i * step, c = vec * WIDE;
             constexpr uint32_t none = DTYPE == YX_F32 ? 0xff800000u : DTYPE == YX_F16 ? 0xfc00fc00u : 0xff80ff80u;
             v[i] = make_uint4(none, none, none, none);
             if (vec >= end) continue;
@@ -193,7 +198,7 @@ struct Tile {
             }
         }
     }
-    __device__ __forceinline__ void unpack(float (&x)[PER_THREAD]) const {
+    __device__ __forceinline__ void unpack(float (&x)[N]) const {
 #pragma unroll
         for (int i = 0; i < VECS; i++) {
             const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
@@ -209,16 +214,12 @@ struct Tile {
             }
         }
     }
-    // The token of element j; past any vocabulary before the row and at or behind vector `end`.
-    static __device__ __forceinline__ uint32_t token(uint64_t first, int j, uint32_t shift, uint64_t end) {
-        const uint64_t vec = first + (uint64_t)(j / WIDE) * THREADS;
-        return vec < end ? (uint32_t)(vec * WIDE) + j % WIDE - shift : 0xffffffffu;
-    }
+    static __device__ __forceinline__ uint32_t first_token(uint64_t vec, uint32_t shift) { return vec * WIDE > shift ? (uint32_t)(vec * WIDE) - shift : 0u; }
 };
 
 template <int DTYPE, bool TOP>
 __global__ void __launch_bounds__(THREADS, 4) logprob_rows_kernel(const __grid_constant__ RowsArgs a) {
-    __shared__ List list;
+    __shared__ Best b;
     __shared__ RowStats scratch[2][WARPS];
     __shared__ bool last;
     using T = Tile<DTYPE>;
@@ -230,16 +231,14 @@ __global__ void __launch_bounds__(THREADS, 4) logprob_rows_kernel(const __grid_c
     const char *base = logits - shift * ES;
     const uint64_t vecs = ((uint64_t)shift + a.cols + T::WIDE - 1) / T::WIDE;
     const uint64_t v0 = vecs * part / a.parts, v1 = vecs * (part + 1) / a.parts;
-    if (TOP && threadIdx.x == 0) list.count = 0;
 
     RowStats r = no_stats();
-    float least = -INFINITY;   // the n-th best logit found, once there are n
-    int added = 0;
+    uint32_t token = T::first_token(v0 + threadIdx.x, shift);   // the first of this thread's largest logits
     T next;
-    next.load(base, shift, a.cols, v0 + threadIdx.x, v1);
-    for (uint64_t v = v0; v < v1; v += T::VECS * THREADS) {
+    next.load(base, shift, a.cols, v0 + threadIdx.x, THREADS, v1);
+    for (uint64_t v = v0 + threadIdx.x; v < v1; v += T::VECS * THREADS) {
         const T tile = next;
-        next.load(base, shift, a.cols, v + T::VECS * THREADS + threadIdx.x, v1);
+        next.load(base, shift, a.cols, v + T::VECS * THREADS, THREADS, v1);
         float x[PER_THREAD];
         tile.unpack(x);
         float most = x[0];
@@ -250,6 +249,13 @@ __global__ void __launch_bounds__(THREADS, 4) logprob_rows_kernel(const __grid_c
 #pragma unroll
                 for (int j = 0; j < PER_THREAD; j++) x[j] = clean(x[j]);
                 most = clean(most);
+            }
+            if constexpr (TOP) {
+                int at = 0;
+#pragma unroll
+                for (int j = PER_THREAD - 1; j >= 0; j--)
+                    if (x[j] == most) at = j;
+                token = (uint32_t)((v + (uint64_t)(at / T::WIDE) * THREADS) * T::WIDE) + at % T::WIDE - shift;
             }
             const float d = distance(r.m, most), c = fast_exp2(d * LOG2_E);
             r.t = c * (r.t + d * r.s);
@@ -262,51 +268,44 @@ __global__ void __launch_bounds__(THREADS, 4) logprob_rows_kernel(const __grid_c
             r.s += e;
             r.t += e * d;
         }
-        if constexpr (TOP) {
-            if (v == v0) {
-                uint64_t best = 0;
+    }
+    if constexpr (TOP) {
+        if (threadIdx.x == 0) b.count = b.threads = 0;
+        const uint64_t mine = v0 + threadIdx.x < v1 ? key_of(r.m, token) : 0;
+        const uint64_t least = nth_of_groups(b, mine, a.n_top);
+        if (mine != 0 && mine >= least) b.thread[atomicAdd(&b.threads, 1u)] = threadIdx.x;
+        __syncthreads();
+        const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+        for (uint32_t i = warp; i < b.threads; i += WARPS) {
+            for (uint64_t v = v0 + b.thread[i]; v < v1; v += 32 * THREADS) {
+                const uint64_t own = v + (uint64_t)lane * THREADS;
+                Tile<DTYPE, T::WIDE> again;
+                again.load(base, shift, a.cols, own, 0, v1);
+                float x[T::WIDE];
+                again.unpack(x);
 #pragma unroll
-                for (int j = PER_THREAD - 1; j >= 0; j--) {
-                    const uint32_t token = T::token(v + threadIdx.x, j, shift, v1);
-                    if (token < a.cols) best = max(best, key_of(x[j], token));
+                for (int e = 0; e < T::WIDE; e++) {
+                    const uint32_t t = (uint32_t)(own * T::WIDE) + e - shift;
+                    const uint64_t key = own < v1 && t < a.cols ? key_of(x[e], t) : 0;
+                    add_to_list(b, key != 0 && key >= least, key);
                 }
-                const uint64_t least_key = nth_of_groups(list, best, a.n_top);
-#pragma unroll
-                for (int j = 0; j < PER_THREAD; j++) {
-                    const uint32_t token = T::token(v + threadIdx.x, j, shift, v1);
-                    const uint64_t key = token < a.cols ? key_of(x[j], token) : 0;
-                    add_to_list(list, key != 0 && key >= least_key, key);
-                }
-            } else if (__any_sync(0xffffffffu, most > least)) {
-                // (tokens come in order: an equal one later is no better)
-#pragma unroll
-                for (int j = 0; j < PER_THREAD; j++) add_to_list(list, x[j] > least, key_of(x[j], T::token(v + threadIdx.x, j, shift, v1)));
-            }
-            // (counted by the barrier itself: the list's own count may be moving again when the last thread reads it)
-            added += __syncthreads_count(v == v0 || most > least);
-            if (added > LIST_AGAIN) {
-                added = 0;
-                if (cut_list(list, a.n_top) == a.n_top) least = key_logit(list.key[a.n_top - 1]);
-                __syncthreads();
             }
         }
-    }
-    uint32_t found = 0;
-    if constexpr (TOP) {
         __syncthreads();
-        found = cut_list(list, a.n_top);
+        const uint64_t t0 = v0 * T::WIDE > shift ? v0 * T::WIDE - shift : 0, t1 = min((uint64_t)a.cols, v1 * T::WIDE - shift);
+        order_list(b, a.n_top, t1 - t0, [&](uint64_t i) { return key_of(load_as_f32(logits, DTYPE, t0 + i), (uint32_t)(t0 + i)); });
     }
     r = merge_cta(r, scratch[0]);
     if (a.parts > 1) {
-        const size_t mine = (size_t)row * a.parts + part;
-        if constexpr (TOP)
-            if (threadIdx.x < a.n_top) __stcg(a.part_best + mine * a.n_top + threadIdx.x, threadIdx.x < found ? list.key[threadIdx.x] : 0ull);
-        if (threadIdx.x == 0) __stcg(a.part_stats + mine, make_float4(r.m, r.s, r.t, 0.0f));
+        if constexpr (TOP)   // (a part of fewer than n_top tokens has them all on the list)
+            if (threadIdx.x < a.n_top) __stcg(a.part_best + ((size_t)row * a.n_top + threadIdx.x) * a.parts + part, threadIdx.x < b.count ? b.key[threadIdx.x] : 0ull);
+        if (threadIdx.x == 0) __stcg(a.part_stats + (size_t)row * a.parts + part, make_float4(r.m, r.s, r.t, 0.0f));
         __threadfence();
         __syncthreads();
         if (threadIdx.x == 0) {
             last = atomicAdd(a.arrived + row, 1u) + 1 == a.parts;
             if (last) a.arrived[row] = 0u;
+            b.count = 0;
         }
         __syncthreads();
         if (!last) return;
@@ -317,6 +316,7 @@ __global__ void __launch_bounds__(THREADS, 4) logprob_rows_kernel(const __grid_c
             r = RowStats{f.x, f.y, f.z};
         }
         if constexpr (TOP) {
+            // (best ones first, so that the groups' largest are the parts' first few)
             const uint32_t keys = a.parts * a.n_top;
             const uint64_t *from = a.part_best + (size_t)row * keys;
             uint64_t key[PER_THREAD], best = 0;
@@ -326,15 +326,14 @@ __global__ void __launch_bounds__(THREADS, 4) logprob_rows_kernel(const __grid_c
                 key[j] = i < keys ? __ldcg(from + i) : 0;
                 best = max(best, key[j]);
             }
-            if (threadIdx.x == 0) list.count = 0;
-            const uint64_t least_key = nth_of_groups(list, best, a.n_top);
+            const uint64_t least = nth_of_groups(b, best, a.n_top);
 #pragma unroll
             for (int j = 0; j < PER_THREAD; j++) {
                 if (j * THREADS >= keys) break;
-                add_to_list(list, key[j] != 0 && key[j] >= least_key, key[j]);
+                add_to_list(b, key[j] != 0 && key[j] >= least, key[j]);
             }
             __syncthreads();
-            cut_list(list, a.n_top);
+            order_list(b, a.n_top, keys, [&](uint64_t i) { return __ldcg(from + i); });
         }
         r = merge_cta(r, scratch[1]);
     }
@@ -345,7 +344,7 @@ __global__ void __launch_bounds__(THREADS, 4) logprob_rows_kernel(const __grid_c
     if (threadIdx.x == 0 && a.entropy) a.entropy[row] = entropy(r);
     if constexpr (TOP) {
         if (threadIdx.x < a.n_top) {
-            const uint64_t key = list.key[threadIdx.x];
+            const uint64_t key = b.key[threadIdx.x];
             a.top_ids[(size_t)row * a.n_top + threadIdx.x] = key_token(key);
             a.top_logprob[(size_t)row * a.n_top + threadIdx.x] = log_prob(key_logit(key), r.m, log_s);
         }
