@@ -160,17 +160,19 @@ def test_large_ones_in_a_few_places(backend, dtype, rows, cols):
 
 
 def test_large_numbers(backend):
-    x = torch.zeros(6, 5000, device="cuda")
+    x = torch.zeros(7, 5000, device="cuda")
     x[0, 17] = INF                      # counts as the largest f32
     x[1, 17], x[1, 4000] = INF, MOST    # ... and is equal to it
     x[2] = MOST
     x[3] = -MOST
     x[4, 9] = 1e30
     x[5, 9], x[5, 10] = MOST, -MOST     # a distance past f32
-    ids = np.tile(np.array([17, 4000, 9, 10]), (6, 1))
+    x[6, 9], x[6, 10] = MOST, INF       # equal, and one thread's
+    ids = np.tile(np.array([17, 4000, 9, 10]), (7, 1))
     r = backend.logprob_rows(x, ids, top=4, entropy=True)
     backend.sync()
     check(x, ids, 4, r)
+    check(x, ids, 1, backend.logprob_rows(x, ids, top=1, entropy=True))
     assert r.logprob[0, 0] == 0 and r.top_ids[1].tolist() == [17, 4000, 0, 1]
 
 

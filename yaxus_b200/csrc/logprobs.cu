@@ -44,20 +44,20 @@ __device__ __forceinline__ RowStats merge_warp(RowStats r) {
 //
 // One pass over the logits.  A row is cut into parts, a CTA each (one part where there are rows enough to fill the chip), and a
 // part into tiles of 16 logits a thread, the next tile's loads in flight while one is worked on.  A thread keeps the
-// statistics (m, s, t) of what it has seen and moves m only when a tile exceeds it, and there notes which token it was.
+// statistics (m, s, t) of what it has seen, m any number near its largest logit, and notes the tile that has that.
 //
 // The n best tokens of a part come from that: of 32 groups of threads, the n-th largest of the groups' best is a bound that n
 // tokens reach, and only the n or so threads whose best reaches it can hold others that do.  Their logits are read once
-// more, a warp to a thread's, and what reaches the bound (n to some 4 n tokens) is put in order.  Keys of logit and token
-// are all different, so that equal logits reach it no more often.  (With a list that grew as the logits went by, and a
+// more, a warp to a thread's, and what reaches the bound (n to some 4 n tokens) is put in order.  Where too many logits
+// equal it the bound is a key of logit and token, which are all different.  (With a list that grew as the logits went by, and a
 // barrier a tile for it, 2048 rows of 50257 took 170 us for five tokens and 82 without.)  The parts' tokens and statistics
 // meet in the row's last CTA.
 constexpr int THREADS = 256, WARPS = THREADS / 32;
 constexpr int PER_THREAD = 16;                              // logits of a tile
 constexpr int TILE = THREADS * PER_THREAD;
 constexpr uint32_t MAX_PARTS = 128;                         // of a row
-constexpr uint32_t MAX_SHARED = 2048;                       // parts of all rows that have more than one
-constexpr uint32_t LIST = 2 * THREADS;                      // tokens put in order by counting
+constexpr uint32_t MAX_SHARED = 2048;                        // parts of all rows that have more than one
+constexpr uint32_t LIST = 512;                              // tokens put in order by counting
 constexpr uint32_t IDS_PARAM = 512;                         // given tokens that ride in kernel-parameter space
 static_assert(MAX_PARTS * YX_TOP_MAX <= TILE, "the last CTA holds the parts' best tokens as one tile");
 
@@ -79,25 +79,30 @@ struct Best {
     uint64_t key[LIST];
     uint64_t group[WARPS][32];
     uint64_t warp_best[2][WARPS];
+    uint64_t least;
     uint32_t count, threads;
-    uint32_t thread[THREADS];
+    uint8_t thread[THREADS];
 };
 
-// The n-th largest of 32 groups' largest keys; a group is a lane of every warp.  All threads get it, after one barrier.
+// The n-th largest of 32 groups' largest keys; a group is a lane of every warp.  All threads get it, after two barriers.
 __device__ __forceinline__ uint64_t nth_of_groups(Best &b, uint64_t best, uint32_t n) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     b.group[warp][lane] = best;
     __syncthreads();
-    uint64_t g = b.group[0][lane];
+    if (warp == 0) {
+        uint64_t g = best;
 #pragma unroll
-    for (int w = 1; w < WARPS; w++) g = max(g, b.group[w][lane]);
-    uint32_t larger = 0;
-#pragma unroll 8
-    for (int i = 0; i < 32; i++) {
-        const uint64_t other = __shfl_sync(0xffffffffu, g, i);
-        larger += other > g || (other == g && i < lane);   // (groups without a token share key 0)
+        for (int w = 1; w < WARPS; w++) g = max(g, b.group[w][lane]);
+        uint32_t larger = 0;
+#pragma unroll
+        for (int i = 0; i < 32; i++) {
+            const uint64_t other = __shfl_sync(0xffffffffu, g, i);
+            larger += other > g || (other == g && i < lane);   // (groups without a token share key 0)
+        }
+        if (larger == n - 1) b.least = g;
     }
-    return __shfl_sync(0xffffffffu, g, __ffs(__ballot_sync(0xffffffffu, larger == n - 1)) - 1);
+    __syncthreads();
+    return b.least;
 }
 
 // Adds this thread's key to the list if `in`; all lanes of a warp call it together.  The list's end is not passed, but
@@ -116,31 +121,32 @@ __device__ __forceinline__ void add_to_list(Best &b, bool in, uint64_t key) {
 // best of `source(0 .. size - 1)` instead, a pass over all of it for each (rows made for it: most of the largest logits in one
 // of 32 places of every 128 or 256).
 template <typename F>
-__device__ __forceinline__ void order_list(Best &b, uint32_t n, uint64_t size, F source) {
+__device__ __forceinline__ void order_list(Best &b, uint32_t n, uint32_t size, F source) {
     const uint32_t count = b.count;
     if (count <= LIST) {
         // A key's place is the number of keys above it.
-        uint64_t key[2];
-        uint32_t place[2] = {0, 0};
+        constexpr int EACH = LIST / THREADS;
+        uint64_t key[EACH];
+        uint32_t place[EACH] = {};
 #pragma unroll
-        for (int j = 0; j < 2; j++) key[j] = threadIdx.x + j * THREADS < count ? b.key[threadIdx.x + j * THREADS] : 0;
+        for (int j = 0; j < EACH; j++) key[j] = threadIdx.x + j * THREADS < count ? b.key[threadIdx.x + j * THREADS] : 0;
         if (threadIdx.x < count) {
 #pragma unroll 4
             for (uint32_t i = 0; i < count; i++) {
                 const uint64_t other = b.key[i];
 #pragma unroll
-                for (int j = 0; j < 2; j++) place[j] += other > key[j];
+                for (int j = 0; j < EACH; j++) place[j] += other > key[j];
             }
         }
         __syncthreads();
 #pragma unroll
-        for (int j = 0; j < 2; j++)
+        for (int j = 0; j < EACH; j++)
             if (key[j] != 0 && place[j] < n) b.key[place[j]] = key[j];
     } else {
         uint64_t below = ~0ull, mine = 0;
         for (uint32_t k = 0; k < n; k++) {
             uint64_t best = 0;
-            for (uint64_t i = threadIdx.x; i < size; i += THREADS) {
+            for (uint32_t i = threadIdx.x; i < size; i += THREADS) {
                 const uint64_t key = source(i);
                 if (key < below && key > best) best = key;
             }
@@ -158,14 +164,56 @@ __device__ __forceinline__ void order_list(Best &b, uint32_t n, uint64_t size, F
     __syncthreads();
 }
 
-// The statistics of all of the CTA's threads, in all of them; `scratch` is the caller's alone.
-__device__ __forceinline__ RowStats merge_cta(RowStats r, RowStats *scratch) {
-    r = merge_warp(r);
-    if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = r;
-    __syncthreads();
-    r = scratch[0];
+__device__ __forceinline__ float warp_max(float v) {   // (passes over what is no number)
+    float r;
+    asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+    return r;
+}
+// (s, t) of statistics under another m
+__device__ __forceinline__ RowStats moved(RowStats r, float m) {
+    const float d = distance(r.m, m), c = fast_exp2(d * LOG2_E);
+    return RowStats{m, c * r.s, c * (r.t + d * r.s)};
+}
+template <int LANES>
+__device__ __forceinline__ RowStats warp_sum(RowStats r) {
+    r = moved(r, warp_max(r.m));
 #pragma unroll
-    for (int i = 1; i < WARPS; i++) r = merge(r, scratch[i]);
+    for (int d = LANES / 2; d > 0; d >>= 1) {
+        r.s += __shfl_xor_sync(0xffffffffu, r.s, d);
+        r.t += __shfl_xor_sync(0xffffffffu, r.t, d);
+    }
+    return r;
+}
+// The statistics of all of the CTA's threads: share_stats by all, a barrier, all_stats.
+__device__ __forceinline__ void share_stats(RowStats r, RowStats *scratch) {
+    r = warp_sum<32>(r);
+    if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = r;
+}
+__device__ __forceinline__ RowStats all_stats(const RowStats *scratch) { return warp_sum<WARPS>(scratch[threadIdx.x & (WARPS - 1)]); }
+
+// Two f32 at a time (add.f32x2 and the like: half the issue slots).
+struct F2 {
+    uint64_t bits;
+};
+__device__ __forceinline__ F2 f2(float a, float b) {
+    F2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r.bits) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void split(F2 v, float &a, float &b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v.bits)); }
+__device__ __forceinline__ F2 operator+(F2 a, F2 b) {
+    F2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.bits) : "l"(a.bits), "l"(b.bits));
+    return r;
+}
+__device__ __forceinline__ F2 operator*(F2 a, F2 b) {
+    F2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.bits) : "l"(a.bits), "l"(b.bits));
+    return r;
+}
+__device__ __forceinline__ F2 fma(F2 a, F2 b, F2 c) {
+    F2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.bits) : "l"(a.bits), "l"(b.bits), "l"(c.bits));
     return r;
 }
 
@@ -175,24 +223,31 @@ struct Tile {
     static constexpr int VECS = N / WIDE;
     uint4 v[VECS];
 
-    // Vectors first, first + step, ... of a row whose logit 0 is element `shift` of vector 0; what lies before the row, behind
-    // it, or at or behind vector `end` counts as forbidden.
-    __device__ __forceinline__ void load(const char *base, uint32_t shift, uint32_t cols, uint64_t first, uint32_t step, uint64_t end) {
+    // Vectors first, first + step, ... , all inside the row.
+    __device__ __forceinline__ void load_inside(const char *base, uint32_t first, uint32_t step) {
+        const uint4 *p = (const uint4 *)base + first;
+#pragma unroll
+        for (int i = 0; i < VECS; i++) v[i] = __ldg(p + (size_t)i * step);
+    }
+    // The same of a row whose logit 0 is element `shift` of vector 0: what lies before the row, behind it, or at or behind
+    // vector `end` counts as forbidden.
+    __device__ __forceinline__ void load(const char *base, uint32_t shift, uint32_t cols, uint32_t first, uint32_t step, uint32_t end) {
 #pragma unroll
         for (int i = 0; i < VECS; i++) {
-            const uint64_t vec = first + (uint64_t)i * step, c = vec * WIDE;
+            const uint32_t vec = first + i * step;
+            const uint64_t c = (uint64_t)vec * WIDE;
             constexpr uint32_t none = DTYPE == YX_F32 ? 0xff800000u : DTYPE == YX_F16 ? 0xfc00fc00u : 0xff80ff80u;
             v[i] = make_uint4(none, none, none, none);
             if (vec >= end) continue;
             if (c >= shift && c + WIDE <= (uint64_t)shift + cols) {
-                v[i] = __ldcs((const uint4 *)(base + vec * 16));
+                v[i] = __ldg((const uint4 *)base + vec);
             } else {
                 uint32_t w[4] = {none, none, none, none};
 #pragma unroll
                 for (int e = 0; e < WIDE; e++) {
                     if (c + e < shift || c + e >= (uint64_t)shift + cols) continue;
-                    if constexpr (DTYPE == YX_F32) w[e] = *(const uint32_t *)(base + vec * 16 + e * 4);
-                    else w[e / 2] = (w[e / 2] & (e & 1 ? 0xffffu : 0xffff0000u)) | (uint32_t)*(const uint16_t *)(base + vec * 16 + e * 2) << (e & 1 ? 16 : 0);
+                    if constexpr (DTYPE == YX_F32) w[e] = *((const uint32_t *)base + c + e);
+                    else w[e / 2] = (w[e / 2] & (e & 1 ? 0xffffu : 0xffff0000u)) | (uint32_t)*((const uint16_t *)base + c + e) << (e & 1 ? 16 : 0);
                 }
                 v[i] = make_uint4(w[0], w[1], w[2], w[3]);
             }
@@ -214,8 +269,12 @@ struct Tile {
             }
         }
     }
-    static __device__ __forceinline__ uint32_t first_token(uint64_t vec, uint32_t shift) { return vec * WIDE > shift ? (uint32_t)(vec * WIDE) - shift : 0u; }
+    static __device__ __forceinline__ uint32_t first_token(uint32_t vec, uint32_t shift) { return vec > 0 ? vec * WIDE - shift : 0u; }
 };
+
+// How far a logit may exceed the m of the statistics before m moves: exp(8) of it still adds up without harm, and after the
+// first tile hardly any thread's m moves again (with m the largest so far, some lane of a warp moved it in most tiles).
+constexpr float HEADROOM = 8.0f;
 
 template <int DTYPE, bool TOP>
 __global__ void __launch_bounds__(THREADS, 4) logprob_rows_kernel(const __grid_constant__ RowsArgs a) {
@@ -229,80 +288,133 @@ __global__ void __launch_bounds__(THREADS, 4) logprob_rows_kernel(const __grid_c
     const char *logits = (const char *)a.logits + (size_t)row * a.stride * ES;
     const uint32_t shift = (uint32_t)((uintptr_t)logits & 15u) / ES;
     const char *base = logits - shift * ES;
-    const uint64_t vecs = ((uint64_t)shift + a.cols + T::WIDE - 1) / T::WIDE;
-    const uint64_t v0 = vecs * part / a.parts, v1 = vecs * (part + 1) / a.parts;
+    const uint32_t vecs = (uint32_t)(((uint64_t)shift + a.cols + T::WIDE - 1) / T::WIDE);
+    const uint32_t v0 = (uint32_t)((uint64_t)vecs * part / a.parts), v1 = (uint32_t)((uint64_t)vecs * (part + 1) / a.parts);
+    // Tiles that begin in [in0, in1) lie inside the row and the part.
+    constexpr uint32_t STEP = T::VECS * THREADS;
+    const uint32_t in0 = shift > 0 && part == 0 ? 1 : v0, inside = min(v1, (uint32_t)(((uint64_t)shift + a.cols) / T::WIDE));
+    const uint32_t in1 = inside >= STEP - 1 ? inside - (STEP - 1) : 0;
+
+    // The first given token's logit is asked for at once: behind the sums it would be one more trip to memory.
+    const uint32_t *ids = (a.ids_dev ? a.ids_dev : a.ids) + (size_t)row * a.n_ids;
+    const float given = threadIdx.x < a.n_ids ? load_as_f32(logits, DTYPE, ids[threadIdx.x]) : 0.0f;
 
     RowStats r = no_stats();
-    uint32_t token = T::first_token(v0 + threadIdx.x, shift);   // the first of this thread's largest logits
+    F2 s2 = f2(0.0f, 0.0f), t2 = s2;
+    float best = -INFINITY;
+    uint32_t best_at = 0xffffffffu;   // the tile of the first of this thread's largest logits
     T next;
-    next.load(base, shift, a.cols, v0 + threadIdx.x, THREADS, v1);
-    for (uint64_t v = v0 + threadIdx.x; v < v1; v += T::VECS * THREADS) {
+    auto load = [&](uint32_t v) {
+        if (v >= in0 && v < in1) next.load_inside(base, v + threadIdx.x, THREADS);
+        else next.load(base, shift, a.cols, v + threadIdx.x, THREADS, v1);
+    };
+    load(v0);
+    for (uint32_t v = v0; v < v1; v += STEP) {
         const T tile = next;
-        next.load(base, shift, a.cols, v + T::VECS * THREADS, THREADS, v1);
+        if (v + STEP < v1) load(v + STEP);
         float x[PER_THREAD];
         tile.unpack(x);
         float most = x[0];
 #pragma unroll
         for (int j = 1; j < PER_THREAD; j++) most = fmaxf(most, x[j]);
-        if (most > r.m) {
+        if (TOP && clean(most) > best) {
+            best = clean(most);
+            best_at = v;
+        }
+        if (most > r.m + HEADROOM) {
             if (most == INFINITY) {
 #pragma unroll
                 for (int j = 0; j < PER_THREAD; j++) x[j] = clean(x[j]);
                 most = clean(most);
             }
-            if constexpr (TOP) {
+            const float d = distance(r.m, most), c = fast_exp2(d * LOG2_E);
+            t2 = f2(c, c) * fma(f2(d, d), s2, t2);
+            s2 = f2(c, c) * s2;
+            r.m = most;
+        }
+        const F2 minus_m = f2(-r.m, -r.m), log2_e = f2(LOG2_E, LOG2_E);
+#pragma unroll
+        for (int j = 0; j < PER_THREAD; j += 2) {
+            float d0, d1, y0, y1;
+            split(f2(x[j], x[j + 1]) + minus_m, d0, d1);
+            const F2 d = f2(fmaxf(d0, LEAST_DISTANCE), fmaxf(d1, LEAST_DISTANCE));   // (see distance())
+            split(d * log2_e, y0, y1);
+            const F2 e = f2(fast_exp2(y0), fast_exp2(y1));
+            s2 = s2 + e;
+            t2 = fma(e, d, t2);
+        }
+    }
+    {
+        float x, y;
+        split(s2, x, y);
+        r.s = x + y;
+        split(t2, x, y);
+        r.t = x + y;
+    }
+    share_stats(r, scratch[0]);
+    if constexpr (TOP) {
+        const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+        // Puts on the list what `reaches` of the logits of the threads that are `in`; between barriers.
+        auto look_again = [&](bool in, auto reaches) {
+            if (in) b.thread[atomicAdd(&b.threads, 1u)] = (uint8_t)threadIdx.x;
+            __syncthreads();
+            for (uint32_t i = warp; i < b.threads; i += WARPS) {
+                for (uint32_t v = v0 + b.thread[i]; v < v1; v += 32 * THREADS) {
+                    if (__any_sync(0xffffffffu, *(volatile uint32_t *)&b.count > LIST)) break;
+                    const uint32_t own = v + lane * THREADS;
+                    Tile<DTYPE, T::WIDE> again;
+                    again.load(base, shift, a.cols, own, 0, v1);
+                    float x[T::WIDE];
+                    again.unpack(x);
+#pragma unroll
+                    for (int e = 0; e < T::WIDE; e++) {
+                        const uint32_t t = own * T::WIDE + e - shift;
+                        add_to_list(b, own < v1 && t < a.cols && reaches(x[e], t), key_of(x[e], t));
+                    }
+                }
+            }
+            __syncthreads();
+        };
+        if (threadIdx.x == 0) b.count = b.threads = 0;
+        // The bound is a logit; only where too many equal it (or it is the forbidden's) is it a logit and a token.
+        const uint64_t bound = nth_of_groups(b, v0 + threadIdx.x < v1 ? key_of(best, 0) : 0, a.n_top);
+        const float least = key_logit(bound);
+        bool precise = bound == 0 || least == -INFINITY;
+        if (!precise) {
+            look_again(best >= least, [&](float x, uint32_t) { return x >= least; });
+            precise = b.count > LIST;
+            __syncthreads();
+        }
+        if (precise) {
+            uint32_t token = T::first_token(v0 + threadIdx.x, shift);   // (all of them -inf or no number)
+            if (best_at != 0xffffffffu) {
+                next.load(base, shift, a.cols, best_at + threadIdx.x, THREADS, v1);
+                float x[PER_THREAD];
+                next.unpack(x);
                 int at = 0;
 #pragma unroll
                 for (int j = PER_THREAD - 1; j >= 0; j--)
-                    if (x[j] == most) at = j;
-                token = (uint32_t)((v + (uint64_t)(at / T::WIDE) * THREADS) * T::WIDE) + at % T::WIDE - shift;
+                    if (clean(x[j]) == best) at = j;
+                token = (best_at + threadIdx.x + at / T::WIDE * THREADS) * T::WIDE + at % T::WIDE - shift;
             }
-            const float d = distance(r.m, most), c = fast_exp2(d * LOG2_E);
-            r.t = c * (r.t + d * r.s);
-            r.s *= c;
-            r.m = most;
+            if (threadIdx.x == 0) b.count = b.threads = 0;
+            const uint64_t mine = v0 + threadIdx.x < v1 ? key_of(best, token) : 0;
+            const uint64_t reached = nth_of_groups(b, mine, a.n_top);
+            look_again(mine != 0 && mine >= reached, [&](float x, uint32_t t) { return key_of(x, t) >= reached; });
         }
-#pragma unroll
-        for (int j = 0; j < PER_THREAD; j++) {
-            const float d = distance(x[j], r.m), e = fast_exp2(d * LOG2_E);
-            r.s += e;
-            r.t += e * d;
-        }
-    }
-    if constexpr (TOP) {
-        if (threadIdx.x == 0) b.count = b.threads = 0;
-        const uint64_t mine = v0 + threadIdx.x < v1 ? key_of(r.m, token) : 0;
-        const uint64_t least = nth_of_groups(b, mine, a.n_top);
-        if (mine != 0 && mine >= least) b.thread[atomicAdd(&b.threads, 1u)] = threadIdx.x;
+        const uint32_t t0 = T::first_token(v0, shift), t1 = min(a.cols, v1 * T::WIDE - shift);
+        order_list(b, a.n_top, t1 - t0, [&](uint32_t i) { return key_of(load_as_f32(logits, DTYPE, t0 + i), t0 + i); });
+    } else {
         __syncthreads();
-        const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-        for (uint32_t i = warp; i < b.threads; i += WARPS) {
-            for (uint64_t v = v0 + b.thread[i]; v < v1; v += 32 * THREADS) {
-                const uint64_t own = v + (uint64_t)lane * THREADS;
-                Tile<DTYPE, T::WIDE> again;
-                again.load(base, shift, a.cols, own, 0, v1);
-                float x[T::WIDE];
-                again.unpack(x);
-#pragma unroll
-                for (int e = 0; e < T::WIDE; e++) {
-                    const uint32_t t = (uint32_t)(own * T::WIDE) + e - shift;
-                    const uint64_t key = own < v1 && t < a.cols ? key_of(x[e], t) : 0;
-                    add_to_list(b, key != 0 && key >= least, key);
-                }
-            }
-        }
-        __syncthreads();
-        const uint64_t t0 = v0 * T::WIDE > shift ? v0 * T::WIDE - shift : 0, t1 = min((uint64_t)a.cols, v1 * T::WIDE - shift);
-        order_list(b, a.n_top, t1 - t0, [&](uint64_t i) { return key_of(load_as_f32(logits, DTYPE, t0 + i), (uint32_t)(t0 + i)); });
     }
-    r = merge_cta(r, scratch[0]);
+    r = all_stats(scratch[0]);
     if (a.parts > 1) {
         if constexpr (TOP)   // (a part of fewer than n_top tokens has them all on the list)
             if (threadIdx.x < a.n_top) __stcg(a.part_best + ((size_t)row * a.n_top + threadIdx.x) * a.parts + part, threadIdx.x < b.count ? b.key[threadIdx.x] : 0ull);
         if (threadIdx.x == 0) __stcg(a.part_stats + (size_t)row * a.parts + part, make_float4(r.m, r.s, r.t, 0.0f));
-        __threadfence();
         __syncthreads();
         if (threadIdx.x == 0) {
+            __threadfence();   // (for all of the CTA's stores, which the barrier puts before it)
             last = atomicAdd(a.arrived + row, 1u) + 1 == a.parts;
             if (last) a.arrived[row] = 0u;
             b.count = 0;
@@ -315,6 +427,7 @@ __global__ void __launch_bounds__(THREADS, 4) logprob_rows_kernel(const __grid_c
             const float4 f = __ldcg(a.part_stats + (size_t)row * a.parts + threadIdx.x);
             r = RowStats{f.x, f.y, f.z};
         }
+        share_stats(r, scratch[1]);
         if constexpr (TOP) {
             // (best ones first, so that the groups' largest are the parts' first few)
             const uint32_t keys = a.parts * a.n_top;
@@ -333,14 +446,16 @@ __global__ void __launch_bounds__(THREADS, 4) logprob_rows_kernel(const __grid_c
                 add_to_list(b, key[j] != 0 && key[j] >= least, key[j]);
             }
             __syncthreads();
-            order_list(b, a.n_top, keys, [&](uint64_t i) { return __ldcg(from + i); });
+            order_list(b, a.n_top, keys, [&](uint32_t i) { return __ldcg(from + i); });
+        } else {
+            __syncthreads();
         }
-        r = merge_cta(r, scratch[1]);
+        r = all_stats(scratch[1]);
     }
     const float log_s = logf(r.s);
-    const uint32_t *ids = a.ids_dev ? a.ids_dev : a.ids;
-    for (uint32_t i = threadIdx.x; i < a.n_ids; i += THREADS)
-        a.logprob[(size_t)row * a.n_ids + i] = log_prob(load_as_f32(logits, DTYPE, ids[(size_t)row * a.n_ids + i]), r.m, log_s);
+    if (threadIdx.x < a.n_ids) a.logprob[(size_t)row * a.n_ids + threadIdx.x] = log_prob(given, r.m, log_s);
+    for (uint32_t i = threadIdx.x + THREADS; i < a.n_ids; i += THREADS)
+        a.logprob[(size_t)row * a.n_ids + i] = log_prob(load_as_f32(logits, DTYPE, ids[i]), r.m, log_s);
     if (threadIdx.x == 0 && a.entropy) a.entropy[row] = entropy(r);
     if constexpr (TOP) {
         if (threadIdx.x < a.n_top) {
@@ -404,9 +519,13 @@ int launch_logprob_rows(yx_ctx *ctx, const void *logits, int dtype, uint32_t row
     a.entropy = entropy;
     a.top_ids = top_ids;
     a.top_logprob = top_logprob;
-    // Rows that fill the chip by themselves are a CTA each; fewer are cut into parts of a tile or more.
-    const uint32_t tiles = (uint32_t)(((uint64_t)cols + TILE - 1) / TILE), want = 4 * (uint32_t)ctx->sm_count;
-    a.parts = rows >= want / 2 ? 1 : std::min({tiles, MAX_PARTS, (want + rows - 1) / rows, MAX_SHARED / rows});
+    // A CTA a row, unless there are few rows and long ones: a CTA takes 48 bytes a nanosecond, and parts meeting in a last
+    // CTA cost 3 us (one row of 50257 f32 with five tokens 8.5 us whole and 7.6 in 13 parts, of 150000 16.9 and 8.2; 100
+    // rows of 50257 9.5 whole, 11.7 in two parts, more in more).
+    const uint32_t tiles = (uint32_t)(((uint64_t)cols + TILE - 1) / TILE);
+    const uint32_t most = std::min({tiles, MAX_PARTS, (uint32_t)ctx->sm_count / rows, MAX_SHARED / rows});
+    const uint64_t bytes = (uint64_t)cols * (dtype == YX_F32 ? 4 : 2);
+    a.parts = most > 1 && bytes - bytes / most > 144 * 1024 ? most : 1;
     // (at the most any call needs, for recordings)
     const size_t stats = MAX_SHARED * sizeof(float4), best = (size_t)MAX_SHARED * YX_TOP_MAX * sizeof(uint64_t);
     char *before = ctx->lp_parts.dev;

@@ -43,12 +43,12 @@ static __device__ __noinline__ float4 activate4(float4 y, int act) {
 // largest f32: `clean` sees to that.  Distances below -150 weigh nothing in f32 (exp(-150) is far below the smallest
 // subnormal); cutting them there, which also takes in -inf - -inf, keeps 0 * inf out of t.
 constexpr float LEAST_DISTANCE = -150.0f;
-constexpr float LOG2_E = 1.4426950408889634f;
+constexpr float LOG2_E = 1.4426950408889634f, LARGEST = 3.402823466e38f;
 struct RowStats {
     float m, s, t;
 };
 __device__ __forceinline__ RowStats no_stats() { return RowStats{-INFINITY, 0.0f, 0.0f}; }
-__device__ __forceinline__ float clean(float l) { return fminf(fmaxf(l, -INFINITY), 3.402823466e38f); }
+__device__ __forceinline__ float clean(float l) { return fminf(fmaxf(l, -INFINITY), LARGEST); }
 // (fmaxf passes over an operand that is no number)
 __device__ __forceinline__ float distance(float l, float m) { return fmaxf(l - m, LEAST_DISTANCE); }
 __device__ __forceinline__ RowStats merge(RowStats a, RowStats b) {
