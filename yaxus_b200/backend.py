@@ -336,7 +336,7 @@ class CudaBackend:
         self._check_product(x, w)
         shape = (x.shape[0], w.shape[0])
         if out is None:
-            out = torch.empty(shape, dtype=out_dtype or (torch.float32 if residual is None else residual.dtype), device=self.device)
+            out = x.new_empty(shape, dtype=out_dtype or (torch.float32 if residual is None else residual.dtype))
         assert self._here(out) and out.shape == shape and out.dtype in _YX_DTYPE and out.is_contiguous()
         assert bias is None or (self._here(bias) and bias.dtype == torch.float32 and bias.shape == shape[1:] and bias.is_contiguous())
         assert residual is None or (self._here(residual) and residual.dtype == out.dtype and residual.shape == shape and residual.is_contiguous())
@@ -352,10 +352,10 @@ class CudaBackend:
         stride = logits.stride(0) if rows > 1 else cols
         idx = None if ids is None else _token_ids(ids)
         assert idx is None or (idx.ndim in (1, 2) and idx.shape[0] == rows), "one row of ids for each row of logits"
-        new = lambda *shape, dtype=torch.float32: torch.empty(shape, dtype=dtype, device=self.device)   # noqa: E731
         n_ids = 0 if idx is None else idx.size // max(rows, 1)
-        r = LogProbs(new(*idx.shape) if n_ids else None, new(rows) if entropy else None,
-                     new(rows, top, dtype=torch.int32) if top else None, new(rows, top) if top else None)
+        new, f32 = logits.new_empty, torch.float32   # (a quarter cheaper than torch.empty: four of them cost what the launch does)
+        r = LogProbs(new(idx.shape, dtype=f32) if n_ids else None, new(rows, dtype=f32) if entropy else None,
+                     new((rows, top), dtype=torch.int32) if top else None, new((rows, top), dtype=f32) if top else None)
         self._L.yx_logprob_rows(self._ctx, _ptr(logits), _YX_DTYPE[logits.dtype], rows, cols, stride, _u32p(idx) if n_ids else None, n_ids,
                                 top, _ptr(r.logprob), _ptr(r.entropy), _ptr(r.top_ids), _ptr(r.top_logprob))
         return r
@@ -365,8 +365,7 @@ class CudaBackend:
         self._check_product(x, w)
         idx = _token_ids(ids)
         assert idx.shape == (x.shape[0],), "one id for each row"
-        r = LogProbs(torch.empty(x.shape[0], dtype=torch.float32, device=self.device),
-                     torch.empty(x.shape[0], dtype=torch.float32, device=self.device) if entropy else None)
+        r = LogProbs(x.new_empty(x.shape[0], dtype=torch.float32), x.new_empty(x.shape[0], dtype=torch.float32) if entropy else None)
         self._L.yx_matmul_logprobs(self._ctx, _ptr(x), _YX_DTYPE[x.dtype], _ptr(w), x.shape[0], w.shape[0], w.shape[1], _u32p(idx),
                                    _ptr(r.logprob), _ptr(r.entropy))
         return r

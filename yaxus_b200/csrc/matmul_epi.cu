@@ -98,7 +98,8 @@ int yx_matmul_epilogue(yx_ctx *ctx, const void *x_dev, int x_dtype, const void *
     Guard guard(ctx->device);
     Product p = product(x_dev, x_dtype, w_bf16_dev, rows, n, k);
     p.out = out_dev;
-    p.e = Epilogue{bias_dev, residual_dev, activation, out_dtype};
+    const size_t quad = 4 * size_of(out_dtype);
+    p.e = Epilogue{bias_dev, residual_dev, activation, out_dtype, n % 4 == 0 && aligned(bias_dev, 16) && aligned(residual_dev, quad) && aligned(out_dev, quad)};
     const bool tensor = exact_tc_takes(p);
     // Other CTAs still read the rows when a result is written: a result over its own rows takes them from a copy.
     if ((!tensor || exact_tc_reads_rows_late(p)) && overlap(out_dev, out_bytes, x_dev, x_bytes)) {

@@ -164,42 +164,92 @@ __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
 }
 
-// N results of this lane's column, pass rows from t0 on: bias, activation, residual.
+// ---- a warp's 32 columns by N pass rows change places -----------------------------------------------------
+//
+// A lane holds a column.  What follows a product wants a pass row's columns side by side: through shared memory, a pass row's
+// 128 bytes in 16-byte chunks at chunk ^ (row & 7), which meets no bank twice either way.
+template <int N, int V>
+__device__ __forceinline__ void stage(const float (&v)[V], int first, float *staged, int lane) {
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < N; i++) staged[i * 32 + (((lane >> 2) ^ (i & 7)) << 2) + (lane & 3)] = v[first + i];
+    __syncwarp();
+}
+__device__ __forceinline__ uint32_t staged_at(uint32_t row, uint32_t column) { return row * 32 + (((column >> 2) ^ (row & 7)) << 2) + (column & 3); }
+
+// Bias, activation and residual of N staged pass rows, t0 and on, by the 32 columns from col0.  All residuals are asked for
+// before the first is used, and what follows is a loop, whose registers move up: unrolled over a thread's up to 128 results
+// the code does not fit the instruction cache, and out of line every sum still in a register goes through local memory
+// (2048 x [14336, 4096] bf16: 220 us plain, 386 onto a residual with a type looked up for each; out of line 296 and 392).
 template <int N>
-__device__ __forceinline__ void finish_rows(const Epilogue &e, void *out, uint32_t T, uint32_t cols, const float (&v)[N], uint32_t t0, uint32_t col) {
-    if (col >= cols) return;
-    const float bias = e.bias ? e.bias[col] : 0.0f;
-    constexpr int H = N < 16 ? N : 16;   // (residuals in flight)
+__device__ __forceinline__ void finish_staged(const Epilogue &e, void *out, uint32_t T, uint32_t cols, const float *staged, uint32_t t0, uint32_t col0, int lane) {
+    if (t0 >= T) return;
+    const uint32_t rows = min((uint32_t)N, T - t0);
+    constexpr int R = N / 4;
+    const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
+    float4 res[R];
+    auto ask = [&](auto load) {   // load(type, i): the residuals of turn i
+        if (!e.residual) {
 #pragma unroll
-    for (int h = 0; h < N; h += H) {
-        const size_t at = (size_t)(t0 + h) * cols + col;
-        float y[H], r[H];
-        if (e.residual) {
+            for (int i = 0; i < R; i++) res[i] = zero;
+        } else if (e.out_dtype == YX_F32) {
 #pragma unroll
-            for (int i = 0; i < H; i++) r[i] = t0 + h + i < T ? load_as_f32(e.residual, e.out_dtype, at + (size_t)i * cols) : 0.0f;
+            for (int i = 0; i < R; i++) res[i] = load(YX_F32, i);
+        } else if (e.out_dtype == YX_F16) {
+#pragma unroll
+            for (int i = 0; i < R; i++) res[i] = load(YX_F16, i);
+        } else {
+#pragma unroll
+            for (int i = 0; i < R; i++) res[i] = load(YX_BF16, i);
         }
+    };
+    auto next = [&](float4 y) {
+        y = activate4(y, e.act);
+        if (e.residual) y = make_float4(y.x + res[0].x, y.y + res[0].y, y.z + res[0].z, y.w + res[0].w);
 #pragma unroll
-        for (int i = 0; i < H; i++) y[i] = v[h + i] + bias;
-        if (e.act != YX_ACT_NONE) {
-#pragma unroll
-            for (int i = 0; i < H; i += 4) *(float4 *)(y + i) = activate4(make_float4(y[i], y[i + 1], y[i + 2], y[i + 3]), e.act);
+        for (int i = 0; i + 1 < R; i++) res[i] = res[i + 1];
+        return y;
+    };
+    if (e.quads) {
+        // A turn: four columns a lane, four pass rows a warp.
+        const uint32_t q = 4 * (lane & 7), col = col0 + q, r0 = lane >> 3;
+        if (col >= cols) return;
+        size_t at = (size_t)(t0 + r0) * cols + col;
+        const float4 bias = e.bias ? *(const float4 *)(e.bias + col) : zero;
+        ask([&](int dtype, int i) { return r0 + 4 * i < rows ? load4_as_f32(e.residual, dtype, at + (size_t)(4 * i) * cols) : zero; });
+#pragma unroll 1
+        for (uint32_t r = r0; r < rows; r += 4, at += (size_t)4 * cols) {
+            const float4 y = *(const float4 *)(staged + staged_at(r, q));
+            store4(out, e.out_dtype, at, next(make_float4(y.x + bias.x, y.y + bias.y, y.z + bias.z, y.w + bias.w)));
         }
-        if (e.residual) {
+    } else {
+        // A turn: a column a lane, four pass rows.
+        const uint32_t col = col0 + lane;
+        if (col >= cols) return;
+        size_t at = (size_t)t0 * cols + col;
+        const float bias = e.bias ? e.bias[col] : 0.0f;
+        ask([&](int dtype, int i) {
+            float v[4];
 #pragma unroll
-            for (int i = 0; i < H; i++) y[i] += r[i];
+            for (int k = 0; k < 4; k++) v[k] = 4 * i + k < (int)rows ? load_as_f32(e.residual, dtype, at + (size_t)(4 * i + k) * cols) : 0.0f;
+            return make_float4(v[0], v[1], v[2], v[3]);
+        });
+#pragma unroll 1
+        for (uint32_t r = 0; r < rows; r += 4) {
+            const float4 y = next(make_float4(staged[staged_at(r, lane)] + bias, staged[staged_at(r + 1, lane)] + bias, staged[staged_at(r + 2, lane)] + bias,
+                                              staged[staged_at(r + 3, lane)] + bias));
+            const float z[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+            for (int k = 0; k < 4; k++, at += cols)
+                if (r + k < rows) store_from_f32(out, e.out_dtype, at, z[k]);
         }
-#pragma unroll
-        for (int i = 0; i < H; i++)
-            if (t0 + h + i < T) store_from_f32(out, e.out_dtype, at + (size_t)i * cols, y[i]);
     }
 }
 
 // ---- softmax statistics of a warp's 32 columns for each of its pass rows --------------------------------
 //
-// A lane holds a column; the sums run over columns.  Sixteen pass rows at a time change places with the columns
-// through 2 KiB of shared memory (16-byte chunks of a pass row's 128 bytes at chunk ^ (row & 7): no bank is met twice
-// either way), after which a lane has half a pass row's columns: 2.5 shared-memory accesses for a logit's eight or so
-// instructions, where summing across lanes would take three shuffles for each.
+// Sixteen pass rows at a time change places with the columns, after which a lane has half a pass row's: 1.25
+// shared-memory accesses for a logit's eight or so instructions, where summing across lanes would take three shuffles.
 constexpr int STATS_SCRATCH = 16 * 32;   // floats a warp
 
 // Statistics of pass rows 0..15 of v over this warp's 32 columns, in lanes r and r + 16 for row r.  `want`: the row's given
@@ -208,13 +258,13 @@ template <int N>
 __device__ __forceinline__ RowStats stats_of_16(const float (&v)[N], int first, bool column, float *scratch, int lane, uint32_t want, float &logit) {
     __syncwarp();
 #pragma unroll
-    for (int i = 0; i < (N < 16 ? N : 16); i++) scratch[i * 32 + (((lane >> 2) ^ (i & 7)) << 2) + (lane & 3)] = column ? v[first + i] : -INFINITY;
+    for (int i = 0; i < (N < 16 ? N : 16); i++) scratch[staged_at(i, lane)] = column ? v[first + i] : -INFINITY;
     __syncwarp();
     const int r = lane & 15;
     float q[16];
 #pragma unroll
-    for (int c = 0; c < 4; c++) *(float4 *)(q + 4 * c) = *(const float4 *)(scratch + r * 32 + ((((lane >> 4) * 4 + c) ^ (r & 7)) << 2));
-    if (want < 32u) logit = scratch[r * 32 + (((want >> 2) ^ (r & 7)) << 2) + (want & 3)];
+    for (int c = 0; c < 4; c++) *(float4 *)(q + 4 * c) = *(const float4 *)(scratch + staged_at(r, ((lane >> 4) * 4 + c) * 4));
+    if (want < 32u) logit = scratch[staged_at(r, want)];
     RowStats st{q[0], 0.0f, 0.0f};
 #pragma unroll
     for (int i = 1; i < 16; i++) st.m = fmaxf(st.m, q[i]);
@@ -300,7 +350,9 @@ matmul_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_const
     __shared__ uint32_t tmem_base_s;
     __shared__ int abort_flag;
     __shared__ int last_s;
-    __shared__ __align__(16) float stats_scratch[KIND == LOGPROBS ? 8 * STATS_SCRATCH : 4];
+    constexpr int SCRATCH = KIND == EPILOGUE ? 32 * 32 : KIND == LOGPROBS ? STATS_SCRATCH : 1;   // floats a warp
+    __shared__ __align__(16) float scratch_s[8 * SCRATCH];
+    float *scratch = scratch_s + ((threadIdx.x >> 5) & 7) * SCRATCH;
     __shared__ float4 stats_results[KIND == LOGPROBS ? 2 : 1][2][4][KIND == LOGPROBS ? 32 : 1];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = blockIdx.x & 1u, pair = blockIdx.x >> 1;
@@ -422,10 +474,12 @@ matmul_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_const
         uint32_t stats_turn = 0;
         auto finish = [&](const float (&v)[32], uint32_t t, uint32_t row) {
             if constexpr (KIND < EPILOGUE) store_rows<KIND == GLU>(a, v, t, row, lane);
-            else if constexpr (KIND == EPILOGUE) finish_rows(a.e, a.out, a.T, a.cols, v, t, row);
-            else
-                stats_rows(a.so, a.T, a.cols, v, t, row, row >> 7, a.ids, stats_scratch + warp * STATS_SCRATCH, stats_results[warp >> 2], stats_turn, 2 + (warp >> 2),
-                           warp, lane);
+            else if constexpr (KIND == EPILOGUE) {
+                stage<32>(v, 0, scratch, lane);
+                finish_staged<32>(a.e, a.out, a.T, a.cols, scratch, t, row - lane, lane);
+            } else {
+                stats_rows(a.so, a.T, a.cols, v, t, row, row >> 7, a.ids, scratch, stats_results[warp >> 2], stats_turn, 2 + (warp >> 2), warp, lane);
+            }
         };
         while (walk.next(a, pair, p)) {
             const uint32_t wr = (warp & 3) * 32 + lane;   // weight row of this CTA's 128
@@ -470,12 +524,27 @@ matmul_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_const
             }
             // A share's sums: four pass rows of each of 128 weight rows, then the next four.
             auto share = [&](uint32_t q) { return (float4 *)(a.part + ((size_t)(2 * q + (q == q0 ? second : 0u)) * 2 + rank) * a.bt * 128u) + wr; };
+            // What follows the sums is written once and gone through chunk by chunk, the next chunk's sums moving up.
+            auto finish_all = [&] {
+#pragma unroll 1
+                for (uint32_t c = c0; c < a.bt; c += 64) {
+                    finish(sum[0], t0 + c, row);
+#pragma unroll
+                    for (int j = 0; j + 1 < CHUNKS; j++)
+#pragma unroll
+                        for (int i = 0; i < 32; i++) sum[j][i] = sum[j + 1][i];
+                }
+            };
+            if (KIND >= EPILOGUE && p.whole) {
+                finish_all();
+                continue;
+            }
 #pragma unroll
             for (int j = 0; j < CHUNKS; j++) {
                 const uint32_t c = c0 + 64 * j;
                 if (c >= a.bt) break;
                 if (p.whole) {
-                    finish(sum[j], t0 + c, row);
+                    if constexpr (KIND < EPILOGUE) finish(sum[j], t0 + c, row);
                 } else {
                     float4 *mine = share(pair) + c / 4 * 128u;
 #pragma unroll
@@ -705,7 +774,9 @@ matmul_rows_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_const
     constexpr bool GLU_TILES = KIND == GLU;
     constexpr uint32_t NB = rows_columns(TP, PARTS), PITCH = rows_pitch(TP, PARTS), X_BYTES = NB * 128, STAGE = W_BYTES + X_BYTES;
     constexpr uint32_t TMEM = ROWS_BUFS * PITCH;
-    __shared__ __align__(16) float stats_scratch[KIND == LOGPROBS ? 4 * STATS_SCRATCH : 4];
+    constexpr int SCRATCH = KIND == EPILOGUE ? TP * 32 : KIND == LOGPROBS ? STATS_SCRATCH : 1;   // floats a warp
+    __shared__ __align__(16) float scratch_s[4 * SCRATCH];
+    float *scratch = scratch_s + ((threadIdx.x >> 5) & 3) * SCRATCH;
     __shared__ float4 stats_results[2][4][KIND == LOGPROBS ? 32 : 1];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t S = a.stages, base = smem_u32(smem);
@@ -869,8 +940,12 @@ matmul_rows_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_const
         uint32_t n = 0, stats_turn = 0;
         auto finish = [&](const float (&v)[TP], uint32_t row) {
             if constexpr (KIND < EPILOGUE) store_few<TP, KIND == GLU>(a, v, row, lane);
-            else if constexpr (KIND == EPILOGUE) finish_rows(a.e, a.out, a.T, a.cols, v, 0, row);
-            else stats_rows(a.so, a.T, a.cols, v, 0, row, row >> 7, a.ids, stats_scratch + warp * STATS_SCRATCH, stats_results, stats_turn, 2, warp, lane);
+            else if constexpr (KIND == EPILOGUE) {
+                stage<TP>(v, 0, scratch, lane);
+                finish_staged<TP>(a.e, a.out, a.T, a.cols, scratch, 0, row - lane, lane);
+            } else {
+                stats_rows(a.so, a.T, a.cols, v, 0, row, row >> 7, a.ids, scratch, stats_results, stats_turn, 2, warp, lane);
+            }
         };
         for (uint32_t u = u0; u < u1;) {
             const uint32_t tile = u / a.ksteps, end = min(u1, (tile + 1) * a.ksteps);
@@ -1024,7 +1099,8 @@ int ensure_counters(yx_ctx *ctx, size_t n) {
     return check_cuda(ctx, cudaMemsetAsync(ctx->mm_counters, 0, ctx->mm_counters_cap, ctx->stream), "matmul: counters");
 }
 
-constexpr uint32_t smem_budget(int kind) { return kind == LOGPROBS ? 200 * 1024 : TC_SMEM_BUDGET; }   // (24 KiB change places there)
+// (what changes places takes 32 KiB of an EPILOGUE's CTA, 24 KiB with the statistics)
+constexpr uint32_t smem_budget(int kind) { return kind == EPILOGUE ? 194 * 1024 : kind == LOGPROBS ? 200 * 1024 : TC_SMEM_BUDGET; }
 
 // CTA pairs that are on the chip together (a GPC with an odd number of SMs leaves one out).
 template <int KIND, int CHUNKS>
@@ -1195,7 +1271,7 @@ int exact_pair_rows(yx_ctx *ctx, const Product &p) {
 template <int TP, int KIND, int PARTS>
 int matmul_few_rows(yx_ctx *ctx, const Product &p) {
     constexpr uint32_t stage_bytes = W_BYTES + rows_columns(TP, PARTS) * 128;
-    constexpr uint32_t stages = std::min<uint32_t>(TC_MAX_STAGES, (KIND == LOGPROBS ? 210 * 1024 : TC_SMEM_BUDGET) / stage_bytes);
+    constexpr uint32_t stages = std::min<uint32_t>(TC_MAX_STAGES, (KIND < EPILOGUE ? TC_SMEM_BUDGET : 210 * 1024) / stage_bytes);
     auto *kernel = matmul_rows_kernel<TP, KIND, PARTS>;
     bool &configured = ctx->mm_rows_configured[KIND][PARTS - 1][TP / 16];
     if (!configured) {

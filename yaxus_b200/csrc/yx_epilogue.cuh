@@ -21,21 +21,31 @@ __device__ __forceinline__ void store_from_f32(void *p, int dtype, size_t i, flo
     else ((__nv_bfloat16 *)p)[i] = __float2bfloat16_rn(v);
 }
 
+// y times the logistic function of u.  The hardware's 2^x and 1 / x (two units and one in the last place): where their
+// error counts, y's own is as large.
+__device__ __forceinline__ float logistic(float y, float u) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + fast_exp2(-1.4426950408889634f * u)));
+    return y * r;
+}
 __device__ __forceinline__ float activate(float y, int act) {
     switch (act) {
     case YX_ACT_RELU: return y < 0.0f ? 0.0f : y;
     case YX_ACT_GELU: return 0.5f * y * (1.0f + erff(y * 0.70710678118654752f));
-    // 0.5 (1 + tanh u) = 1 / (1 + exp(-2 u)): one exponential, and no cancellation where tanh is near -1.
-    case YX_ACT_GELU_TANH: return y / (1.0f + expf(-1.5957691216057308f * (y + 0.044715f * y * y * y)));
-    case YX_ACT_SILU: return y / (1.0f + expf(-y));
+    // 0.5 (1 + tanh u) is the logistic function of 2 u: no cancellation where tanh is near -1.
+    case YX_ACT_GELU_TANH: return logistic(y, 1.5957691216057308f * (y + 0.044715f * y * y * y));
+    case YX_ACT_SILU: return logistic(y, y);
     default: return y;
     }
 }
-
-// (out of line: a tile's epilogue is unrolled over up to 128 results, and five activations in each would not fit the
-// instruction cache; four at a time, the call costs less than the exponentials)
-static __device__ __noinline__ float4 activate4(float4 y, int act) {
-    return make_float4(activate(y.x, act), activate(y.y, act), activate(y.z, act), activate(y.w, act));
+__device__ __forceinline__ float4 activate4(float4 y, int act) {   // (the choice once for four, whose exponentials then overlap)
+#define YX_FOUR(A) make_float4(activate(y.x, A), activate(y.y, A), activate(y.z, A), activate(y.w, A))
+    if (act == YX_ACT_NONE) return y;
+    if (act == YX_ACT_SILU) return YX_FOUR(YX_ACT_SILU);
+    if (act == YX_ACT_GELU_TANH) return YX_FOUR(YX_ACT_GELU_TANH);
+    if (act == YX_ACT_GELU) return YX_FOUR(YX_ACT_GELU);
+    return YX_FOUR(YX_ACT_RELU);
+#undef YX_FOUR
 }
 
 // A softmax's statistics over some of a row's logits l: the largest m, s = sum exp(l - m), t = sum exp(l - m) (l - m).

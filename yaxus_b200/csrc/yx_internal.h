@@ -397,6 +397,7 @@ struct Epilogue {
     const void *residual;    // [rows, cols] of the output's type or null; may be the output itself
     int act;                 // yx_activation
     int out_dtype;           // yx_dtype
+    bool quads;              // four columns at a time: their number is a multiple of four, and so are the tensors' addresses
 };
 // out = x . w^T on the tensor cores for many rows (matmul_tc.cu says what it takes).
 int launch_matmul_tc(yx_ctx *ctx, const float *x, const void *w, uint32_t T, uint32_t N, uint32_t K, bool glu, float *out);
