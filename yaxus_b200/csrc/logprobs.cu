@@ -191,32 +191,6 @@ __device__ __forceinline__ void share_stats(RowStats r, RowStats *scratch) {
 }
 __device__ __forceinline__ RowStats all_stats(const RowStats *scratch) { return warp_sum<WARPS>(scratch[threadIdx.x & (WARPS - 1)]); }
 
-// Two f32 at a time (add.f32x2 and the like: half the issue slots).
-struct F2 {
-    uint64_t bits;
-};
-__device__ __forceinline__ F2 f2(float a, float b) {
-    F2 r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r.bits) : "f"(a), "f"(b));
-    return r;
-}
-__device__ __forceinline__ void split(F2 v, float &a, float &b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v.bits)); }
-__device__ __forceinline__ F2 operator+(F2 a, F2 b) {
-    F2 r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.bits) : "l"(a.bits), "l"(b.bits));
-    return r;
-}
-__device__ __forceinline__ F2 operator*(F2 a, F2 b) {
-    F2 r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.bits) : "l"(a.bits), "l"(b.bits));
-    return r;
-}
-__device__ __forceinline__ F2 fma(F2 a, F2 b, F2 c) {
-    F2 r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.bits) : "l"(a.bits), "l"(b.bits), "l"(c.bits));
-    return r;
-}
-
 template <int DTYPE, int N = PER_THREAD>
 struct Tile {
     static constexpr int WIDE = DTYPE == YX_F32 ? 4 : 8;   // logits in 16 bytes
@@ -332,17 +306,7 @@ __global__ void __launch_bounds__(THREADS, 4) logprob_rows_kernel(const __grid_c
             s2 = f2(c, c) * s2;
             r.m = most;
         }
-        const F2 minus_m = f2(-r.m, -r.m), log2_e = f2(LOG2_E, LOG2_E);
-#pragma unroll
-        for (int j = 0; j < PER_THREAD; j += 2) {
-            float d0, d1, y0, y1;
-            split(f2(x[j], x[j + 1]) + minus_m, d0, d1);
-            const F2 d = f2(fmaxf(d0, LEAST_DISTANCE), fmaxf(d1, LEAST_DISTANCE));   // (see distance())
-            split(d * log2_e, y0, y1);
-            const F2 e = f2(fast_exp2(y0), fast_exp2(y1));
-            s2 = s2 + e;
-            t2 = fma(e, d, t2);
-        }
+        add_up(x, r.m, s2, t2);
     }
     {
         float x, y;

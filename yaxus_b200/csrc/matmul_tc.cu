@@ -249,7 +249,7 @@ __device__ __forceinline__ void finish_staged(const Epilogue &e, void *out, uint
 // ---- softmax statistics of a warp's 32 columns for each of its pass rows --------------------------------
 //
 // Sixteen pass rows at a time change places with the columns, after which a lane has half a pass row's: 1.25
-// shared-memory accesses for a logit's eight or so instructions, where summing across lanes would take three shuffles.
+// shared-memory accesses for a logit's six or so instructions, where summing across lanes would take three shuffles.
 constexpr int STATS_SCRATCH = 16 * 32;   // floats a warp
 
 // Statistics of pass rows 0..15 of v over this warp's 32 columns, in lanes r and r + 16 for row r.  `want`: the row's given
@@ -265,29 +265,29 @@ __device__ __forceinline__ RowStats stats_of_16(const float (&v)[N], int first, 
 #pragma unroll
     for (int c = 0; c < 4; c++) *(float4 *)(q + 4 * c) = *(const float4 *)(scratch + staged_at(r, ((lane >> 4) * 4 + c) * 4));
     if (want < 32u) logit = scratch[staged_at(r, want)];
-    RowStats st{q[0], 0.0f, 0.0f};
+    float m = q[0];
 #pragma unroll
-    for (int i = 1; i < 16; i++) st.m = fmaxf(st.m, q[i]);
-    if (!(st.m < INFINITY)) {   // an infinity (or nothing but no numbers)
+    for (int i = 1; i < 16; i++) m = fmaxf(m, q[i]);
+    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+    if (!(m < INFINITY)) {   // an infinity (or nothing but no numbers)
 #pragma unroll
         for (int i = 0; i < 16; i++) q[i] = clean(q[i]);
-        st.m = clean(st.m);
+        m = clean(m);
     }
-#pragma unroll
-    for (int i = 0; i < 16; i++) {
-        const float d = distance(q[i], st.m), e = fast_exp2(d * LOG2_E);
-        st.s += e;
-        st.t += e * d;
-    }
-    return merge(st, RowStats{__shfl_xor_sync(0xffffffffu, st.m, 16), __shfl_xor_sync(0xffffffffu, st.s, 16), __shfl_xor_sync(0xffffffffu, st.t, 16)});
+    F2 s2 = f2(0.0f, 0.0f), t2 = s2;
+    add_up(q, m, s2, t2);
+    float s, t, s1, t1;
+    split(s2, s, s1);
+    split(t2, t, t1);
+    s += s1;
+    t += t1;
+    return RowStats{m, s + __shfl_xor_sync(0xffffffffu, s, 16), t + __shfl_xor_sync(0xffffffffu, t, 16)};
 }
 
-// Up to 32 pass rows from t0 on: each warp's 32 columns, then the four warps of a barrier together.  `turn` counts the
-// group's calls: the warps' results go to two buffers in turn, so that one barrier a call is enough.  Warp `turn` mod
-// four merges and writes.
+// Of N pass rows from t0 on: this warp's 32 columns, lane i row t0 + i, and the given tokens' logits where they are among them.
 template <int N>
-__device__ __forceinline__ void stats_rows(const StatsOut &so, uint32_t T, uint32_t cols, const float (&v)[N], uint32_t t0, uint32_t row, uint32_t block,
-                                           const uint32_t *ids, float *scratch, float4 (*results)[4][32], uint32_t &turn, int barrier, int warp, int lane) {
+__device__ __forceinline__ float4 stats_of(const StatsOut &so, uint32_t T, uint32_t cols, const float (&v)[N], uint32_t t0, uint32_t row, const uint32_t *ids,
+                                           float *scratch, int lane) {
     const uint32_t t = t0 + lane;
     const uint32_t want = lane < N && t < T ? ids[t] - (row - lane) : 0xffffffffu;
     float logit = 0.0f;
@@ -297,18 +297,19 @@ __device__ __forceinline__ void stats_rows(const StatsOut &so, uint32_t T, uint3
         if (lane >= 16) st = hi;
     }
     if (want < 32u) so.picked[t] = logit;
-    results[turn & 1][warp & 3][lane] = make_float4(st.m, st.s, st.t, 0.0f);
-    asm volatile("bar.sync %0, 128;" ::"r"(barrier) : "memory");
-    if ((turn & 3) == (uint32_t)(warp & 3) && lane < N && t < T) {
-        RowStats all = no_stats();
+    return make_float4(st.m, st.s, st.t, 0.0f);
+}
+// Four warps' statistics of the same pass rows as one.
+__device__ __forceinline__ float4 merge_four(const float4 (&f)[4]) {
+    const float m = fmaxf(fmaxf(f[0].x, f[1].x), fmaxf(f[2].x, f[3].x));
+    float s = 0.0f, t = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const float4 f = results[turn & 1][i][lane];
-            all = merge(all, RowStats{f.x, f.y, f.z});
-        }
-        so.stats[(size_t)t * so.blocks + block] = make_float4(all.m, all.s, all.t, 0.0f);
+    for (int i = 0; i < 4; i++) {
+        const float d = distance(f[i].x, m), c = fast_exp2(d * LOG2_E);
+        s += c * f[i].y;
+        t += c * (f[i].z + d * f[i].y);
     }
-    turn++;
+    return make_float4(m, s, t, 0.0f);
 }
 
 // 32 pass rows from `t0` on of this lane's weight row.
@@ -353,7 +354,7 @@ matmul_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_const
     constexpr int SCRATCH = KIND == EPILOGUE ? 32 * 32 : KIND == LOGPROBS ? STATS_SCRATCH : 1;   // floats a warp
     __shared__ __align__(16) float scratch_s[8 * SCRATCH];
     float *scratch = scratch_s + ((threadIdx.x >> 5) & 7) * SCRATCH;
-    __shared__ float4 stats_results[KIND == LOGPROBS ? 2 : 1][2][4][KIND == LOGPROBS ? 32 : 1];
+    __shared__ float4 stats_s[KIND == LOGPROBS ? CHUNKS : 1][8][KIND == LOGPROBS ? 32 : 1];   // of a tile, by chunks and warps
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = blockIdx.x & 1u, pair = blockIdx.x >> 1;
     const uint32_t parts = KIND < EPILOGUE ? 2u : a.parts;
@@ -471,15 +472,25 @@ matmul_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_const
         Walk walk(a, pair);
         Piece p;
         AccTurn turn;
-        uint32_t stats_turn = 0;
-        auto finish = [&](const float (&v)[32], uint32_t t, uint32_t row) {
+        auto finish = [&](const float (&v)[32], uint32_t t, uint32_t row, uint32_t chunk) {
             if constexpr (KIND < EPILOGUE) store_rows<KIND == GLU>(a, v, t, row, lane);
             else if constexpr (KIND == EPILOGUE) {
                 stage<32>(v, 0, scratch, lane);
                 finish_staged<32>(a.e, a.out, a.T, a.cols, scratch, t, row - lane, lane);
             } else {
-                stats_rows(a.so, a.T, a.cols, v, t, row, row >> 7, a.ids, scratch, stats_results[warp >> 2], stats_turn, 2 + (warp >> 2), warp, lane);
+                stats_s[chunk][warp][lane] = stats_of(a.so, a.T, a.cols, v, t, row, a.ids, scratch, lane);
             }
+        };
+        // A tile's statistics: the four warps of the same pass rows each take a chunk of them.
+        auto finish_stats = [&](uint32_t t0, uint32_t c0, uint32_t row) {
+            asm volatile("bar.sync %0, 128;" ::"r"(2 + (warp >> 2)) : "memory");
+            const uint32_t chunk = warp & 3, t = t0 + c0 + 64 * chunk + lane;
+            if (chunk < CHUNKS && c0 + 64 * chunk < a.bt && t < a.T) {
+                const int g = warp & 4;
+                const float4 four[4] = {stats_s[chunk][g][lane], stats_s[chunk][g + 1][lane], stats_s[chunk][g + 2][lane], stats_s[chunk][g + 3][lane]};
+                a.so.stats[(size_t)t * a.so.blocks + (row >> 7)] = merge_four(four);
+            }
+            asm volatile("bar.sync %0, 128;" ::"r"(2 + (warp >> 2)) : "memory");
         };
         while (walk.next(a, pair, p)) {
             const uint32_t wr = (warp & 3) * 32 + lane;   // weight row of this CTA's 128
@@ -527,8 +538,8 @@ matmul_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_const
             // What follows the sums is written once and gone through chunk by chunk, the next chunk's sums moving up.
             auto finish_all = [&] {
 #pragma unroll 1
-                for (uint32_t c = c0; c < a.bt; c += 64) {
-                    finish(sum[0], t0 + c, row);
+                for (uint32_t c = c0, chunk = 0; c < a.bt; c += 64, chunk++) {
+                    finish(sum[0], t0 + c, row, chunk);
 #pragma unroll
                     for (int j = 0; j + 1 < CHUNKS; j++)
 #pragma unroll
@@ -537,6 +548,7 @@ matmul_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_const
             };
             if (KIND >= EPILOGUE && p.whole) {
                 finish_all();
+                if constexpr (KIND == LOGPROBS) finish_stats(t0, c0, row);
                 continue;
             }
 #pragma unroll
@@ -544,7 +556,7 @@ matmul_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_const
                 const uint32_t c = c0 + 64 * j;
                 if (c >= a.bt) break;
                 if (p.whole) {
-                    if constexpr (KIND < EPILOGUE) finish(sum[j], t0 + c, row);
+                    if constexpr (KIND < EPILOGUE) finish(sum[j], t0 + c, row, 0);
                 } else {
                     float4 *mine = share(pair) + c / 4 * 128u;
 #pragma unroll
@@ -592,8 +604,9 @@ matmul_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_const
 #pragma unroll
                     for (int i = 0; i < 4; i++) *(float4 *)(v + 16 * h + 4 * i) = sum[i];
                 }
-                finish(v, t0 + c, row);
+                finish(v, t0 + c, row, c / 64);
             }
+            if constexpr (KIND == LOGPROBS) finish_stats(t0, 32u * (warp >> 2), row);
         }
     }
     __syncwarp();
@@ -777,7 +790,7 @@ matmul_rows_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_const
     constexpr int SCRATCH = KIND == EPILOGUE ? TP * 32 : KIND == LOGPROBS ? STATS_SCRATCH : 1;   // floats a warp
     __shared__ __align__(16) float scratch_s[4 * SCRATCH];
     float *scratch = scratch_s + ((threadIdx.x >> 5) & 3) * SCRATCH;
-    __shared__ float4 stats_results[2][4][KIND == LOGPROBS ? 32 : 1];
+    __shared__ float4 stats_s[4][KIND == LOGPROBS ? 32 : 1];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t S = a.stages, base = smem_u32(smem);
     const uint32_t b_full = smem_u32(bar_store), b_empty = b_full + 8 * TC_MAX_STAGES;
@@ -937,14 +950,20 @@ matmul_rows_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_const
         }
     } else {
         // ---- epilogue -------------------------------------------------------------------------
-        uint32_t n = 0, stats_turn = 0;
+        uint32_t n = 0;
         auto finish = [&](const float (&v)[TP], uint32_t row) {
             if constexpr (KIND < EPILOGUE) store_few<TP, KIND == GLU>(a, v, row, lane);
             else if constexpr (KIND == EPILOGUE) {
                 stage<TP>(v, 0, scratch, lane);
                 finish_staged<TP>(a.e, a.out, a.T, a.cols, scratch, 0, row - lane, lane);
             } else {
-                stats_rows(a.so, a.T, a.cols, v, 0, row, row >> 7, a.ids, scratch, stats_results, stats_turn, 2, warp, lane);
+                stats_s[warp][lane] = stats_of(a.so, a.T, a.cols, v, 0, row, a.ids, scratch, lane);
+                asm volatile("bar.sync 2, 128;" ::: "memory");
+                if (warp == 0 && lane < (int)a.T) {
+                    const float4 four[4] = {stats_s[0][lane], stats_s[1][lane], stats_s[2][lane], stats_s[3][lane]};
+                    a.so.stats[(size_t)lane * a.so.blocks + (row >> 7)] = merge_four(four);
+                }
+                asm volatile("bar.sync 2, 128;" ::: "memory");
             }
         };
         for (uint32_t u = u0; u < u1;) {
@@ -1099,8 +1118,8 @@ int ensure_counters(yx_ctx *ctx, size_t n) {
     return check_cuda(ctx, cudaMemsetAsync(ctx->mm_counters, 0, ctx->mm_counters_cap, ctx->stream), "matmul: counters");
 }
 
-// (what changes places takes 32 KiB of an EPILOGUE's CTA, 24 KiB with the statistics)
-constexpr uint32_t smem_budget(int kind) { return kind == EPILOGUE ? 194 * 1024 : kind == LOGPROBS ? 200 * 1024 : TC_SMEM_BUDGET; }
+// (what changes places takes 32 KiB, in LOGPROBS half of that with the statistics in the other)
+constexpr uint32_t smem_budget(int kind) { return kind < EPILOGUE ? TC_SMEM_BUDGET : 194 * 1024; }
 
 // CTA pairs that are on the chip together (a GPC with an odd number of SMs leaves one out).
 template <int KIND, int CHUNKS>

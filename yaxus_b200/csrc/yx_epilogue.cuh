@@ -70,6 +70,48 @@ __device__ __forceinline__ RowStats merge(RowStats a, RowStats b) {
     r.t = ca * (a.t + da * a.s) + cb * (b.t + db * b.s);
     return r;
 }
+// Two f32 at a time (add.f32x2 and the like: half the issue slots).
+struct F2 {
+    uint64_t bits;
+};
+__device__ __forceinline__ F2 f2(float a, float b) {
+    F2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r.bits) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void split(F2 v, float &a, float &b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v.bits)); }
+__device__ __forceinline__ F2 operator+(F2 a, F2 b) {
+    F2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.bits) : "l"(a.bits), "l"(b.bits));
+    return r;
+}
+__device__ __forceinline__ F2 operator*(F2 a, F2 b) {
+    F2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.bits) : "l"(a.bits), "l"(b.bits));
+    return r;
+}
+__device__ __forceinline__ F2 fma(F2 a, F2 b, F2 c) {
+    F2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.bits) : "l"(a.bits), "l"(b.bits), "l"(c.bits));
+    return r;
+}
+
+// Adds exp(x - m) to s and exp(x - m) (x - m) to t, for N values.
+template <int N>
+__device__ __forceinline__ void add_up(const float (&x)[N], float m, F2 &s, F2 &t) {
+    const F2 minus_m = f2(-m, -m), log2_e = f2(LOG2_E, LOG2_E);
+#pragma unroll
+    for (int j = 0; j < N; j += 2) {
+        float d0, d1, y0, y1;
+        split(f2(x[j], x[j + 1]) + minus_m, d0, d1);
+        const F2 d = f2(fmaxf(d0, LEAST_DISTANCE), fmaxf(d1, LEAST_DISTANCE));   // (see distance())
+        split(d * log2_e, y0, y1);
+        const F2 e = f2(fast_exp2(y0), fast_exp2(y1));
+        s = s + e;
+        t = fma(e, d, t);
+    }
+}
+
 // The log probability of a logit under the row's statistics; -inf in a row with nothing left.
 __device__ __forceinline__ float log_prob(float l, float m, float log_s) { return m == -INFINITY ? -INFINITY : clean(l) - m - log_s; }
 __device__ __forceinline__ float entropy(RowStats r) { return r.m == -INFINITY ? 0.0f : logf(r.s) - r.t / r.s; }
