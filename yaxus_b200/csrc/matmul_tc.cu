@@ -60,7 +60,10 @@ constexpr uint32_t TC_SMEM_BUDGET = 220 * 1024;
 // 80 rows pays 19 us of 399 for chains of eight in place of 16.
 constexpr uint32_t TC_CHAIN = 16, TC_FIRST_CHAIN = 32, TC_SHORT_CHAIN = 8, TC_CUT_CHAIN = 6, TC_LEAST_CHAIN = 4;
 constexpr int TC_MAX_BUFS = 4;
-// The same for rows taken exactly (EPILOGUE, LOGPROBS), by their parts, and for results of 16 bits, which keep none of it.
+// The same for rows taken exactly (EPILOGUE, LOGPROBS), by their parts: what keeps the result within a millionth (2-norm of
+// the error over the result's, 2048 x [14336, 4096] and 80 x [4096, 4096]: one part in chains of 4, 8 and 12 steps 2.4, 4.7 and 7.1e-7,
+// two of 3 and 6 4.5 and 8.3e-7, three of 2, 3 and 4 7.1, 9.3 and 11.6e-7; yx_matmul 27e-7).  Results of 16 bits keep none of it.
+constexpr uint32_t MAX_CLUSTER = 4;         // pairs of a cluster (eight CTAs: the most that any chip of this kind places)
 constexpr uint32_t EXACT_CHAIN[3] = {12, 6, 3}, NARROW_CHAIN = 32;
 constexpr uint32_t GLU_GROUP = 16;          // gate and up rows alternate in a tile sixteen by sixteen: a warp holds both
 
@@ -82,6 +85,7 @@ struct StatsOut {
 struct PairArgs {
     uint32_t T, cols;                 // pass rows; columns of the result
     uint32_t parts;                   // bf16 parts of a pass row (EPILOGUE, LOGPROBS)
+    uint32_t cluster;                 // pairs that share a tile as one cluster (EPILOGUE, LOGPROBS; 1: none)
     bool early_w;                     // what wrote the weights is complete when this kernel starts
     uint32_t bt, t_tiles;             // pass rows of a tile (multiple of 32), tiles of them
     uint32_t ksteps;
@@ -112,11 +116,16 @@ __device__ __forceinline__ uint32_t rest_owner(const PairArgs &a, uint32_t u) {
     return (uint32_t)((((uint64_t)u + 1) * a.rest_pairs - 1) / a.rest_units);
 }
 
-// Walks a pair's pieces: its share of the left-over tiles (at most two pieces), then its whole tiles.
+// Walks a pair's pieces: its share of the left-over tiles (at most two pieces), then its whole tiles.  In a cluster of several
+// pairs there is one piece: the pair's share of the cluster's tile.
 struct Walk {
     uint32_t u, u_end, round;
     __device__ __forceinline__ Walk(const PairArgs &a, uint32_t pair) : u(0), u_end(0), round(0) {
-        if (pair < a.rest_pairs) {
+        if (a.cluster > 1) {
+            const uint32_t tile = pair / a.cluster, at = pair - tile * a.cluster;
+            u = tile * a.ksteps + at * a.ksteps / a.cluster;
+            u_end = tile * a.ksteps + (at + 1) * a.ksteps / a.cluster;
+        } else if (pair < a.rest_pairs) {
             u = rest_begin(a, pair);
             u_end = rest_begin(a, pair + 1);
         }
@@ -158,6 +167,16 @@ __device__ __forceinline__ uint32_t mapa(uint32_t addr, uint32_t rank) {
     uint32_t r;
     asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
     return r;
+}
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ float4 load_cluster(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+    return v;
 }
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release;" ::: "memory");
@@ -344,8 +363,7 @@ __device__ __forceinline__ void store_rows(const PairArgs &a, const float (&v)[3
 // 128 pass rows, three for up to 192: before the chains of eight above, steps of 80 and of 311 rows took 391 and 453 us with
 // room for four, 382 and 437 so; with them 399 and 440).
 template <int KIND, int CHUNKS>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TC_THREADS, 1)
-matmul_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap x_map, const PairArgs a) {
+__device__ __forceinline__ void pair_body(const CUtensorMap &w_map, const CUtensorMap &x_map, const PairArgs &a) {
     extern __shared__ __align__(1024) unsigned char smem[];
     __shared__ __align__(8) uint64_t bar_store[2 * TC_MAX_STAGES + 2 * TC_MAX_BUFS];
     __shared__ uint32_t tmem_base_s;
@@ -355,8 +373,9 @@ matmul_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_const
     __shared__ __align__(16) float scratch_s[8 * SCRATCH];
     float *scratch = scratch_s + ((threadIdx.x >> 5) & 7) * SCRATCH;
     __shared__ float4 stats_s[KIND == LOGPROBS ? CHUNKS : 1][8][KIND == LOGPROBS ? 32 : 1];   // of a tile, by chunks and warps
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const uint32_t rank = blockIdx.x & 1u, pair = blockIdx.x >> 1;
+    const uint32_t first = KIND < EPILOGUE ? 0u : cluster_rank() & ~1u;   // the pair's first CTA
     const uint32_t parts = KIND < EPILOGUE ? 2u : a.parts;
     const uint32_t S = a.stages, x_bytes = parts * a.bt * 64u, stage_bytes = W_BYTES + x_bytes;   // x: bt / 2 rows, the high part first
     const uint32_t base = smem_u32(smem);
@@ -376,7 +395,7 @@ matmul_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_const
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == TC_TMA_WARP && lane == 0) {
+    if (warp == TC_TMA_WARP && elect()) {
         prefetch_tensormap(&w_map);
         prefetch_tensormap(&x_map);
     }
@@ -390,81 +409,99 @@ matmul_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_const
     tc_fence_after();
     const uint32_t tmem = tmem_base_s;
 
-    if (warp == TC_TMA_WARP && lane == 0) {
-        // ---- producer -------------------------------------------------------------------------
-        const uint32_t full0 = mapa(b_full, 0);   // the first CTA's barriers count both CTAs' bytes
-        auto load_w = [&](uint32_t s, const Piece &p, uint32_t k) {
-            const uint32_t m0 = (p.tile / a.t_tiles) * TC_M + rank * 128u;
-            if (rank == 0) mbar_expect_tx(b_full + 8 * s, 2 * stage_bytes);
-            tma_load_4d_pair(base + s * stage_bytes, &w_map, (int)(k * TC_KSTEP), KIND == GLU ? 0 : (int)m0, 0, KIND == GLU ? (int)(m0 / (2 * GLU_GROUP)) : 0,
-                             full0 + 8 * s);
-        };
-        auto load_x = [&](uint32_t s, const Piece &p, uint32_t k) {
-            const uint32_t t0 = (p.tile % a.t_tiles) * a.bt + rank * (a.bt / 2);
-            tma_load_3d_pair(base + s * stage_bytes + W_BYTES, &x_map, (int)(k * TC_KSTEP), (int)t0, 0, full0 + 8 * s);
-        };
-        // The kernel ahead (the split of the activations) let this one start only after its own wait, so nothing
-        // that may still run writes the weights: the ring's first weights are on their way before the wait.  (Rows that are
-        // bf16 already have no split ahead of them.)
-        uint32_t ahead = 0;
-        if (KIND < EPILOGUE || a.early_w) {
-            Walk walk(a, pair);
-            Piece p;
-            while (ahead < S && walk.next(a, pair, p))
-                for (uint32_t k = p.k0; k < p.k1 && ahead < S; k++) load_w(ahead++, p, k);
-        }
-        asm volatile("griddepcontrol.wait;" ::: "memory");
-        asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-        Walk walk(a, pair);
-        Piece p;
-        uint32_t it = 0, s = 0, phase = 0;
-        while (walk.next(a, pair, p)) {
-            for (uint32_t k = p.k0; k < p.k1; k++, it++) {
-                if (it >= ahead) {
-                    mbar_wait(b_empty + 8 * s, phase ^ 1u, abortp, a.status, 501);
-                    if (*abortp) break;
-                    load_w(s, p, k);
-                }
-                load_x(s, p, k);
-                if (++s == S) {
-                    s = 0;
-                    phase ^= 1u;
+    if (warp == TC_TMA_WARP) {
+        if (elect()) {
+            // ---- producer -------------------------------------------------------------------------
+            // One thread issues every copy: nothing is computed in the loops that does not change there, and the thread is
+            // elected (see elect).  80 rows bf16 x [14336, 4096]: 34.7 us, without the divisions and the flag 31.8, elected 28.4.
+            const uint32_t full0 = mapa(b_full, first);   // the first CTA's barriers count both CTAs' bytes
+            struct Place {
+                int row, group, x;   // weight row (PLAIN) or group of them (GLU), pass row
+            };
+            auto place = [&](const Piece &p) {
+                const uint32_t at = p.tile / a.t_tiles, m0 = at * TC_M + rank * 128u;
+                return Place{KIND == GLU ? 0 : (int)m0, KIND == GLU ? (int)(m0 / (2 * GLU_GROUP)) : 0, (int)((p.tile - at * a.t_tiles) * a.bt + rank * (a.bt / 2))};
+            };
+            auto load_w = [&](uint32_t s, const Place &at, uint32_t k) {
+                if (rank == 0) mbar_expect_tx(b_full + 8 * s, 2 * stage_bytes);
+                tma_load_4d_pair(base + s * stage_bytes, &w_map, (int)(k * TC_KSTEP), at.row, 0, at.group, full0 + 8 * s);
+            };
+            auto load_x = [&](uint32_t s, const Place &at, uint32_t k) {
+                tma_load_3d_pair(base + s * stage_bytes + W_BYTES, &x_map, (int)(k * TC_KSTEP), at.x, 0, full0 + 8 * s);
+            };
+            // The kernel ahead (the split of the activations) let this one start only after its own wait, so nothing
+            // that may still run writes the weights: the ring's first weights are on their way before the wait.  (Rows that are
+            // bf16 already have no split ahead of them.)
+            uint32_t ahead = 0;
+            if (KIND < EPILOGUE || a.early_w) {
+                Walk walk(a, pair);
+                Piece p;
+                while (ahead < S && walk.next(a, pair, p)) {
+                    const Place at = place(p);
+                    for (uint32_t k = p.k0; k < p.k1 && ahead < S; k++) load_w(ahead++, at, k);
                 }
             }
-            if (*abortp) break;
-        }
-    } else if (warp == TC_MMA_WARP && lane == 0 && rank == 0) {
-        // ---- MMA issuer -----------------------------------------------------------------------
-        const uint32_t idesc = f16_instr_desc(true, false, TC_M, a.bt);
-        Walk walk(a, pair);
-        Piece p;
-        uint32_t s = 0, phase = 0;
-        AccTurn turn;
-        while (!*abortp && walk.next(a, pair, p)) {
-            for (uint32_t k0 = p.k0; k0 < p.k1 && !*abortp; turn.next(a.bufs)) {
-                const uint32_t acc = tmem + turn.buf * a.buf_columns, k_end = chain_end(a, p, k0);
-                if (turn.round > 0) mbar_wait(b_acc_empty + 8 * turn.buf, (turn.round - 1) & 1u, abortp, a.status, 502);
-                tc_fence_after();
-                for (uint32_t k = k0; k < k_end; k++) {
-                    mbar_wait(b_full + 8 * s, phase, abortp, a.status, 503);
-                    if (*abortp) break;
-                    tc_fence_after();
-                    const uint32_t w_lo = desc_lo(base + s * stage_bytes, 0), h_lo = w_lo + W_BYTES / 16;
-#pragma unroll
-                    for (uint32_t kk = 0; kk < 4; kk++) umma2_ss_lo(acc, w_lo + 2 * kk, h_lo + 2 * kk, idesc, k > k0 || kk > 0);
-                    for (uint32_t part = 1; part < parts; part++) {
-                        const uint32_t l_lo = h_lo + part * (a.bt * 4u);
-#pragma unroll
-                        for (uint32_t kk = 0; kk < 4; kk++) umma2_ss_lo(acc, w_lo + 2 * kk, l_lo + 2 * kk, idesc, 1);
+            asm volatile("griddepcontrol.wait;" ::: "memory");
+            asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+            Walk walk(a, pair);
+            Piece p;
+            uint32_t it = 0, s = 0, phase = 0;
+            bool gone = false;
+            while (!gone && walk.next(a, pair, p)) {
+                const Place at = place(p);
+                for (uint32_t k = p.k0; k < p.k1; k++, it++) {
+                    if (it >= ahead) {
+                        if (!mbar_try(b_empty + 8 * s, phase ^ 1u)) {
+                            mbar_wait_slow(b_empty + 8 * s, phase ^ 1u, abortp, a.status, 501);
+                            gone = *abortp;
+                            if (gone) break;
+                        }
+                        load_w(s, at, k);
                     }
-                    umma2_commit(b_empty + 8 * s);
+                    load_x(s, at, k);
                     if (++s == S) {
                         s = 0;
                         phase ^= 1u;
                     }
                 }
-                umma2_commit(b_acc_full + 8 * turn.buf);
-                k0 = k_end;
+            }
+        }
+    } else if (warp == TC_MMA_WARP) {
+        if (rank == 0 && elect()) {
+            // ---- MMA issuer -----------------------------------------------------------------------
+            const uint32_t idesc = f16_instr_desc(true, false, TC_M, a.bt);
+            Walk walk(a, pair);
+            Piece p;
+            uint32_t s = 0, phase = 0;
+            AccTurn turn;
+            while (!*abortp && walk.next(a, pair, p)) {
+                for (uint32_t k0 = p.k0; k0 < p.k1 && !*abortp; turn.next(a.bufs)) {
+                    const uint32_t acc = tmem + turn.buf * a.buf_columns, k_end = chain_end(a, p, k0);
+                    if (turn.round > 0) mbar_wait(b_acc_empty + 8 * turn.buf, (turn.round - 1) & 1u, abortp, a.status, 502);
+                    tc_fence_after();
+                    for (uint32_t k = k0; k < k_end; k++) {
+                        if (!mbar_try(b_full + 8 * s, phase)) {
+                            mbar_wait_slow(b_full + 8 * s, phase, abortp, a.status, 503);
+                            if (*abortp) break;
+                        }
+                        tc_fence_after();
+                        const uint32_t w_lo = desc_lo(base + s * stage_bytes, 0), h_lo = w_lo + W_BYTES / 16;
+#pragma unroll
+                        for (uint32_t kk = 0; kk < 4; kk++) umma2_ss_lo(acc, w_lo + 2 * kk, h_lo + 2 * kk, idesc, k > k0 || kk > 0);
+                        for (uint32_t part = 1; part < parts; part++) {
+                            const uint32_t l_lo = h_lo + part * (a.bt * 4u);
+#pragma unroll
+                            for (uint32_t kk = 0; kk < 4; kk++) umma2_ss_lo(acc, w_lo + 2 * kk, l_lo + 2 * kk, idesc, 1);
+                        }
+                        umma2_commit(b_empty + 8 * s, first);
+                        if (++s == S) {
+                            s = 0;
+                            phase ^= 1u;
+                        }
+                    }
+                    umma2_commit(b_acc_full + 8 * turn.buf, first);
+                    k0 = k_end;
+                }
             }
         }
     } else if (warp < 8) {
@@ -472,11 +509,12 @@ matmul_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_const
         Walk walk(a, pair);
         Piece p;
         AccTurn turn;
-        auto finish = [&](const float (&v)[32], uint32_t t, uint32_t row, uint32_t chunk) {
+        auto finish = [&](const auto &v, uint32_t t, uint32_t row, uint32_t chunk) {
+            constexpr int N = sizeof(v) / sizeof(float);
             if constexpr (KIND < EPILOGUE) store_rows<KIND == GLU>(a, v, t, row, lane);
             else if constexpr (KIND == EPILOGUE) {
-                stage<32>(v, 0, scratch, lane);
-                finish_staged<32>(a.e, a.out, a.T, a.cols, scratch, t, row - lane, lane);
+                stage<N>(v, 0, scratch, lane);
+                finish_staged<N>(a.e, a.out, a.T, a.cols, scratch, t, row - lane, lane);
             } else {
                 stats_s[chunk][warp][lane] = stats_of(a.so, a.T, a.cols, v, t, row, a.ids, scratch, lane);
             }
@@ -499,7 +537,7 @@ matmul_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_const
             // The pairs that share left-over tile `rest`, found while it is being summed.  Only the first of them may
             // have begun in the tile before it, which makes this tile its second piece.
             uint32_t q0 = 0, q1 = 0, second = 0;
-            if (!p.whole) {
+            if (!p.whole && (KIND < EPILOGUE || a.cluster == 1)) {
                 q0 = rest_owner(a, rest * a.ksteps);
                 q1 = rest_owner(a, (rest + 1) * a.ksteps - 1);
                 second = rest - rest_begin(a, q0) / a.ksteps;
@@ -531,7 +569,7 @@ matmul_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_const
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0)
-                    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(mapa(b_acc_empty + 8 * turn.buf, 0)) : "memory");
+                    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(mapa(b_acc_empty + 8 * turn.buf, first)) : "memory");
             }
             // A share's sums: four pass rows of each of 128 weight rows, then the next four.
             auto share = [&](uint32_t q) { return (float4 *)(a.part + ((size_t)(2 * q + (q == q0 ? second : 0u)) * 2 + rank) * a.bt * 128u) + wr; };
@@ -546,6 +584,20 @@ matmul_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_const
                         for (int i = 0; i < 32; i++) sum[j][i] = sum[j + 1][i];
                 }
             };
+            if constexpr (KIND >= EPILOGUE) {
+                if (a.cluster > 1) {
+                    // The pairs' sums stay in their shared memory, which no copy and no product needs any more.
+#pragma unroll
+                    for (int j = 0; j < CHUNKS; j++) {
+                        const uint32_t c = c0 + 64 * j;
+                        if (c >= a.bt) break;
+#pragma unroll
+                        for (int i = 0; i < 8; i++)
+                            *(float4 *)(smem + ((c / 4 + i) * 128u + wr) * 16u) = make_float4(sum[j][4 * i], sum[j][4 * i + 1], sum[j][4 * i + 2], sum[j][4 * i + 3]);
+                    }
+                    break;
+                }
+            }
             if (KIND >= EPILOGUE && p.whole) {
                 finish_all();
                 if constexpr (KIND == LOGPROBS) finish_stats(t0, c0, row);
@@ -610,13 +662,68 @@ matmul_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_const
         }
     }
     __syncwarp();
+    if constexpr (KIND >= EPILOGUE) {
+        if (a.cluster > 1) {
+            // Sixteen pass rows at a time are added up, in the order of k, and finished by one pair of the cluster.
+            cluster_sync();
+            const uint32_t tile = pair / a.cluster, at = pair - tile * a.cluster, wr = (warp & 3) * 32 + lane;
+            const uint32_t row = (tile / a.t_tiles) * TC_M + rank * 128u + wr, t0 = (tile % a.t_tiles) * a.bt;
+            for (uint32_t c = 16 * (at + a.cluster * (warp >> 2)); warp < 8 && c < a.bt && t0 + c < a.T; c += 32 * a.cluster) {
+                float4 f[MAX_CLUSTER][4];   // (all on their way at once)
+#pragma unroll
+                for (uint32_t q = 0; q < MAX_CLUSTER; q++) {
+                    const uint32_t from = mapa(base + (c / 4 * 128u + wr) * 16u, 2 * min(q, a.cluster - 1) + rank);
+#pragma unroll
+                    for (int i = 0; i < 4; i++) f[q][i] = load_cluster(from + i * 128u * 16u);
+                }
+                float v[16];
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    float4 sum = f[0][i];
+#pragma unroll
+                    for (uint32_t q = 1; q < MAX_CLUSTER; q++)
+                        if (q < a.cluster) sum = make_float4(sum.x + f[q][i].x, sum.y + f[q][i].y, sum.z + f[q][i].z, sum.w + f[q][i].w);
+                    v[4 * i] = sum.x;
+                    v[4 * i + 1] = sum.y;
+                    v[4 * i + 2] = sum.z;
+                    v[4 * i + 3] = sum.w;
+                }
+                if constexpr (KIND == EPILOGUE) {
+                    stage<16>(v, 0, scratch, lane);
+                    finish_staged<16>(a.e, a.out, a.T, a.cols, scratch, t0 + c, row - lane, lane);
+                } else {
+                    stats_s[0][warp][lane] = stats_of(a.so, a.T, a.cols, v, t0 + c, row, a.ids, scratch, lane);
+                    asm volatile("bar.sync %0, 128;" ::"r"(2 + (warp >> 2)) : "memory");
+                    const uint32_t t = t0 + c + lane;
+                    if ((warp & 3) == 0 && lane < 16 && t < a.T) {
+                        const float4 four[4] = {stats_s[0][warp][lane], stats_s[0][warp + 1][lane], stats_s[0][warp + 2][lane], stats_s[0][warp + 3][lane]};
+                        a.so.stats[(size_t)t * a.so.blocks + (row >> 7)] = merge_four(four);
+                    }
+                    asm volatile("bar.sync %0, 128;" ::"r"(2 + (warp >> 2)) : "memory");
+                }
+            }
+            __syncwarp();
+        }
+    }
     if (*abortp)
         for (int i = 0; i < 64; i++) __nanosleep(1000);   // copies and products in flight come to rest
     tc_fence_before();
     __syncthreads();
-    cluster_sync();   // the partner's copies and completions still land in this CTA
+    cluster_sync();   // the partner's copies and completions still land in this CTA, and its sums are read there
     tc_fence_after();
     if (warp == TC_MMA_WARP) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(512) : "memory");
+}
+
+template <int KIND, int CHUNKS>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TC_THREADS, 1)
+matmul_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap x_map, const __grid_constant__ PairArgs a) {
+    pair_body<KIND, CHUNKS>(w_map, x_map, a);
+}
+// (EPILOGUE and LOGPROBS: clusters of one to MAX_CLUSTER pairs)
+template <int KIND, int CHUNKS>
+__global__ void __launch_bounds__(TC_THREADS, 1)
+matmul_exact_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap x_map, const __grid_constant__ PairArgs a) {
+    pair_body<KIND, CHUNKS>(w_map, x_map, a);
 }
 
 // x [n] f32 -> its high and its low bf16 part, x = hi + lo to 16 bits of mantissa; eight elements a thread.
@@ -791,7 +898,7 @@ matmul_rows_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_const
     __shared__ __align__(16) float scratch_s[4 * SCRATCH];
     float *scratch = scratch_s + ((threadIdx.x >> 5) & 3) * SCRATCH;
     __shared__ float4 stats_s[4][KIND == LOGPROBS ? 32 : 1];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const uint32_t S = a.stages, base = smem_u32(smem);
     const uint32_t b_full = smem_u32(bar_store), b_empty = b_full + 8 * TC_MAX_STAGES;
     const uint32_t b_acc_full = b_empty + 8 * TC_MAX_STAGES, b_acc_empty = b_acc_full + 8 * ROWS_BUFS;
@@ -804,7 +911,7 @@ matmul_rows_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_const
         y = GLU_TILES ? 0 : (int)(tile * ROWS_M);
         z = GLU_TILES ? (int)(tile * (ROWS_M / (2 * GLU_GROUP))) : 0;
     };
-    if (warp == 4 && lane == 0) {
+    if (warp == 4 && elect()) {
         prefetch_tensormap(&w_map);
         for (uint32_t u = u0; u < u1 && u - u0 < S; u++) {
             int x, y, z;
@@ -837,15 +944,24 @@ matmul_rows_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_const
 
     if (warp == 4) {
         // ---- weights --------------------------------------------------------------------------
-        if (lane == 0) {
+        if (elect()) {
+            // (see the pair kernel's: one thread, and nothing in its loop that can be kept out)
             uint32_t s = 0, phase = 0;
+            int x, y, z;
+            weight_rows(u0, x, y, z);
             for (uint32_t u = u0; u < u1; u++) {
-                if (u - u0 >= S) mbar_wait(b_empty + 8 * s, phase ^ 1u, abortp, a.status, 511);
-                if (*abortp) break;
-                int x, y, z;
-                weight_rows(u, x, y, z);
+                if (u - u0 >= S && !mbar_try(b_empty + 8 * s, phase ^ 1u)) {
+                    mbar_wait_slow(b_empty + 8 * s, phase ^ 1u, abortp, a.status, 511);
+                    if (*abortp) break;
+                }
                 mbar_expect_tx(b_full + 8 * s, W_BYTES);
                 tma_load_4d(base + s * STAGE, &w_map, x, y, 0, z, b_full + 8 * s);
+                x += TC_KSTEP;
+                if (x == (int)(a.ksteps * TC_KSTEP)) {   // the next tile
+                    x = 0;
+                    if (GLU_TILES) z += ROWS_M / (2 * GLU_GROUP);
+                    else y += ROWS_M;
+                }
                 if (++s == S) {
                     s = 0;
                     phase ^= 1u;
@@ -854,7 +970,7 @@ matmul_rows_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_const
         }
     } else if (warp == 5) {
         // ---- MMA issuer -----------------------------------------------------------------------
-        if (lane == 0) {
+        if (elect()) {
             constexpr uint32_t idesc = f16_instr_desc(true, false, ROWS_M, NB);
             uint32_t s = 0, phase = 0, n = 0, piece_end = u0;
             for (uint32_t u = u0; u < u1 && !*abortp; n++) {
@@ -864,8 +980,10 @@ matmul_rows_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_const
                 if (n >= ROWS_BUFS) mbar_wait(b_acc_empty + 8 * buf, (n / ROWS_BUFS - 1) & 1u, abortp, a.status, 512);
                 tc_fence_after();
                 for (uint32_t first = u; u < end; u++) {
-                    mbar_wait(b_full + 8 * s, phase, abortp, a.status, 513);
-                    if (*abortp) break;
+                    if (!mbar_try(b_full + 8 * s, phase)) {
+                        mbar_wait_slow(b_full + 8 * s, phase, abortp, a.status, 513);
+                        if (*abortp) break;
+                    }
                     tc_fence_after();
                     const uint32_t w_lo = desc_lo(base + s * STAGE, 0), x_lo = w_lo + W_BYTES / 16;
 #pragma unroll
@@ -1121,30 +1239,43 @@ int ensure_counters(yx_ctx *ctx, size_t n) {
 // (what changes places takes 32 KiB, in LOGPROBS half of that with the statistics in the other)
 constexpr uint32_t smem_budget(int kind) { return kind < EPILOGUE ? TC_SMEM_BUDGET : 194 * 1024; }
 
-// CTA pairs that are on the chip together (a GPC with an odd number of SMs leaves one out).
 template <int KIND, int CHUNKS>
-int resident_pairs(yx_ctx *ctx, int *out) {
-    int &n = ctx->mm_pairs[KIND][CHUNKS - 2];
+constexpr auto pair_kernel() {
+    if constexpr (KIND < EPILOGUE) return matmul_pair_kernel<KIND, CHUNKS>;
+    else return matmul_exact_kernel<KIND, CHUNKS>;
+}
+
+// Clusters of `pairs` CTA pairs that are on the chip together (a GPC with an odd number of SMs leaves one out).
+template <int KIND, int CHUNKS>
+int resident_clusters(yx_ctx *ctx, int pairs, int *out) {
+    int &n = ctx->mm_clusters[KIND][CHUNKS - 2][pairs - 1];   // (0: not asked yet; -1: none)
     if (n == 0) {
-        auto *kernel = matmul_pair_kernel<KIND, CHUNKS>;
+        auto *kernel = pair_kernel<KIND, CHUNKS>();
         if (int rc = check_cuda(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_budget(KIND)),
                                 "matmul: shared memory attribute"))
             return rc;
         cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3((unsigned)ctx->sm_count / 2 * 2);
+        cfg.gridDim = dim3((unsigned)(ctx->sm_count / (2 * pairs) * 2 * pairs));
         cfg.blockDim = dim3(TC_THREADS);
         cfg.dynamicSmemBytes = smem_budget(KIND);
         cudaLaunchAttribute attr[1];
         attr[0].id = cudaLaunchAttributeClusterDimension;
-        attr[0].val.clusterDim.x = 2;
+        attr[0].val.clusterDim.x = 2 * pairs;
         attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
         cfg.attrs = attr;
         cfg.numAttrs = 1;
         int found = 0;
-        if (int rc = check_cuda(ctx, cudaOccupancyMaxActiveClusters(&found, kernel, &cfg), "matmul: resident pairs")) return rc;
-        n = std::max(1, std::min(found, ctx->sm_count / 2));
+        const cudaError_t e = cudaOccupancyMaxActiveClusters(&found, kernel, &cfg);
+        if (pairs == 1)
+            if (int rc = check_cuda(ctx, e, "matmul: resident pairs")) return rc;
+        if (e != cudaSuccess) {   // (a size this device does not place)
+            cudaGetLastError();
+            found = 0;
+        }
+        n = std::min(found, ctx->sm_count / (2 * pairs));
+        if (n == 0) n = pairs == 1 ? 1 : -1;
     }
-    *out = n;
+    *out = std::max(n, 0);
     return YX_OK;
 }
 
@@ -1171,7 +1302,8 @@ uint32_t share_rest(uint32_t tiles, uint32_t ksteps, uint32_t pairs, uint32_t bt
 template <int KIND, int CHUNKS>
 int plan_pairs(yx_ctx *ctx, const Product &p, PairArgs &a) {
     int pairs = 0;
-    if (int rc = resident_pairs<KIND, CHUNKS>(ctx, &pairs)) return rc;
+    if (int rc = resident_clusters<KIND, CHUNKS>(ctx, 1, &pairs)) return rc;
+    a.cluster = 1;
     a.T = p.T;
     a.cols = KIND == GLU ? p.N / 2 : p.N;
     a.parts = kind_parts(KIND, p.parts);
@@ -1182,7 +1314,22 @@ int plan_pairs(yx_ctx *ctx, const Product &p, PairArgs &a) {
     a.pairs = (uint32_t)pairs;
     a.rounds = tiles / a.pairs;
     a.rest_units = (tiles - a.rounds * a.pairs) * a.ksteps;
-    if (a.rest_units > 0) a.rest_pairs = share_rest(tiles - a.rounds * a.pairs, a.ksteps, a.pairs, a.bt, a.rounds > 0, 0.001f * (float)a.parts);
+    if (KIND >= EPILOGUE && a.rounds == 0) {
+        // Tiles that leave every other pair or more idle may be cut along k into one share for each pair of a cluster, whose
+        // sums meet in shared memory.  Meeting in scratch takes 9 ns a pass row and share longer; in exchange all pairs take
+        // part, not only whole clusters.  In scratch and in clusters, us: 80 rows bf16 x [4096, 4096] 19.7 and 17.1, 256 rows
+        // 31 and 22, 128 x [2048, 2048] 19.0 and 10.5, 512 f32 x [1024, 2816] 39 and 24; 80 x [4096, 14336] 36.8 and 39.7, 80 x [1024,
+        // 14336] 25.8 and 30.2.
+        for (uint32_t c = std::min({MAX_CLUSTER, a.pairs / tiles, a.ksteps}); c > 1; c--) {
+            int resident = 0;
+            if (int rc = resident_clusters<KIND, CHUNKS>(ctx, (int)c, &resident)) return rc;
+            if (tiles > (uint32_t)resident) continue;
+            const float step = 0.26f + 0.001f * (float)(a.parts * a.bt), more = (float)a.ksteps * (1.0f / (float)c - (float)tiles / (float)a.pairs);
+            if (1.2f * more * step < 0.0088f * (float)a.bt * (float)a.pairs / (float)tiles) a.cluster = c;
+            break;
+        }
+    }
+    if (a.cluster == 1 && a.rest_units > 0) a.rest_pairs = share_rest(tiles - a.rounds * a.pairs, a.ksteps, a.pairs, a.bt, a.rounds > 0, 0.001f * (float)a.parts);
     a.stages = std::min<uint32_t>(TC_MAX_STAGES, (smem_budget(KIND) - 1024) / (W_BYTES + a.parts * a.bt * 64u));
     a.bufs = a.bt <= 128 ? 4 : a.bt <= 160 ? 3 : 2;
     a.buf_columns = 512 / a.bufs / 32 * 32;
@@ -1199,9 +1346,11 @@ int plan_pairs(yx_ctx *ctx, const Product &p, PairArgs &a) {
 
 template <int KIND, int CHUNKS>
 int launch_pairs(yx_ctx *ctx, const CUtensorMap &w_map, const CUtensorMap &x_map, const PairArgs &a) {
-    const uint32_t grid = 2 * (a.rounds > 0 ? a.pairs : a.rest_pairs);
-    return launch_dependent(ctx, "matmul kernel launch", matmul_pair_kernel<KIND, CHUNKS>, dim3(grid), dim3(TC_THREADS),
-                            a.stages * (W_BYTES + a.parts * a.bt * 64u), w_map, x_map, a);
+    const uint32_t shares = a.cluster > 1 ? a.rest_units / a.ksteps * a.cluster : a.rest_pairs;
+    const dim3 grid(2 * (a.rounds > 0 ? a.pairs : shares)), block(TC_THREADS);
+    const size_t smem = a.stages * (W_BYTES + a.parts * a.bt * 64u);
+    if constexpr (KIND < EPILOGUE) return launch_dependent(ctx, "matmul kernel launch", pair_kernel<KIND, CHUNKS>(), grid, block, smem, w_map, x_map, a);
+    else return launch_cluster(ctx, "matmul kernel launch", pair_kernel<KIND, CHUNKS>(), grid, block, smem, 2 * a.cluster, w_map, x_map, a);
 }
 
 // The map of `parts` matrices [T, K] one behind the other: a CTA's half of a tile's rows, of every part.

@@ -196,18 +196,26 @@ __device__ __forceinline__ unsigned long long gtime() {
 // kernels (2 to 3 us) out of the chain of a decode step.  The kernel begins with
 // griddepcontrol.wait (dev::dependent_entry, or later where it has work that needs no wait).
 template <typename... P, typename... A>
-int launch_dependent(yx_ctx *ctx, const char *what, void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, A... args) {
+int launch_cluster(yx_ctx *ctx, const char *what, void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, uint32_t cluster, A... args) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = block;
     cfg.dynamicSmemBytes = smem;
     cfg.stream = ctx->stream;
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = cluster;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = cluster > 0 ? 2 : 1;
     ctx->launches++;
     return check_cuda(ctx, cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...), what);
+}
+// (a kernel without clusters, or whose clusters are its own affair)
+template <typename... P, typename... A>
+int launch_dependent(yx_ctx *ctx, const char *what, void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, A... args) {
+    return launch_cluster(ctx, what, kernel, grid, block, smem, 0, args...);
 }
 }  // namespace yx

@@ -7,6 +7,15 @@
 namespace yx {
 namespace dev {
 
+// One thread of a warp, for work that a single thread issues.  The compiler knows that a branch on this has one thread in
+// it, and takes the operands of copies and products there as they are; in a branch on a lane's number it makes each of them
+// uniform first, which doubled what a k step of the matmul kernels costs their issuing threads.
+__device__ __forceinline__ bool elect() {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+    return r != 0;
+}
+
 // The low word of a shared-memory matrix descriptor (start address and leading offset, 16-byte units) and
 // the constant high word (stride 1024 bytes, version 1, 128-byte swizzle): stepping an operand along K
 // is then one add, which matters because a single thread issues every MMA of a CTA.
@@ -38,8 +47,9 @@ __device__ __forceinline__ void umma2_ss_lo(uint32_t d_tmem, uint32_t a_lo, uint
                  "r"(a_lo), "r"(b_lo), "r"(DESC_HI), "r"(idesc), "r"(acc)
                  : "memory");
 }
-__device__ __forceinline__ void umma2_commit(uint32_t bar) {
-    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((uint16_t)3)
+// `first`: the pair's first CTA's rank in its cluster.
+__device__ __forceinline__ void umma2_commit(uint32_t bar, uint32_t first = 0) {
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((uint16_t)(3u << first))
                  : "memory");
 }
 
