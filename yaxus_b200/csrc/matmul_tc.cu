@@ -837,11 +837,13 @@ constexpr uint32_t ROWS_MAX = 32;           // pass rows
 // what lies below its accumulator's last place: chains of 64 steps erred by 8.1e-6 of a GLU's result (16 rows x
 // [28672, 4096]), the mma.sync kernel by 4.2e-6.  Chains of 16 are
 // at 4.0e-6 (but 3.9e-6 against 3.7e-6 for twenty rows x [11264, 2048]), chains of eight at 3.7e-6 for 1.5 % of a step.
+constexpr uint32_t ROWS_CLUSTER = 8;        // CTAs of a cluster, at most
 constexpr uint32_t ROWS_CHAIN = 8, ROWS_BUFS = 4;   // (and four accumulators: the tensor cores run on while an epilogue adds shares up)
 
 struct RowsArgs {
     const void *x;
     uint32_t T, K, cols, ksteps, units, ctas, stages;
+    uint32_t cluster;                 // CTAs that share a tile as one cluster (EPILOGUE, LOGPROBS; 1: none)
     uint32_t x_vec16;
     float *out;
     Epilogue e;                       // EPILOGUE (`out` is of its type)
@@ -903,7 +905,15 @@ matmul_rows_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_const
     const uint32_t b_full = smem_u32(bar_store), b_empty = b_full + 8 * TC_MAX_STAGES;
     const uint32_t b_acc_full = b_empty + 8 * TC_MAX_STAGES, b_acc_empty = b_acc_full + 8 * ROWS_BUFS;
     volatile int *abortp = &abort_flag;
-    const uint32_t u0 = share_begin(a, blockIdx.x), u1 = share_begin(a, blockIdx.x + 1);
+    uint32_t u0, u1;
+    if (KIND >= EPILOGUE && a.cluster > 1) {
+        const uint32_t tile = blockIdx.x / a.cluster, at = blockIdx.x - tile * a.cluster;
+        u0 = tile * a.ksteps + at * a.ksteps / a.cluster;
+        u1 = tile * a.ksteps + (at + 1) * a.ksteps / a.cluster;
+    } else {
+        u0 = share_begin(a, blockIdx.x);
+        u1 = share_begin(a, blockIdx.x + 1);
+    }
 
     auto weight_rows = [&](uint32_t u, int &x, int &y, int &z) {
         const uint32_t tile = u / a.ksteps;
@@ -941,6 +951,22 @@ matmul_rows_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_const
     const uint32_t tmem = tmem_base_s;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+    auto finish = [&](const float (&v)[TP], uint32_t row) {
+        if constexpr (KIND < EPILOGUE) store_few<TP, KIND == GLU>(a, v, row, lane);
+        else if constexpr (KIND == EPILOGUE) {
+            stage<TP>(v, 0, scratch, lane);
+            finish_staged<TP>(a.e, a.out, a.T, a.cols, scratch, 0, row - lane, lane);
+        } else {
+            stats_s[warp][lane] = stats_of(a.so, a.T, a.cols, v, 0, row, a.ids, scratch, lane);
+            asm volatile("bar.sync 2, 128;" ::: "memory");
+            if (warp == 0 && lane < (int)a.T) {
+                const float4 four[4] = {stats_s[0][lane], stats_s[1][lane], stats_s[2][lane], stats_s[3][lane]};
+                a.so.stats[(size_t)lane * a.so.blocks + (row >> 7)] = merge_four(four);
+            }
+            asm volatile("bar.sync 2, 128;" ::: "memory");
+        }
+    };
 
     if (warp == 4) {
         // ---- weights --------------------------------------------------------------------------
@@ -1069,21 +1095,6 @@ matmul_rows_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_const
     } else {
         // ---- epilogue -------------------------------------------------------------------------
         uint32_t n = 0;
-        auto finish = [&](const float (&v)[TP], uint32_t row) {
-            if constexpr (KIND < EPILOGUE) store_few<TP, KIND == GLU>(a, v, row, lane);
-            else if constexpr (KIND == EPILOGUE) {
-                stage<TP>(v, 0, scratch, lane);
-                finish_staged<TP>(a.e, a.out, a.T, a.cols, scratch, 0, row - lane, lane);
-            } else {
-                stats_s[warp][lane] = stats_of(a.so, a.T, a.cols, v, 0, row, a.ids, scratch, lane);
-                asm volatile("bar.sync 2, 128;" ::: "memory");
-                if (warp == 0 && lane < (int)a.T) {
-                    const float4 four[4] = {stats_s[0][lane], stats_s[1][lane], stats_s[2][lane], stats_s[3][lane]};
-                    a.so.stats[(size_t)lane * a.so.blocks + (row >> 7)] = merge_four(four);
-                }
-                asm volatile("bar.sync 2, 128;" ::: "memory");
-            }
-        };
         for (uint32_t u = u0; u < u1;) {
             const uint32_t tile = u / a.ksteps, end = min(u1, (tile + 1) * a.ksteps);
             const bool whole = end - u == a.ksteps;
@@ -1091,7 +1102,7 @@ matmul_rows_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_const
             // The CTAs that share this tile, found while the tile is being summed (the divisions take a third of a
             // microsecond).  Only the first of them may have begun in a tile before it: then this is its last piece.
             uint32_t q0 = 0, q1 = 0, later = 0;
-            if (!whole) {
+            if (!whole && (KIND < EPILOGUE || a.cluster == 1)) {
                 q0 = share_owner(a, tile * a.ksteps);
                 q1 = share_owner(a, (tile + 1) * a.ksteps - 1);
                 later = share_begin(a, q0) < tile * a.ksteps;
@@ -1146,6 +1157,13 @@ matmul_rows_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_const
                 finish(v, row);
                 continue;
             }
+            if constexpr (KIND >= EPILOGUE) {
+                if (a.cluster > 1) {   // (as in the pair kernel: the sums stay in shared memory)
+#pragma unroll
+                    for (int i = 0; i < TP; i += 4) *(float4 *)(smem + (i / 4 * 128u + wr) * 16u) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+                    break;
+                }
+            }
             auto share = [&](uint32_t q) { return a.part + (size_t)(2 * q + (q == q0 ? later : 0u)) * TP * 128u + wr; };
             float *mine = share(blockIdx.x);
 #pragma unroll
@@ -1182,6 +1200,29 @@ matmul_rows_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_const
         }
     }
     __syncwarp();
+    if constexpr (KIND >= EPILOGUE) {
+        if (a.cluster > 1) {
+            // The cluster's first CTA adds up, in the order of k, and finishes.
+            cluster_sync();
+            if (blockIdx.x % a.cluster == 0 && warp < 4) {
+                const uint32_t wr = warp * 32 + lane;
+                float v[TP];
+#pragma unroll
+                for (int i = 0; i < TP; i += 4) {
+                    float4 f[ROWS_CLUSTER];
+#pragma unroll
+                    for (uint32_t q = 0; q < ROWS_CLUSTER; q++) f[q] = load_cluster(mapa(base + (i / 4 * 128u + wr) * 16u, min(q, a.cluster - 1)));
+#pragma unroll
+                    for (uint32_t q = 1; q < ROWS_CLUSTER; q++)
+                        if (q < a.cluster) f[0] = make_float4(f[0].x + f[q].x, f[0].y + f[q].y, f[0].z + f[q].z, f[0].w + f[q].w);
+                    *(float4 *)(v + i) = f[0];
+                }
+                finish(v, blockIdx.x / a.cluster * ROWS_M + wr);
+            }
+            __syncwarp();
+            cluster_sync();   // the sums are read
+        }
+    }
     if (*abortp)
         for (int i = 0; i < 64; i++) __nanosleep(1000);   // copies and products in flight come to rest
     tc_fence_before();
@@ -1245,38 +1286,42 @@ constexpr auto pair_kernel() {
     else return matmul_exact_kernel<KIND, CHUNKS>;
 }
 
-// Clusters of `pairs` CTA pairs that are on the chip together (a GPC with an odd number of SMs leaves one out).
-template <int KIND, int CHUNKS>
-int resident_clusters(yx_ctx *ctx, int pairs, int *out) {
-    int &n = ctx->mm_clusters[KIND][CHUNKS - 2][pairs - 1];   // (0: not asked yet; -1: none)
-    if (n == 0) {
-        auto *kernel = pair_kernel<KIND, CHUNKS>();
-        if (int rc = check_cuda(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_budget(KIND)),
-                                "matmul: shared memory attribute"))
-            return rc;
+// Clusters of `size` CTAs that are on the chip together (a GPC leaves some of its SMs out).  `known` remembers: 0 not asked
+// yet, -1 none.  The kernel's shared memory is opted in for.
+template <typename Kernel>
+int resident_of(yx_ctx *ctx, int *known, Kernel kernel, unsigned threads, size_t smem, uint32_t size, int *out) {
+    if (*known == 0) {
         cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3((unsigned)(ctx->sm_count / (2 * pairs) * 2 * pairs));
-        cfg.blockDim = dim3(TC_THREADS);
-        cfg.dynamicSmemBytes = smem_budget(KIND);
+        cfg.gridDim = dim3((unsigned)ctx->sm_count / size * size);
+        cfg.blockDim = dim3(threads);
+        cfg.dynamicSmemBytes = smem;
         cudaLaunchAttribute attr[1];
         attr[0].id = cudaLaunchAttributeClusterDimension;
-        attr[0].val.clusterDim.x = 2 * pairs;
+        attr[0].val.clusterDim.x = size;
         attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
         cfg.attrs = attr;
         cfg.numAttrs = 1;
         int found = 0;
         const cudaError_t e = cudaOccupancyMaxActiveClusters(&found, kernel, &cfg);
-        if (pairs == 1)
-            if (int rc = check_cuda(ctx, e, "matmul: resident pairs")) return rc;
         if (e != cudaSuccess) {   // (a size this device does not place)
             cudaGetLastError();
             found = 0;
         }
-        n = std::min(found, ctx->sm_count / (2 * pairs));
-        if (n == 0) n = pairs == 1 ? 1 : -1;
+        found = std::min(found, ctx->sm_count / (int)size);
+        *known = found > 0 ? found : -1;
     }
-    *out = std::max(n, 0);
+    *out = std::max(*known, 0);
     return YX_OK;
+}
+template <int KIND, int CHUNKS>
+int resident_clusters(yx_ctx *ctx, int pairs, int *out) {
+    auto *kernel = pair_kernel<KIND, CHUNKS>();
+    int &n = ctx->mm_clusters[KIND][CHUNKS - 2][pairs - 1];
+    if (n == 0)
+        if (int rc = check_cuda(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_budget(KIND)), "matmul: shared memory attribute"))
+            return rc;
+    if (int rc = resident_of(ctx, &n, kernel, TC_THREADS, smem_budget(KIND), 2 * pairs, out)) return rc;
+    return pairs > 1 || *out > 0 ? YX_OK : fail(ctx, YX_ERR_CUDA, "matmul: no CTA pair is placed");
 }
 
 // Pass rows are spread evenly over as few tiles as hold them: 300 rows are two tiles of 160, not 256 and 64.
@@ -1315,17 +1360,15 @@ int plan_pairs(yx_ctx *ctx, const Product &p, PairArgs &a) {
     a.rounds = tiles / a.pairs;
     a.rest_units = (tiles - a.rounds * a.pairs) * a.ksteps;
     if (KIND >= EPILOGUE && a.rounds == 0) {
-        // Tiles that leave every other pair or more idle may be cut along k into one share for each pair of a cluster, whose
-        // sums meet in shared memory.  Meeting in scratch takes 9 ns a pass row and share longer; in exchange all pairs take
-        // part, not only whole clusters.  In scratch and in clusters, us: 80 rows bf16 x [4096, 4096] 19.7 and 17.1, 256 rows
-        // 31 and 22, 128 x [2048, 2048] 19.0 and 10.5, 512 f32 x [1024, 2816] 39 and 24; 80 x [4096, 14336] 36.8 and 39.7, 80 x [1024,
-        // 14336] 25.8 and 30.2.
+        // Tiles that leave every other pair or more idle are cut along k into one share for each pair of a cluster, whose
+        // sums meet in shared memory.  Through scratch and through clusters, us: 80 rows bf16 x [4096, 4096] 17.9 and 13.3, 256 rows
+        // 30 and 20, 128 x [2048, 2048] 18.4 and 8.7, 512 f32 x [1024, 2816] 39 and 23; even where clusters leave half of the pairs
+        // without work, as 80 x [1024, 14336] does, 24.7 and 18.8.
         for (uint32_t c = std::min({MAX_CLUSTER, a.pairs / tiles, a.ksteps}); c > 1; c--) {
             int resident = 0;
             if (int rc = resident_clusters<KIND, CHUNKS>(ctx, (int)c, &resident)) return rc;
             if (tiles > (uint32_t)resident) continue;
-            const float step = 0.26f + 0.001f * (float)(a.parts * a.bt), more = (float)a.ksteps * (1.0f / (float)c - (float)tiles / (float)a.pairs);
-            if (1.2f * more * step < 0.0088f * (float)a.bt * (float)a.pairs / (float)tiles) a.cluster = c;
+            a.cluster = c;
             break;
         }
     }
@@ -1468,6 +1511,18 @@ int matmul_few_rows(yx_ctx *ctx, const Product &p) {
     const uint32_t tiles = (N + ROWS_M - 1) / ROWS_M;
     a.units = tiles * a.ksteps;
     a.ctas = std::min((uint32_t)ctx->sm_count, std::max(1u, a.units / 2));
+    a.cluster = 1;
+    if constexpr (KIND >= EPILOGUE) {
+        // (as in the pair kernel)
+        for (uint32_t c = std::min({ROWS_CLUSTER, (uint32_t)ctx->sm_count / tiles, a.ksteps}); c > 1; c--) {
+            int resident = 0;
+            if (int rc = resident_of(ctx, &ctx->mm_rows_clusters[KIND][PARTS - 1][TP / 16][c - 1], kernel, ROWS_THREADS, stages * stage_bytes, c, &resident)) return rc;
+            if (tiles > (uint32_t)resident) continue;
+            a.cluster = c;
+            a.ctas = tiles * c;
+            break;
+        }
+    }
     a.stages = stages;
     a.x_vec16 = ((uintptr_t)a.x & 15u) == 0;
     a.out = (float *)p.out;
@@ -1487,7 +1542,7 @@ int matmul_few_rows(yx_ctx *ctx, const Product &p) {
     CUtensorMap w_map;
     if (int rc = encode_weights(ctx, &w_map, p.w, N, K, KIND == GLU)) return rc;
     ctx->last_launch = yx_ctx::LAST_OTHER;
-    return launch_dependent(ctx, "matmul kernel launch", kernel, dim3(a.ctas), dim3(ROWS_THREADS), stages * stage_bytes, w_map, a);
+    return launch_cluster(ctx, "matmul kernel launch", kernel, dim3(a.ctas), dim3(ROWS_THREADS), stages * stage_bytes, a.cluster > 1 ? a.cluster : 0, w_map, a);
 }
 
 template <int KIND>
