@@ -250,8 +250,10 @@ struct Tile {
 // first tile hardly any thread's m moves again (with m the largest so far, some lane of a warp moved it in most tiles).
 constexpr float HEADROOM = 8.0f;
 
+// Five CTAs an SM: 48 registers a thread, and two or three of them spilled (2048 rows of 50257 bf16 with five tokens 58 us; four
+// CTAs 64, three 73, six with half the logits in flight each 69).
 template <int DTYPE, bool TOP>
-__global__ void __launch_bounds__(THREADS, 4) logprob_rows_kernel(const __grid_constant__ RowsArgs a) {
+__global__ void __launch_bounds__(THREADS, 5) logprob_rows_kernel(const __grid_constant__ RowsArgs a) {
     __shared__ Best b;
     __shared__ RowStats scratch[2][WARPS];
     __shared__ bool last;
