@@ -60,11 +60,12 @@ constexpr uint32_t TC_SMEM_BUDGET = 220 * 1024;
 // 80 rows pays 19 us of 399 for chains of eight in place of 16.
 constexpr uint32_t TC_CHAIN = 16, TC_FIRST_CHAIN = 32, TC_SHORT_CHAIN = 8, TC_CUT_CHAIN = 6, TC_LEAST_CHAIN = 4;
 constexpr int TC_MAX_BUFS = 4;
-// The same for rows taken exactly (EPILOGUE, LOGPROBS), by their parts: what keeps the result within a millionth (2-norm of
-// the error over the result's, 2048 x [14336, 4096] and 80 x [4096, 4096]: one part in chains of 4, 8 and 12 steps 2.4, 4.7 and 7.1e-7,
-// two of 3 and 6 4.5 and 8.3e-7, three of 2, 3 and 4 7.1, 9.3 and 11.6e-7; yx_matmul 27e-7).  Results of 16 bits keep none of it.
+// The same for rows taken exactly (EPILOGUE, LOGPROBS), by their parts: what keeps the result well within a millionth (2-norm
+// of the error over the result's, 2048 x [14336, 4096]: one part in chains of 8, 12 and 16 steps 4.7, 7.1 and 9.9e-7 and 235, 225 and
+// 216 us, two of 4, 6 and 8 4.7, 7.2 and 10.1e-7 and 369, 356 and 348 us, three of 2, 3 and 4 3.4, 5.5 and 7.7e-7 and 547, 514 and 505 us; a library's
+// f32 products 6 to 12e-7, yx_matmul 27e-7).  Results of 16 bits keep none of it.
 constexpr uint32_t MAX_CLUSTER = 4;         // pairs of a cluster (eight CTAs: the most that any chip of this kind places)
-constexpr uint32_t EXACT_CHAIN[3] = {12, 6, 3}, NARROW_CHAIN = 32;
+constexpr uint32_t EXACT_CHAIN[3] = {12, 6, 4}, NARROW_CHAIN = 32;
 constexpr uint32_t GLU_GROUP = 16;          // gate and up rows alternate in a tile sixteen by sixteen: a warp holds both
 
 // What becomes of a product.
@@ -486,12 +487,19 @@ __device__ __forceinline__ void pair_body(const CUtensorMap &w_map, const CUtens
                         }
                         tc_fence_after();
                         const uint32_t w_lo = desc_lo(base + s * stage_bytes, 0), h_lo = w_lo + W_BYTES / 16;
+                        if constexpr (KIND < EPILOGUE) {
 #pragma unroll
-                        for (uint32_t kk = 0; kk < 4; kk++) umma2_ss_lo(acc, w_lo + 2 * kk, h_lo + 2 * kk, idesc, k > k0 || kk > 0);
-                        for (uint32_t part = 1; part < parts; part++) {
-                            const uint32_t l_lo = h_lo + part * (a.bt * 4u);
+                            for (uint32_t kk = 0; kk < 4; kk++) umma2_ss_lo(acc, w_lo + 2 * kk, h_lo + 2 * kk, idesc, k > k0 || kk > 0);
 #pragma unroll
-                            for (uint32_t kk = 0; kk < 4; kk++) umma2_ss_lo(acc, w_lo + 2 * kk, l_lo + 2 * kk, idesc, 1);
+                            for (uint32_t kk = 0; kk < 4; kk++) umma2_ss_lo(acc, w_lo + 2 * kk, h_lo + a.bt * 4u + 2 * kk, idesc, 1);
+                        } else {
+                            // The smallest part first: in a chain's first step the large sum is not there yet to drop its bits.
+                            for (uint32_t part = parts; part-- > 0;) {
+                                const uint32_t x_lo = h_lo + part * (a.bt * 4u);
+                                const bool fresh = k == k0 && part == parts - 1;
+#pragma unroll
+                                for (uint32_t kk = 0; kk < 4; kk++) umma2_ss_lo(acc, w_lo + 2 * kk, x_lo + 2 * kk, idesc, !fresh || kk > 0);
+                            }
                         }
                         umma2_commit(b_empty + 8 * s, first);
                         if (++s == S) {
