@@ -1333,9 +1333,40 @@ int resident_clusters(yx_ctx *ctx, int pairs, int *out) {
 }
 
 // Pass rows are spread evenly over as few tiles as hold them: 300 rows are two tiles of 160, not 256 and 64.
-uint32_t tile_rows(uint32_t T) {
-    const uint32_t tiles = (T + TC_MAX_BT - 1) / TC_MAX_BT;
-    return ((T + tiles - 1) / tiles + 31) / 32 * 32;
+uint32_t rows_of_tiles(uint32_t T, uint32_t tiles) { return ((T + tiles - 1) / tiles + 31) / 32 * 32; }
+uint32_t tile_rows(uint32_t T) { return rows_of_tiles(T, (T + TC_MAX_BT - 1) / TC_MAX_BT); }
+
+// Pairs of a cluster for each of `tiles` tiles: as many as the chip places at once.
+template <int KIND, int CHUNKS>
+int cluster_for(yx_ctx *ctx, uint32_t tiles, uint32_t ksteps, uint32_t *out) {
+    *out = 1;
+    for (uint32_t c = std::min({MAX_CLUSTER, (uint32_t)ctx->sm_count / 2 / tiles, ksteps}); c > 1; c--) {
+        int resident = 0;
+        if (int rc = resident_clusters<KIND, CHUNKS>(ctx, (int)c, &resident)) return rc;
+        if (tiles > (uint32_t)resident) continue;
+        *out = c;
+        break;
+    }
+    return YX_OK;
+}
+
+// Tiles that pass rows taken exactly are spread over.  More than hold them where that leaves fewer pairs idle: a k step takes
+// a CTA what its 16 KiB of weights and 64 bytes a pass row and part take at some 60 bytes a nanosecond, and pairs of a
+// cluster share it (300 f32 rows x [5633, 2040]: 46 tiles of 160 rows 34.6 us, 69 of 128 29.7; 600 bf16 x [4096, 4096] 40.3 and 27.7).
+template <int KIND>
+int exact_row_tiles(yx_ctx *ctx, const Product &p, uint32_t *out) {
+    const uint32_t columns = (p.N + TC_M - 1) / TC_M, least = (p.T + TC_MAX_BT - 1) / TC_MAX_BT, ksteps = (p.K + TC_KSTEP - 1) / TC_KSTEP;
+    *out = least;
+    float best = 0.0f;
+    for (uint32_t t = least; t <= least + 4 && (uint64_t)columns * t <= (uint64_t)ctx->sm_count / 2; t++) {
+        uint32_t shared = 1;
+        if (int rc = cluster_for<KIND, 2>(ctx, columns * t, ksteps, &shared)) return rc;
+        const float cost = (16384.0f + 64.0f * (float)(p.parts * (int)rows_of_tiles(p.T, t))) / (float)shared;
+        if (t > least && cost >= best) continue;
+        *out = t;
+        best = cost;
+    }
+    return YX_OK;
 }
 
 // How many pairs share the k steps of `tiles` left-over tiles.  Either every tile is cut into the same number of
@@ -1360,25 +1391,20 @@ int plan_pairs(yx_ctx *ctx, const Product &p, PairArgs &a) {
     a.T = p.T;
     a.cols = KIND == GLU ? p.N / 2 : p.N;
     a.parts = kind_parts(KIND, p.parts);
-    a.t_tiles = (p.T + TC_MAX_BT - 1) / TC_MAX_BT;
-    a.bt = tile_rows(p.T);
+    a.t_tiles = KIND < EPILOGUE ? (p.T + TC_MAX_BT - 1) / TC_MAX_BT : p.t_tiles;
+    a.bt = rows_of_tiles(p.T, a.t_tiles);
     a.ksteps = (p.K + TC_KSTEP - 1) / TC_KSTEP;
     const uint32_t tiles = ((p.N + TC_M - 1) / TC_M) * a.t_tiles;
     a.pairs = (uint32_t)pairs;
     a.rounds = tiles / a.pairs;
     a.rest_units = (tiles - a.rounds * a.pairs) * a.ksteps;
-    if (KIND >= EPILOGUE && a.rounds == 0) {
+    if constexpr (KIND >= EPILOGUE) {
         // Tiles that leave every other pair or more idle are cut along k into one share for each pair of a cluster, whose
         // sums meet in shared memory.  Through scratch and through clusters, us: 80 rows bf16 x [4096, 4096] 17.9 and 13.3, 256 rows
         // 30 and 20, 128 x [2048, 2048] 18.4 and 8.7, 512 f32 x [1024, 2816] 39 and 23; even where clusters leave half of the pairs
         // without work, as 80 x [1024, 14336] does, 24.7 and 18.8.
-        for (uint32_t c = std::min({MAX_CLUSTER, a.pairs / tiles, a.ksteps}); c > 1; c--) {
-            int resident = 0;
-            if (int rc = resident_clusters<KIND, CHUNKS>(ctx, (int)c, &resident)) return rc;
-            if (tiles > (uint32_t)resident) continue;
-            a.cluster = c;
-            break;
-        }
+        if (a.rounds == 0)
+            if (int rc = cluster_for<KIND, CHUNKS>(ctx, tiles, a.ksteps, &a.cluster)) return rc;
     }
     if (a.cluster == 1 && a.rest_units > 0) a.rest_pairs = share_rest(tiles - a.rounds * a.pairs, a.ksteps, a.pairs, a.bt, a.rounds > 0, 0.001f * (float)a.parts);
     a.stages = std::min<uint32_t>(TC_MAX_STAGES, (smem_budget(KIND) - 1024) / (W_BYTES + a.parts * a.bt * 64u));
@@ -1576,10 +1602,12 @@ template <int KIND>
 int exact_tc(yx_ctx *ctx, const Product &p) {
     if (p.T <= ROWS_MAX)
         return p.parts == 1 ? exact_few_rows<KIND, 1>(ctx, p) : p.parts == 2 ? exact_few_rows<KIND, 2>(ctx, p) : exact_few_rows<KIND, 3>(ctx, p);
-    const uint32_t rows = tile_rows(p.T);
-    if (rows <= 128) return exact_pair_rows<KIND, 2>(ctx, p);
-    if (rows <= 192) return exact_pair_rows<KIND, 3>(ctx, p);
-    return exact_pair_rows<KIND, 4>(ctx, p);
+    Product q = p;
+    if (int rc = exact_row_tiles<KIND>(ctx, p, &q.t_tiles)) return rc;
+    const uint32_t rows = rows_of_tiles(p.T, q.t_tiles);
+    if (rows <= 128) return exact_pair_rows<KIND, 2>(ctx, q);
+    if (rows <= 192) return exact_pair_rows<KIND, 3>(ctx, q);
+    return exact_pair_rows<KIND, 4>(ctx, q);
 }
 
 }  // namespace

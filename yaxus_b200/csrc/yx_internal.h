@@ -408,6 +408,7 @@ struct Product {
     const void *x, *w;
     uint32_t T, N, K;
     int parts;
+    uint32_t t_tiles;        // tiles that more than 32 pass rows are spread over
     void *out;
     Epilogue e;              // yx_matmul_epilogue
     void *stats;             // yx_matmul_logprobs: float4 [T][blocks], blocks = logprobs_block(p)
