@@ -185,6 +185,16 @@ def test_many_rows(backend, rows, cols):
     check(x, ids, 3, r)
 
 
+@pytest.mark.parametrize("rows,n_ids", [(2, 300), (100, 10), (3, 2667), (1, 17001)])
+def test_many_given_tokens(backend, rows, n_ids):
+    # past what rides in the kernel's parameters, in one launch and in several
+    x = logits_of(rows, 5003, torch.float32)
+    ids = np.random.default_rng(n_ids).integers(0, 5003, (rows, n_ids))
+    r = backend.logprob_rows(x, ids)
+    backend.sync()
+    check(x, ids, 0, r)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 def test_rows_off_any_alignment(backend, dtype):
     # a first row that starts one element past an aligned address, rows an odd number of elements apart
@@ -315,6 +325,8 @@ def test_refusals(backend):
         lambda: L.yx_logprob_rows(c, None, 0, 2, 50, 50, i, 1, 0, o, None, None, None),     # no logits
         lambda: L.yx_logprob_rows(c, p, 0, 2, 0, 50, i, 1, 0, o, None, None, None),         # no columns
         lambda: L.yx_logprob_rows(c, p, 0, 2, 50, 49, i, 1, 0, o, None, None, None),        # rows over one another
+        lambda: L.yx_logprob_rows(c, p, 0, 1, 2 ** 31, 2 ** 31, i, 1, 0, o, None, None, None),   # too long a row
+        lambda: L.yx_matmul_logprobs(c, h.data_ptr(), 0, w.data_ptr(), 2, 2 ** 31, 64, i, o, None),
         lambda: L.yx_logprob_rows(c, p + 2, 0, 2, 50, 50, i, 1, 0, o, None, None, None),    # off alignment
         lambda: L.yx_logprob_rows(c, p, 0, 2, 50, 50, i, 1, 0, o + 1, None, None, None),
         lambda: L.yx_logprob_rows(c, p, 0, 2, 50, 50, bad.ctypes.data, 1, 0, o, None, None, None),   # a token past the vocabulary

@@ -210,6 +210,22 @@ def test_numbers_that_are_none_stay_in_their_rows_and_columns(backend):
         assert torch.equal(got[same], want[same])
 
 
+@pytest.mark.parametrize("rows", [3, 64])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_infinities_and_the_largest_numbers(backend, rows, dtype):
+    # an infinity in a row is one in its results, of the weight's sign; the largest finite value of the type is no infinity
+    x, w, _, _ = inputs(rows, 96, 128, dtype)
+    x[1, 70] = float("inf")
+    x[2] = 0
+    x[2, 9] = torch.finfo(dtype).max
+    w[:, 9] = 0.25
+    got = backend.matmul_epilogue(x, w)
+    backend.sync()
+    assert torch.equal(got[1], torch.sign(w[:, 70].float()) * float("inf"))
+    assert torch.equal(got[2], torch.full_like(got[2], 0.25 * torch.finfo(dtype).max))
+    assert got[0].isfinite().all()
+
+
 @pytest.mark.parametrize("rows", [1, 24, 100])
 @pytest.mark.parametrize("dtype", TYPES)
 def test_recorded_and_replayed(backend, rows, dtype):
@@ -275,7 +291,7 @@ def test_refusals(backend):
             a[at[name]] = v
         return L.yx_matmul_epilogue(*a)
     for kw in (dict(x_dtype=3), dict(out_dtype=-1), dict(act=5), dict(act=-1), dict(x=None), dict(w=None), dict(out=None), dict(k=0),
-               dict(x=x.data_ptr() + 2), dict(w=w.data_ptr() + 1), dict(bias=b.data_ptr() + 2), dict(residual=r.data_ptr() + 2), dict(out=out.data_ptr() + 2),
+               dict(n=2 ** 31), dict(k=2 ** 31), dict(rows=2 ** 31), dict(x=x.data_ptr() + 2), dict(w=w.data_ptr() + 1), dict(bias=b.data_ptr() + 2), dict(residual=r.data_ptr() + 2), dict(out=out.data_ptr() + 2),
                dict(out=w.data_ptr()), dict(out=b.data_ptr()), dict(residual=out.data_ptr() + 256)):
         assert with_(**kw) == _lib.YX_ERR_INVALID and backend.status() == _lib.YX_ERR_INVALID, kw
         with pytest.raises(BackendError):

@@ -13,14 +13,23 @@ using namespace dev;
 
 // Given tokens on their way to the device: in kernel-parameter space, which is copied with the call, so that nothing on the
 // host has to outlive it and a recorded call keeps its own.
-constexpr uint32_t IDS_A_LAUNCH = 1000;
+// (Two sizes: a launch takes longer with 32 KB of parameters than with four, and three launches longer than that.)
+template <uint32_t N>
 struct Ids {
-    uint32_t v[IDS_A_LAUNCH];
+    uint32_t v[N];
 };
-__global__ void __launch_bounds__(256) put_ids_kernel(const __grid_constant__ Ids ids, uint32_t n, uint32_t *__restrict__ out) {
+template <uint32_t N>
+__global__ void __launch_bounds__(256) put_ids_kernel(const __grid_constant__ Ids<N> ids, uint32_t n, uint32_t *__restrict__ out) {
     dependent_entry();
     for (uint32_t i = threadIdx.x; i < n; i += blockDim.x) out[i] = ids.v[i];
 }
+template <uint32_t N>
+int put_ids_launch(yx_ctx *ctx, const uint32_t *host, uint32_t n, uint32_t *out) {
+    Ids<N> ids;
+    memcpy(ids.v, host, (size_t)n * 4);
+    return launch_dependent(ctx, "token id kernel launch", put_ids_kernel<N>, dim3(1), dim3(256), 0, ids, n, out);
+}
+constexpr uint32_t FEW_IDS = 1000, MANY_IDS = 8000;
 
 // A logit and its token as one whole number, larger for a larger logit and, between equal ones, for the smaller token.
 __device__ __forceinline__ uint64_t key_of(float l, uint32_t token) {
@@ -201,7 +210,7 @@ struct Tile {
     __device__ __forceinline__ void load_inside(const char *base, uint32_t first, uint32_t step) {
         const uint4 *p = (const uint4 *)base + first;
 #pragma unroll
-        for (int i = 0; i < VECS; i++) v[i] = __ldg(p + (size_t)i * step);
+        for (int i = 0; i < VECS; i++) v[i] = p[(size_t)i * step];
     }
     // The same of a row whose logit 0 is element `shift` of vector 0: what lies before the row, behind it, or at or behind
     // vector `end` counts as forbidden.
@@ -214,7 +223,7 @@ struct Tile {
             v[i] = make_uint4(none, none, none, none);
             if (vec >= end) continue;
             if (c >= shift && c + WIDE <= (uint64_t)shift + cols) {
-                v[i] = __ldg((const uint4 *)base + vec);
+                v[i] = *((const uint4 *)base + vec);
             } else {
                 uint32_t w[4] = {none, none, none, none};
 #pragma unroll
@@ -458,11 +467,10 @@ int put_ids(yx_ctx *ctx, const uint32_t *host, size_t n, const uint32_t **out) {
     if (int rc = grow(ctx, ctx->lp_ids, n * 4)) return rc;
     *out = (const uint32_t *)ctx->lp_ids.dev;
     ctx->last_launch = yx_ctx::LAST_OTHER;
-    Ids ids;
-    for (size_t i = 0; i < n; i += IDS_A_LAUNCH) {
-        const uint32_t m = (uint32_t)std::min<size_t>(IDS_A_LAUNCH, n - i);
-        memcpy(ids.v, host + i, (size_t)m * 4);
-        if (int rc = launch_dependent(ctx, "token id kernel launch", put_ids_kernel, dim3(1), dim3(256), 0, ids, m, (uint32_t *)ctx->lp_ids.dev + i)) return rc;
+    for (size_t i = 0; i < n; i += MANY_IDS) {
+        const uint32_t m = (uint32_t)std::min<size_t>(MANY_IDS, n - i);
+        uint32_t *to = (uint32_t *)ctx->lp_ids.dev + i;
+        if (int rc = m <= FEW_IDS ? put_ids_launch<FEW_IDS>(ctx, host + i, m, to) : put_ids_launch<MANY_IDS>(ctx, host + i, m, to)) return rc;
     }
     return YX_OK;
 }

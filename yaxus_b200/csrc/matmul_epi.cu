@@ -32,6 +32,7 @@ bool overlap(const void *a, size_t an, const void *b, size_t bn) {
     return a && b && (uintptr_t)a < (uintptr_t)b + bn && (uintptr_t)b < (uintptr_t)a + an;
 }
 
+constexpr uint32_t MOST = 0x7fffffffu;   // rows, columns, inner size: coordinates of copies are signed
 bool aligned(const void *p, size_t size) { return ((uintptr_t)p & (size - 1)) == 0; }
 
 struct Guard {
@@ -87,6 +88,7 @@ int yx_matmul_epilogue(yx_ctx *ctx, const void *x_dev, int x_dtype, const void *
     if (activation < YX_ACT_NONE || activation > YX_ACT_SILU) return fail(ctx, YX_ERR_INVALID, "matmul_epilogue: unknown activation");
     if (rows == 0 || n == 0) return YX_OK;
     if (!x_dev || !w_bf16_dev || !out_dev || k == 0) return fail(ctx, YX_ERR_INVALID, "matmul_epilogue: null tensor or empty inner dimension");
+    if (rows > MOST || n > MOST || k > MOST) return fail(ctx, YX_ERR_INVALID, "matmul_epilogue: a size of 2^31 or more");
     if (!aligned(x_dev, size_of(x_dtype)) || !aligned(w_bf16_dev, 2) || !aligned(bias_dev, 4) || !aligned(residual_dev, size_of(out_dtype)) ||
         !aligned(out_dev, size_of(out_dtype)))
         return fail(ctx, YX_ERR_INVALID, "matmul_epilogue: a tensor off its type's alignment");
@@ -120,6 +122,7 @@ int yx_matmul_logprobs(yx_ctx *ctx, const void *x_dev, int x_dtype, const void *
     if (rows == 0) return YX_OK;
     if (!x_dev || !w_bf16_dev || !ids_host || !logprob_dev || n == 0 || k == 0)
         return fail(ctx, YX_ERR_INVALID, "matmul_logprobs: null tensor, no columns or empty inner dimension");
+    if (rows > MOST || n > MOST || k > MOST) return fail(ctx, YX_ERR_INVALID, "matmul_logprobs: a size of 2^31 or more");
     if (!aligned(x_dev, size_of(x_dtype)) || !aligned(w_bf16_dev, 2) || !aligned(logprob_dev, 4) || !aligned(entropy_dev, 4))
         return fail(ctx, YX_ERR_INVALID, "matmul_logprobs: a tensor off its type's alignment");
     for (uint32_t r = 0; r < rows; r++)

@@ -514,6 +514,8 @@ __device__ __forceinline__ void pair_body(const CUtensorMap &w_map, const CUtens
         }
     } else if (warp < 8) {
         // ---- epilogue -------------------------------------------------------------------------
+        // (it reads what the kernels ahead wrote, residuals and given tokens, with loads of its own)
+        if constexpr (KIND >= EPILOGUE) asm volatile("griddepcontrol.wait;" ::: "memory");
         Walk walk(a, pair);
         Piece p;
         AccTurn turn;
