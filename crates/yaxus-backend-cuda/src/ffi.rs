@@ -22,6 +22,14 @@ pub const YX_F32: c_int = 0;
 pub const YX_F16: c_int = 1;
 pub const YX_BF16: c_int = 2;
 
+pub const YX_ACT_NONE: c_int = 0;
+pub const YX_ACT_RELU: c_int = 1;
+pub const YX_ACT_GELU: c_int = 2;
+pub const YX_ACT_GELU_TANH: c_int = 3;
+pub const YX_ACT_SILU: c_int = 4;
+
+pub const YX_TOP_MAX: usize = 32;
+
 pub const YX_STATIC_SPLITS: usize = 8;
 pub const YX_STATIC_MAX_ROW_HEADS: usize = 1024;
 

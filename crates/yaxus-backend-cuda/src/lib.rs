@@ -145,6 +145,139 @@ impl CudaBackend {
     }
 }
 
+/// What follows a product in `matmul_epilogue`.
+#[derive(Debug, Clone, Copy, PartialEq, Eq)]
+pub enum Activation {
+    None,
+    Relu,
+    Gelu,
+    GeluTanh,
+    Silu,
+}
+
+/// Log probabilities of rows of logits, in host memory.
+pub struct LogProbs {
+    /// Of each row's given token.
+    pub logprob: Vec<f32>,
+    pub entropy: Vec<f32>,
+    /// `top` tokens a row, the most probable first.
+    pub top_ids: Vec<u32>,
+    pub top_logprob: Vec<f32>,
+}
+
+/// Beside the trait: from hidden states to log probabilities.
+impl CudaBackend {
+    /// act(x . w^T + bias) + residual.
+    pub fn matmul_epilogue(&mut self, x: &Tensor, w: &Weight, bias: Option<&Weight>, act: Activation, residual: Option<&Tensor>) -> Tensor {
+        assert_eq!(x.cols, w.shape[1], "matmul inner dim");
+        let act = match act {
+            Activation::None => ffi::YX_ACT_NONE,
+            Activation::Relu => ffi::YX_ACT_RELU,
+            Activation::Gelu => ffi::YX_ACT_GELU,
+            Activation::GeluTanh => ffi::YX_ACT_GELU_TANH,
+            Activation::Silu => ffi::YX_ACT_SILU,
+        };
+        if let Some(b) = bias {
+            assert_eq!(b.shape, [w.shape[0]], "one bias for each column");
+        }
+        if let Some(r) = residual {
+            assert_eq!((r.rows, r.cols), (x.rows, w.shape[0]), "the residual has the result's shape");
+        }
+        let out = self.alloc(x.rows, w.shape[0]);
+        let ctx = self.ctx.lock().unwrap();
+        unsafe {
+            ffi::yx_matmul_epilogue(
+                ctx.0,
+                x.ptr,
+                ffi::YX_F32,
+                w.ptr,
+                bias.map_or(std::ptr::null(), |b| b.ptr as *const f32),
+                act,
+                residual.map_or(std::ptr::null(), |r| r.ptr as *const c_void),
+                x.rows as u32,
+                w.shape[0] as u32,
+                w.shape[1] as u32,
+                out.ptr,
+                ffi::YX_F32,
+            )
+        };
+        drop(ctx);
+        out
+    }
+
+    /// The log probability of one given token a row, the entropy and the `top` most probable tokens.  A read-back.
+    pub fn logprob_rows(&mut self, logits: &Tensor, ids: &[u32], top: usize) -> Result<LogProbs> {
+        assert_eq!(ids.len(), logits.rows, "one token for each row");
+        let (logprob, entropy) = (self.alloc(logits.rows, 1), self.alloc(logits.rows, 1));
+        let (top_ids, top_logprob) = (self.alloc(logits.rows, top), self.alloc(logits.rows, top));
+        let mut r = LogProbs {
+            logprob: vec![0.0; logits.rows],
+            entropy: vec![0.0; logits.rows],
+            top_ids: vec![0; logits.rows * top],
+            top_logprob: vec![0.0; logits.rows * top],
+        };
+        {
+            let ctx = self.ctx.lock().unwrap();
+            let some = |t: &Tensor| if top > 0 { t.ptr } else { std::ptr::null_mut() };
+            unsafe {
+                ffi::yx_logprob_rows(
+                    ctx.0,
+                    logits.ptr,
+                    ffi::YX_F32,
+                    logits.rows as u32,
+                    logits.cols as u32,
+                    logits.cols,
+                    ids.as_ptr(),
+                    1,
+                    top as u32,
+                    logprob.ptr as *mut f32,
+                    entropy.ptr as *mut f32,
+                    some(&top_ids) as *mut u32,
+                    some(&top_logprob) as *mut f32,
+                );
+                ffi::yx_download(ctx.0, r.logprob.as_mut_ptr() as *mut c_void, logprob.ptr, logits.rows * 4, 0);
+                ffi::yx_download(ctx.0, r.entropy.as_mut_ptr() as *mut c_void, entropy.ptr, logits.rows * 4, 0);
+                if top > 0 {
+                    ffi::yx_download(ctx.0, r.top_ids.as_mut_ptr() as *mut c_void, top_ids.ptr, logits.rows * top * 4, 0);
+                    ffi::yx_download(ctx.0, r.top_logprob.as_mut_ptr() as *mut c_void, top_logprob.ptr, logits.rows * top * 4, 0);
+                }
+            }
+        }
+        self.check()?;
+        Ok(r)
+    }
+
+    /// The log probability of one given token a row and the entropy under softmax(x . w^T), without the logits: scores of
+    /// prompts and drafts.  A read-back.
+    pub fn matmul_logprobs(&mut self, x: &Tensor, w: &Weight, ids: &[u32]) -> Result<(Vec<f32>, Vec<f32>)> {
+        assert_eq!(x.cols, w.shape[1], "matmul inner dim");
+        assert_eq!(ids.len(), x.rows, "one token for each row");
+        let (logprob, entropy) = (self.alloc(x.rows, 1), self.alloc(x.rows, 1));
+        let (mut p, mut h) = (vec![0f32; x.rows], vec![0f32; x.rows]);
+        {
+            let ctx = self.ctx.lock().unwrap();
+            unsafe {
+                ffi::yx_matmul_logprobs(
+                    ctx.0,
+                    x.ptr,
+                    ffi::YX_F32,
+                    w.ptr,
+                    x.rows as u32,
+                    w.shape[0] as u32,
+                    w.shape[1] as u32,
+                    ids.as_ptr(),
+                    logprob.ptr as *mut f32,
+                    entropy.ptr as *mut f32,
+                );
+                ffi::yx_download(ctx.0, p.as_mut_ptr() as *mut c_void, logprob.ptr, x.rows * 4, 0);
+                ffi::yx_download(ctx.0, h.as_mut_ptr() as *mut c_void, entropy.ptr, x.rows * 4, 0);
+            }
+        }
+        self.check()?;
+        Ok((p, h))
+    }
+}
+
 impl Backend for CudaBackend {
     type Tensor = Tensor;
     type Weight = Weight;
