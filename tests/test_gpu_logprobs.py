@@ -195,6 +195,63 @@ def test_many_given_tokens(backend, rows, n_ids):
     check(x, ids, 0, r)
 
 
+def test_offsets_past_32_bits(backend):
+    # the last rows of 8.6 GB of logits, and of a head's hidden states: both begin past 2^32 elements
+    rows, cols = 43000, 100003
+    x = torch.zeros(rows, cols, dtype=torch.bfloat16, device="cuda")
+    x[-3:] = logits_of(3, cols, torch.bfloat16)
+    ids = np.arange(rows) % cols
+    r = backend.logprob_rows(x, ids, top=4, entropy=True)
+    backend.sync()
+    check(x[-3:], ids[-3:], 4, type(r)(*(t[-3:] for t in r)))
+    assert torch.allclose(r.logprob[:5], torch.full((5,), -float(np.log(cols)), device="cuda"))
+    del x, r
+    rows, k = 270000, 16384
+    h = torch.zeros(rows, k, dtype=torch.bfloat16, device="cuda")
+    h[-40:].normal_()
+    w = (torch.randn(100, k, device="cuda") * k ** -0.5).bfloat16()
+    ids = np.arange(rows) % 100
+    p = backend.matmul_logprobs(h, w, ids)
+    backend.sync()
+    lp = torch.log_softmax(h[-40:].double() @ w.double().T, 1)
+    want = lp.gather(1, torch.as_tensor(ids[-40:], device="cuda")[:, None])[:, 0]
+    assert (p.logprob[-40:] - want).abs().max() <= 1e-4 and torch.allclose(p.logprob[:9], torch.full((9,), -float(np.log(100)), device="cuda"))
+
+
+def test_two_contexts_at_once(backend):
+    # each has a stream and scratch of its own: what one computes does not show in the other
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    backends = [CudaBackend(0, s) for s in streams]
+    work = []
+    for i, s in enumerate(streams):
+        with torch.cuda.stream(s):
+            w = (torch.randn(6000, 512, device="cuda") * 0.1).bfloat16()
+            work.append([(torch.randn(rows, 512, device="cuda").to(t), w, np.random.default_rng(rows).integers(0, 6000, rows))
+                         for rows in (1, 30, 70, 300) for t in TYPES])
+    torch.cuda.synchronize()
+    alone = []
+    for b, s, jobs in zip(backends, streams, work):
+        with torch.cuda.stream(s):
+            alone.append([(b.matmul_logprobs(*j), b.logprob_rows(b.matmul_epilogue(*j[:2]), j[2], top=7)) for j in jobs])
+            b.sync()
+    together = [[], []]
+    for turn in range(3):
+        for n in range(len(work[0])):
+            for i in range(2):
+                with torch.cuda.stream(streams[i]):
+                    j = work[i][n]
+                    together[i].append((backends[i].matmul_logprobs(*j), backends[i].logprob_rows(backends[i].matmul_epilogue(*j[:2]), j[2], top=7)))
+    for b in backends:
+        b.sync()
+    for i in range(2):
+        for n, (p, r) in enumerate(together[i]):
+            q, t = alone[i][n % len(work[0])]
+            assert torch.equal(p.logprob, q.logprob) and torch.equal(p.entropy, q.entropy)
+            assert torch.equal(r.logprob, t.logprob) and torch.equal(r.top_ids, t.top_ids) and torch.equal(r.top_logprob, t.top_logprob)
+    for b in backends:
+        b.close()
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 def test_rows_off_any_alignment(backend, dtype):
     # a first row that starts one element past an aligned address, rows an odd number of elements apart

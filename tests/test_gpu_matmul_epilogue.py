@@ -195,6 +195,16 @@ def test_more_rows_than_a_grid_s_extent(backend):
     check(got, x, w, b, r, "relu")
 
 
+def test_results_past_32_bits(backend):
+    x = torch.zeros(70000, 64, device="cuda").bfloat16()
+    x[-50:].normal_()
+    w = (torch.randn(65536, 64, device="cuda") * 0.125).bfloat16()
+    got = backend.matmul_epilogue(x, w, activation="relu", out_dtype=torch.bfloat16)     # 4.6e9 results
+    backend.sync()
+    check(got[-50:], x[-50:], w, None, None, "relu")
+    assert (got[:100] == 0).all()
+
+
 def test_numbers_that_are_none_stay_in_their_rows_and_columns(backend):
     for rows in (6, 64):
         x, w, b, r = inputs(rows, 160, 192, torch.float32)
