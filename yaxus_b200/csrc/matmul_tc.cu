@@ -1,5 +1,6 @@
 // out [T, N] f32 = x [T, K] f32 . w [N, K]^T (bf16) for passes of many rows, on the fifth-generation
 // tensor cores, and the same with silu(gate) * up taken in the epilogue (crates/yaxus-model/src/lib.rs:128,164-168).
+// Two more kinds of the kernels take their rows exactly and end in something else (yx_matmul_epilogue, yx_matmul_logprobs): see Kind.
 //
 // Activations keep 16 bits of mantissa: x = hi + lo, two bf16 matrices, and every weight tile that reaches
 // shared memory is multiplied by both, into one f32 accumulator in tensor memory.  The arithmetic is twice
@@ -18,9 +19,9 @@
 // is a chain of L2 latencies: with one warp to a lane quarter and one share at a time it took 15 to 20 us.
 //
 // Large passes are bound by the tensor cores: 2048 rows on 4096 -> 28672 (gate and up) take 608 us, 1.58 PFLOP/s
-// of bf16 products; 80 rows by the weights' way through L2 and shared memory: 412 MB in 100 us.  Against two
+// of bf16 products; 80 rows by the weights' way into shared memory: 235 MB in 64 us.  Against two
 // library products (high part, then low part added to it) and a SwiGLU kernel, whole steps of one layer went from
-// 2151 to 1700 us (2048 rows) and from 1244 to 399 us (80 rows).
+// 2151 to 1509 us (2048 rows) and from 1244 to 358 us (80 rows).
 //
 // Warps 0-7 epilogue (two to each 32 lanes of tensor memory, taking turns at 32 pass rows), warp 8 TMA, warp 9
 // issues the MMAs (first CTA of the pair).  All waits are bounded; on expiry the CTA records where, stops waiting
@@ -835,10 +836,10 @@ __global__ void __launch_bounds__(256) cut_rows_kernel(const void *__restrict__ 
 // The kernel starts under the one ahead of it and asks its first stages into L2 before it waits: weights are not
 // written by the kernel ahead, and even if they were, L2 is where such writes land.
 //
-// Bound by HBM from some 200 MB on (one row on 28672 x 4096: 45 us, the part above a launch's fixed 8 to 12 us at
+// Bound by HBM from some 200 MB on (one row on 28672 x 4096: 40 us, the part above a launch's fixed 6 to 8 us at
 // 7.2 TB/s), by a chain of latencies below.  The kernel with weights straight from global memory into mma.sync
 // fragments, a packing kernel before it and a finishing kernel behind took 58 us for sixteen rows of that weight;
-// steps went from 419 to 360 us (one row, large), 538 to 424 us (sixteen rows), 417 to 340 us (one row, small).
+// steps went from 419 to 340 us (one row, large), 538 to 406 us (sixteen rows), 417 to 298 us (one row, small).
 constexpr int ROWS_THREADS = 14 * 32;
 constexpr int ROWS_CONVERT_WARP = 6, ROWS_CONVERTERS = 8;
 constexpr uint32_t ROWS_M = 128;
@@ -1396,6 +1397,7 @@ int plan_pairs(yx_ctx *ctx, const Product &p, PairArgs &a) {
     a.t_tiles = KIND < EPILOGUE ? (p.T + TC_MAX_BT - 1) / TC_MAX_BT : p.t_tiles;
     a.bt = rows_of_tiles(p.T, a.t_tiles);
     a.ksteps = (p.K + TC_KSTEP - 1) / TC_KSTEP;
+    a.stages = std::min<uint32_t>(TC_MAX_STAGES, (smem_budget(KIND) - 1024) / (W_BYTES + a.parts * a.bt * 64u));
     const uint32_t tiles = ((p.N + TC_M - 1) / TC_M) * a.t_tiles;
     a.pairs = (uint32_t)pairs;
     a.rounds = tiles / a.pairs;
@@ -1405,11 +1407,11 @@ int plan_pairs(yx_ctx *ctx, const Product &p, PairArgs &a) {
         // sums meet in shared memory.  Through scratch and through clusters, us: 80 rows bf16 x [4096, 4096] 17.9 and 13.3, 256 rows
         // 30 and 20, 128 x [2048, 2048] 18.4 and 8.7, 512 f32 x [1024, 2816] 39 and 23; even where clusters leave half of the pairs
         // without work, as 80 x [1024, 14336] does, 24.7 and 18.8.
-        if (a.rounds == 0)
+        // (the sums take 512 bytes a pass row of the ring, which has room for that as long as it fills shared memory)
+        if (a.rounds == 0 && a.stages * (W_BYTES + a.parts * a.bt * 64u) >= a.bt * 512u)
             if (int rc = cluster_for<KIND, CHUNKS>(ctx, tiles, a.ksteps, &a.cluster)) return rc;
     }
     if (a.cluster == 1 && a.rest_units > 0) a.rest_pairs = share_rest(tiles - a.rounds * a.pairs, a.ksteps, a.pairs, a.bt, a.rounds > 0, 0.001f * (float)a.parts);
-    a.stages = std::min<uint32_t>(TC_MAX_STAGES, (smem_budget(KIND) - 1024) / (W_BYTES + a.parts * a.bt * 64u));
     a.bufs = a.bt <= 128 ? 4 : a.bt <= 160 ? 3 : 2;
     a.buf_columns = 512 / a.bufs / 32 * 32;
     if (KIND < EPILOGUE) {
