@@ -393,6 +393,10 @@ def test_refusals(backend):
         lambda: L.yx_logprob_rows(c, p, 0, 2, 50, 50, None, 0, 33, None, None, o, o + 400),  # more than YX_TOP_MAX
         lambda: L.yx_logprob_rows(c, p, 0, 2, 20, 50, None, 0, 21, None, None, o, o + 400),  # more than there are
         lambda: L.yx_logprob_rows(c, p, 0, 2, 50, 50, None, 0, 5, None, None, o, None),
+        lambda: L.yx_logprob_rows(c, p, 0, 2, 50, 50, i, 1, 0, p + 396, None, None, None),  # results over the logits
+        lambda: L.yx_logprob_rows(c, p, 0, 2, 50, 50, None, 0, 4, None, p + 400, o, p - 16),
+        lambda: L.yx_matmul_logprobs(c, h.data_ptr(), 0, w.data_ptr(), 2, 50, 64, i, h.data_ptr() + 8, None),
+        lambda: L.yx_matmul_logprobs(c, h.data_ptr(), 0, w.data_ptr(), 2, 50, 64, i, o, w.data_ptr()),
         lambda: L.yx_matmul_logprobs(c, h.data_ptr(), 9, w.data_ptr(), 2, 50, 64, i, o, None),
         lambda: L.yx_matmul_logprobs(c, h.data_ptr(), 0, None, 2, 50, 64, i, o, None),
         lambda: L.yx_matmul_logprobs(c, h.data_ptr(), 0, w.data_ptr(), 2, 0, 64, i, o, None),

@@ -332,31 +332,41 @@ class CudaBackend:
         """act(x [T, K] . w [N, K]^T + bias) + residual, for x and result f32 or 16-bit and w a bf16 matrix.  `activation`:
         "relu", "gelu", "gelu_tanh", "silu" or None.  `out` may be the residual.  The result's type is `out`'s, else
         `out_dtype`, else the residual's, else f32."""
-        assert activation in _lib.ACTIVATIONS, "unknown activation"
+        act = _lib.ACTIVATIONS.get(activation)
+        assert act is not None, "unknown activation"
         self._check_product(x, w)
-        shape = (x.shape[0], w.shape[0])
+        rows, (n, k) = x.shape[0], w.shape
         if out is None:
-            out = x.new_empty(shape, dtype=out_dtype or (torch.float32 if residual is None else residual.dtype))
-        assert self._here(out) and out.shape == shape and out.dtype in _YX_DTYPE and out.is_contiguous()
-        assert bias is None or (self._here(bias) and bias.dtype == torch.float32 and bias.shape == shape[1:] and bias.is_contiguous())
-        assert residual is None or (self._here(residual) and residual.dtype == out.dtype and residual.shape == shape and residual.is_contiguous())
-        self._L.yx_matmul_epilogue(self._ctx, _ptr(x), _YX_DTYPE[x.dtype], _ptr(w), _ptr(bias), _lib.ACTIVATIONS[activation],
-                                   _ptr(residual), x.shape[0], w.shape[0], w.shape[1], _ptr(out), _YX_DTYPE[out.dtype])
+            dtype = out_dtype or (torch.float32 if residual is None else residual.dtype)
+            assert dtype in _YX_DTYPE
+            out = x.new_empty(rows, n, dtype=dtype)
+        else:
+            assert self._here(out) and out.shape == (rows, n) and out.dtype in _YX_DTYPE and out.is_contiguous()
+        if bias is not None:
+            assert self._here(bias) and bias.dtype == torch.float32 and bias.shape == (n,) and bias.is_contiguous()
+        if residual is not None:
+            assert self._here(residual) and residual.dtype == out.dtype and residual.shape == (rows, n) and residual.is_contiguous()
+        self._L.yx_matmul_epilogue(self._ctx, x.data_ptr(), _YX_DTYPE[x.dtype], w.data_ptr(), _ptr(bias), act, _ptr(residual), rows, n, k,
+                                   out.data_ptr(), _YX_DTYPE[out.dtype])
         return out
 
     def logprob_rows(self, logits: torch.Tensor, ids=None, top: int = 0, entropy: bool = False) -> LogProbs:
         """Log probabilities under the softmax of each row of `logits` (f32 or 16-bit; rows may lie further apart than they
         are long): of the given tokens `ids` ([rows] or [rows, n], on the host), the entropy, the `top` most probable."""
-        assert self._here(logits) and logits.dim() == 2 and logits.dtype in _YX_DTYPE and (logits.shape[1] <= 1 or logits.stride(1) == 1)
-        rows, cols = logits.shape
-        stride = logits.stride(0) if rows > 1 else cols
-        idx = None if ids is None else _token_ids(ids)
-        assert idx is None or (idx.ndim in (1, 2) and idx.shape[0] == rows), "one row of ids for each row of logits"
-        n_ids = 0 if idx is None else idx.size // max(rows, 1)
-        new, f32 = logits.new_empty, torch.float32   # (a quarter cheaper than torch.empty: four of them cost what the launch does)
-        r = LogProbs(new(idx.shape, dtype=f32) if n_ids else None, new(rows, dtype=f32) if entropy else None,
-                     new((rows, top), dtype=torch.int32) if top else None, new((rows, top), dtype=f32) if top else None)
-        self._L.yx_logprob_rows(self._ctx, _ptr(logits), _YX_DTYPE[logits.dtype], rows, cols, stride, _u32p(idx) if n_ids else None, n_ids,
+        dtype = _YX_DTYPE.get(logits.dtype)
+        assert dtype is not None and self._here(logits) and logits.dim() == 2
+        (rows, cols), (stride, step) = logits.shape, logits.stride()
+        assert step == 1 or cols <= 1
+        idx, n_ids = None, 0
+        if ids is not None:
+            idx = _token_ids(ids)
+            assert idx.ndim in (1, 2) and idx.shape[0] == rows, "one row of ids for each row of logits"
+            n_ids = idx.size // max(rows, 1)
+        # (allocations are half of a call's time on the host; sizes as plain arguments and no type where it is the logits' are quickest)
+        new = logits.new_empty if dtype == F32 else lambda *shape: logits.new_empty(*shape, dtype=torch.float32)   # noqa: E731
+        r = LogProbs(new(*idx.shape) if n_ids else None, new(rows) if entropy else None,
+                     logits.new_empty(rows, top, dtype=torch.int32) if top else None, new(rows, top) if top else None)
+        self._L.yx_logprob_rows(self._ctx, logits.data_ptr(), dtype, rows, cols, stride if rows > 1 else cols, _u32p(idx) if n_ids else None, n_ids,
                                 top, _ptr(r.logprob), _ptr(r.entropy), _ptr(r.top_ids), _ptr(r.top_logprob))
         return r
 
@@ -365,9 +375,10 @@ class CudaBackend:
         self._check_product(x, w)
         idx = _token_ids(ids)
         assert idx.shape == (x.shape[0],), "one id for each row"
-        r = LogProbs(x.new_empty(x.shape[0], dtype=torch.float32), x.new_empty(x.shape[0], dtype=torch.float32) if entropy else None)
-        self._L.yx_matmul_logprobs(self._ctx, _ptr(x), _YX_DTYPE[x.dtype], _ptr(w), x.shape[0], w.shape[0], w.shape[1], _u32p(idx),
-                                   _ptr(r.logprob), _ptr(r.entropy))
+        rows, (n, k), f32 = x.shape[0], w.shape, torch.float32
+        r = LogProbs(x.new_empty(rows, dtype=f32), x.new_empty(rows, dtype=f32) if entropy else None)
+        self._L.yx_matmul_logprobs(self._ctx, x.data_ptr(), _YX_DTYPE[x.dtype], w.data_ptr(), rows, n, k, _u32p(idx), r.logprob.data_ptr(),
+                                   _ptr(r.entropy))
         return r
 
     def attention(self, qkv: torch.Tensor, q_norm: torch.Tensor, k_norm: torch.Tensor, kv: Kv, hq: int, eps: float,

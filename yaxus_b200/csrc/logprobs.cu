@@ -65,7 +65,7 @@ constexpr int THREADS = 256, WARPS = THREADS / 32;
 constexpr int PER_THREAD = 16;                              // logits of a tile
 constexpr int TILE = THREADS * PER_THREAD;
 constexpr uint32_t MAX_PARTS = 128;                         // of a row
-constexpr uint32_t MAX_SHARED = 2048;                        // parts of all rows that have more than one
+constexpr uint32_t MAX_SHARED = 2048;                       // parts of all rows that have more than one
 constexpr uint32_t LIST = 512;                              // tokens put in order by counting
 constexpr uint32_t IDS_PARAM = 512;                         // given tokens that ride in kernel-parameter space
 static_assert(MAX_PARTS * YX_TOP_MAX <= TILE, "the last CTA holds the parts' best tokens as one tile");
@@ -543,6 +543,13 @@ extern "C" int yx_logprob_rows(yx_ctx *ctx, const void *logits_dev, int dtype, u
     if ((n_ids > 0) != (logprob_dev != nullptr) || (n_ids > 0 && !ids_host)) return fail(ctx, YX_ERR_INVALID, "logprob_rows: given tokens and their result go together");
     if ((n_top > 0) != (top_ids_dev != nullptr) || (n_top > 0) != (top_logprob_dev != nullptr))
         return fail(ctx, YX_ERR_INVALID, "logprob_rows: alternatives and their results go together");
+    // Rows are read while others' results are written.
+    const size_t read = (((size_t)rows - 1) * stride + cols) * (dtype == YX_F32 ? 4 : 2);
+    auto over = [&](const void *p, size_t each) {
+        return p && (uintptr_t)p < (uintptr_t)logits_dev + read && (uintptr_t)logits_dev < (uintptr_t)p + (size_t)rows * each * 4;
+    };
+    if (over(logprob_dev, n_ids) || over(entropy_dev, 1) || over(top_ids_dev, n_top) || over(top_logprob_dev, n_top))
+        return fail(ctx, YX_ERR_INVALID, "logprob_rows: a result lies over the logits");
     for (size_t i = 0; i < (size_t)rows * n_ids; i++)
         if (ids_host[i] >= cols) return fail(ctx, YX_ERR_INVALID, "logprob_rows: a token id is outside the vocabulary");
     if (n_ids == 0 && n_top == 0 && !entropy_dev) return YX_OK;

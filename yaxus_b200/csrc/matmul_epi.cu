@@ -125,6 +125,10 @@ int yx_matmul_logprobs(yx_ctx *ctx, const void *x_dev, int x_dtype, const void *
     if (rows > MOST || n > MOST || k > MOST) return fail(ctx, YX_ERR_INVALID, "matmul_logprobs: a size of 2^31 or more");
     if (!aligned(x_dev, size_of(x_dtype)) || !aligned(w_bf16_dev, 2) || !aligned(logprob_dev, 4) || !aligned(entropy_dev, 4))
         return fail(ctx, YX_ERR_INVALID, "matmul_logprobs: a tensor off its type's alignment");
+    const size_t x_bytes = (size_t)rows * k * size_of(x_dtype), w_bytes = (size_t)n * k * 2, results = (size_t)rows * 4;
+    if (overlap(logprob_dev, results, x_dev, x_bytes) || overlap(logprob_dev, results, w_bf16_dev, w_bytes) || overlap(entropy_dev, results, x_dev, x_bytes) ||
+        overlap(entropy_dev, results, w_bf16_dev, w_bytes))
+        return fail(ctx, YX_ERR_INVALID, "matmul_logprobs: a result lies over the rows or the weight");
     for (uint32_t r = 0; r < rows; r++)
         if (ids_host[r] >= n) return fail(ctx, YX_ERR_INVALID, "matmul_logprobs: a token id is outside the vocabulary");
     Guard guard(ctx->device);
