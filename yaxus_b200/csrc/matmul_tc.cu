@@ -64,9 +64,10 @@ constexpr int TC_MAX_BUFS = 4;
 // The same for rows taken exactly (EPILOGUE, LOGPROBS), by their parts: what keeps the result well within a millionth (2-norm
 // of the error over the result's, 2048 x [14336, 4096]: one part in chains of 8, 12 and 16 steps 4.7, 7.1 and 9.9e-7 and 235, 225 and
 // 216 us, two of 4, 6 and 8 4.7, 7.2 and 10.1e-7 and 369, 356 and 348 us, three of 2, 3 and 4 3.4, 5.5 and 7.7e-7 and 547, 514 and 505 us; a library's
-// f32 products 6 to 12e-7, yx_matmul 27e-7).  Results of 16 bits keep none of it.
+// f32 products 6 to 12e-7, yx_matmul 27e-7).  Results of 16 bits keep none of it and take chains that lose some 4e-6, a whole tile's
+// where K is 4096 (2048 bf16 rows x [14336, 4096] 180 us, with chains of 32 195).
 constexpr uint32_t MAX_CLUSTER = 4;         // pairs of a cluster (eight CTAs: the most that any chip of this kind places)
-constexpr uint32_t EXACT_CHAIN[3] = {12, 6, 4}, NARROW_CHAIN = 32;
+constexpr uint32_t EXACT_CHAIN[3] = {12, 6, 4}, NARROW_CHAIN[3] = {64, 48, 32};
 constexpr uint32_t GLU_GROUP = 16;          // gate and up rows alternate in a tile sixteen by sixteen: a warp holds both
 
 // What becomes of a product.
@@ -1432,7 +1433,7 @@ int plan_pairs(yx_ctx *ctx, const Product &p, PairArgs &a) {
         a.chain = large ? TC_CHAIN : std::min(a.rounds > 0 ? TC_SHORT_CHAIN : TC_CUT_CHAIN, std::max(TC_LEAST_CHAIN, a.ksteps / 2));
         a.long_first = large && a.bufs == 2;
     } else {
-        a.chain = KIND == EPILOGUE && p.e.out_dtype != YX_F32 ? NARROW_CHAIN : EXACT_CHAIN[a.parts - 1];
+        a.chain = KIND == EPILOGUE && p.e.out_dtype != YX_F32 ? NARROW_CHAIN[a.parts - 1] : EXACT_CHAIN[a.parts - 1];
     }
     a.status = ctx->dev_status;
     return YX_OK;
