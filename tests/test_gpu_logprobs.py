@@ -306,6 +306,26 @@ def test_head(backend, rows, n, k, dtype):
     assert only.entropy is None and torch.equal(only.logprob, r.logprob)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,n,k", [(1, 4096, 14336), (16, 4096, 14336), (32, 4096, 14336), (25, 50257, 2048), (64, 4096, 14336), (200, 900, 14336)])
+def test_head_again_and_again(backend, dtype, rows, n, k):
+    # many turns of the operands' ring: a slot filled too early or too late shows in one call of several, and in no two alike
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(rows)
+    for _ in range(4):
+        w = (torch.randn(n, k, generator=gen, device="cuda") * 2 * k ** -0.5).bfloat16()
+        x = torch.randn(rows, k, generator=gen, device="cuda").to(dtype)
+        ids = np.arange(rows) * 7 % n
+        lp = torch.log_softmax(x.double() @ w.double().T, 1).gather(1, torch.as_tensor(ids, device="cuda")[:, None])[:, 0]
+        first = backend.matmul_logprobs(x, w, ids)
+        for _ in range(12):
+            got = backend.matmul_logprobs(x, w, ids)
+            backend.sync()
+            assert torch.equal(got.logprob, first.logprob) and torch.equal(got.entropy, first.entropy)
+        # (the bound of test_head, on all rows together)
+        assert (first.logprob - lp).norm() <= 2e-6 * lp.norm() + 1e-7 * rows ** 0.5
+
+
 def test_head_of_no_numbers(backend):
     # a row of hidden states that is no number has no logits left; its neighbours are as they were
     for rows in (3, 40):

@@ -96,6 +96,22 @@ def test_rows_are_taken_exactly(backend, dtype, rows, n, k):
     assert (got - want).norm() <= 1e-6 * want.norm()
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,n,k", [(1, 4096, 14336), (8, 4096, 14336), (13, 1001, 14336), (16, 20000, 4096), (20, 4096, 14336), (32, 4096, 14336),
+                                      (32, 32000, 2048), (40, 4096, 14336), (150, 700, 14336), (300, 2000, 8200)])
+def test_long_sums_again_and_again(backend, dtype, rows, n, k):
+    # many turns of the operands' ring: a slot filled too early or too late shows in one call of several, and in no two alike
+    for seed in range(4):
+        x, w, _, _ = inputs(rows, n, k, dtype, bias=False, residual=False, seed=seed)
+        want = x.double() @ w.double().T
+        first = backend.matmul_epilogue(x, w)
+        for _ in range(12):
+            got = backend.matmul_epilogue(x, w)
+            backend.sync()
+            assert torch.equal(got, first)
+        assert (first - want).norm() <= 1e-6 * want.norm()
+
+
 @pytest.mark.parametrize("rows", [4, 50])
 def test_every_bit_of_a_row_counts(backend, rows):
     # one nonzero in each row and column: the results are the rows' own values, bit for bit (normal numbers whose least bit

@@ -64,8 +64,8 @@ constexpr int TC_MAX_BUFS = 4;
 // The same for rows taken exactly (EPILOGUE, LOGPROBS), by their parts: what keeps the result well within a millionth (2-norm
 // of the error over the result's, 2048 x [14336, 4096]: one part in chains of 8, 12 and 16 steps 4.7, 7.1 and 9.9e-7 and 235, 225 and
 // 216 us, two of 4, 6 and 8 4.7, 7.2 and 10.1e-7 and 369, 356 and 348 us, three of 2, 3 and 4 3.4, 5.5 and 7.7e-7 and 547, 514 and 505 us; a library's
-// f32 products 6 to 12e-7, yx_matmul 27e-7).  Results of 16 bits keep none of it and take chains that lose some 4e-6, a whole tile's
-// where K is 4096 (2048 bf16 rows x [14336, 4096] 180 us, with chains of 32 195).
+// f32 products 6 to 12e-7, yx_matmul 27e-7).  Results of 16 bits keep none of it and take chains that lose 4 to 7e-6
+// (64 steps are a whole tile's where K is 4096: 2048 bf16 rows x [14336, 4096] 180 us, with chains of 32 steps 195).
 constexpr uint32_t MAX_CLUSTER = 4;         // pairs of a cluster (eight CTAs: the most that any chip of this kind places)
 constexpr uint32_t EXACT_CHAIN[3] = {12, 6, 4}, NARROW_CHAIN[3] = {64, 48, 32};
 constexpr uint32_t GLU_GROUP = 16;          // gate and up rows alternate in a tile sixteen by sixteen: a warp holds both
@@ -854,7 +854,7 @@ constexpr uint32_t ROWS_CHAIN = 8, ROWS_BUFS = 4;   // (and four accumulators: t
 
 struct RowsArgs {
     const void *x;
-    uint32_t T, K, cols, ksteps, units, ctas, stages;
+    uint32_t T, K, cols, ksteps, units, ctas;
     uint32_t cluster;                 // CTAs that share a tile as one cluster (EPILOGUE, LOGPROBS; 1: none)
     bool whole;                       // every CTA takes whole tiles (EPILOGUE, LOGPROBS)
     uint32_t x_vec16;
@@ -897,6 +897,17 @@ constexpr uint32_t rows_pitch(int tp, int parts) {
     while (c < rows_columns(tp, parts)) c *= 2;
     return c;
 }
+// Stages of the ring, and the warps that fill its activations in turn.  A barrier's parity tells a phase from the one before,
+// not from the one two before: a warp that waits for a slot's last use to be over has to know that the use before that is, and
+// knows so from its own step before, whose slot was free, as long as the warps are no more than the stages.
+constexpr uint32_t rows_stage_bytes(int tp, int parts) { return W_BYTES + rows_columns(tp, parts) * 128; }
+constexpr uint32_t rows_stages(int tp, int kind, int parts) {
+    const uint32_t n = (kind < EPILOGUE ? TC_SMEM_BUDGET : 210 * 1024) / rows_stage_bytes(tp, parts);
+    return n < TC_MAX_STAGES ? n : TC_MAX_STAGES;
+}
+constexpr uint32_t rows_converters(int tp, int kind, int parts) {
+    return rows_stages(tp, kind, parts) < ROWS_CONVERTERS ? rows_stages(tp, kind, parts) : ROWS_CONVERTERS;
+}
 
 template <int TP, int KIND, int PARTS>
 __global__ void __launch_bounds__(ROWS_THREADS, 1)
@@ -907,14 +918,16 @@ matmul_rows_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_const
     __shared__ int abort_flag;
     __shared__ int last_s;
     constexpr bool GLU_TILES = KIND == GLU;
-    constexpr uint32_t NB = rows_columns(TP, PARTS), PITCH = rows_pitch(TP, PARTS), X_BYTES = NB * 128, STAGE = W_BYTES + X_BYTES;
+    constexpr uint32_t NB = rows_columns(TP, PARTS), PITCH = rows_pitch(TP, PARTS), STAGE = rows_stage_bytes(TP, PARTS);
+    constexpr uint32_t S = rows_stages(TP, KIND, PARTS), CONVERTERS = rows_converters(TP, KIND, PARTS);
+    static_assert(CONVERTERS <= S, "a step's slot has to be free one use after the warp's step before");
     constexpr uint32_t TMEM = ROWS_BUFS * PITCH;
     constexpr int SCRATCH = KIND == EPILOGUE ? TP * 32 : KIND == LOGPROBS ? STATS_SCRATCH : 1;   // floats a warp
     __shared__ __align__(16) float scratch_s[4 * SCRATCH];
     float *scratch = scratch_s + ((threadIdx.x >> 5) & 3) * SCRATCH;
     __shared__ float4 stats_s[4][KIND == LOGPROBS ? 32 : 1];
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-    const uint32_t S = a.stages, base = smem_u32(smem);
+    const uint32_t base = smem_u32(smem);
     const uint32_t b_full = smem_u32(bar_store), b_empty = b_full + 8 * TC_MAX_STAGES;
     const uint32_t b_acc_full = b_empty + 8 * TC_MAX_STAGES, b_acc_empty = b_acc_full + 8 * ROWS_BUFS;
     volatile int *abortp = &abort_flag;
@@ -1042,7 +1055,8 @@ matmul_rows_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_const
         }
     } else if (warp >= ROWS_CONVERT_WARP) {
         // ---- activations: every eighth step is this warp's ------------------------------------------
-        for (uint32_t u = u0 + (uint32_t)(warp - ROWS_CONVERT_WARP); u < u1; u += ROWS_CONVERTERS) {
+        // (of a ring of seven stages every seventh; the eighth warp has none)
+        for (uint32_t u = warp - ROWS_CONVERT_WARP < (int)CONVERTERS ? u0 + (uint32_t)(warp - ROWS_CONVERT_WARP) : u1; u < u1; u += CONVERTERS) {
             const uint32_t it = u - u0, s = it % S, use = it / S;
             const uint32_t k = (u % a.ksteps) * TC_KSTEP + (lane & 7) * 8;
             constexpr int R = TP / 4;          // 16-byte operand chunks (eight k of a pass row) a lane
@@ -1533,8 +1547,7 @@ int exact_pair_rows(yx_ctx *ctx, const Product &p) {
 
 template <int TP, int KIND, int PARTS>
 int matmul_few_rows(yx_ctx *ctx, const Product &p) {
-    constexpr uint32_t stage_bytes = W_BYTES + rows_columns(TP, PARTS) * 128;
-    constexpr uint32_t stages = std::min<uint32_t>(TC_MAX_STAGES, (KIND < EPILOGUE ? TC_SMEM_BUDGET : 210 * 1024) / stage_bytes);
+    constexpr uint32_t stage_bytes = rows_stage_bytes(TP, PARTS), stages = rows_stages(TP, KIND, PARTS);
     auto *kernel = matmul_rows_kernel<TP, KIND, PARTS>;
     bool &configured = ctx->mm_rows_configured[KIND][PARTS - 1][TP / 16];
     if (!configured) {
@@ -1582,7 +1595,6 @@ int matmul_few_rows(yx_ctx *ctx, const Product &p) {
             a.ctas = std::min(a.ctas, tiles);
         }
     }
-    a.stages = stages;
     a.x_vec16 = ((uintptr_t)a.x & 15u) == 0;
     a.out = (float *)p.out;
     a.e = p.e;
