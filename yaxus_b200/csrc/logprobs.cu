@@ -18,16 +18,18 @@ template <uint32_t N>
 struct Ids {
     uint32_t v[N];
 };
+constexpr uint32_t IDS_CTA = 256;   // (an SM reads parameters one thread's after another: 8000 tokens by one CTA took 10 us)
 template <uint32_t N>
-__global__ void __launch_bounds__(256) put_ids_kernel(const __grid_constant__ Ids<N> ids, uint32_t n, uint32_t *__restrict__ out) {
+__global__ void __launch_bounds__(IDS_CTA) put_ids_kernel(const __grid_constant__ Ids<N> ids, uint32_t n, uint32_t *__restrict__ out) {
     dependent_entry();
-    for (uint32_t i = threadIdx.x; i < n; i += blockDim.x) out[i] = ids.v[i];
+    const uint32_t i = blockIdx.x * IDS_CTA + threadIdx.x;
+    if (i < n) out[i] = ids.v[i];
 }
 template <uint32_t N>
 int put_ids_launch(yx_ctx *ctx, const uint32_t *host, uint32_t n, uint32_t *out) {
     Ids<N> ids;
     memcpy(ids.v, host, (size_t)n * 4);
-    return launch_dependent(ctx, "token id kernel launch", put_ids_kernel<N>, dim3(1), dim3(256), 0, ids, n, out);
+    return launch_dependent(ctx, "token id kernel launch", put_ids_kernel<N>, dim3((n + IDS_CTA - 1) / IDS_CTA), dim3(IDS_CTA), 0, ids, n, out);
 }
 constexpr uint32_t FEW_IDS = 1000, MANY_IDS = 8000;
 
