@@ -307,6 +307,30 @@ def test_head(backend, rows, n, k, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,n", [(1, 9480), (32, 11264), (7, 9601), (32, 18941), (20, 25600)])
+def test_head_of_tiles_of_other_heights(backend, dtype, rows, n):
+    # given tokens of every place in a tile, those at its ends among them
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(n)
+    w = (torch.randn(n, 64, generator=gen, device="cuda") / 4).bfloat16()
+    x = torch.randn(rows, 64, generator=gen, device="cuda").to(dtype)
+    logits = x.double() @ w.double().T
+    lp = torch.log_softmax(logits, 1)
+    h = torch.special.entr(lp.exp()).sum(1)
+    lp_tol, h_tol = tolerances(n, lp, h)
+    # (the move of test_head; 64 products of three parts at most are 192 additions)
+    move = 192 * 2.0 ** -23 * (x.double().abs() @ w.double().abs().T).amax(1)
+    spread = logits.amax(1) - logits.amin(1)
+    for first in range(0, 600, rows):
+        ids = np.arange(first, first + rows) * (1 if first < 300 else 17) % n
+        r = backend.matmul_logprobs(x, w, ids)
+        backend.sync()
+        at = torch.as_tensor(ids, device="cuda")[:, None]
+        assert ((r.logprob - lp.gather(1, at)[:, 0]).abs() <= 2 * move + lp_tol.gather(1, at)[:, 0]).all()
+        assert ((r.entropy - h).abs() <= 2 * move * (1 + spread) + h_tol).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("rows,n,k", [(1, 4096, 14336), (16, 4096, 14336), (32, 4096, 14336), (25, 50257, 2048), (64, 4096, 14336), (200, 900, 14336)])
 def test_head_again_and_again(backend, dtype, rows, n, k):
     # many turns of the operands' ring: a slot filled too early or too late shows in one call of several, and in no two alike

@@ -112,6 +112,16 @@ def test_long_sums_again_and_again(backend, dtype, rows, n, k):
         assert (first - want).norm() <= 1e-6 * want.norm()
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("out_dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,n,k", [(1, 9480, 64), (8, 11264, 256), (3, 9601, 136), (32, 18944, 128), (17, 18941, 72), (16, 25600, 128), (2, 40, 64)])
+def test_tiles_of_other_heights(backend, dtype, out_dtype, rows, n, k):
+    x, w, b, r = inputs(rows, n, k, dtype, out_dtype)
+    got = backend.matmul_epilogue(x, w, bias=b, activation="silu", residual=r, out_dtype=out_dtype)
+    backend.sync()
+    check(got, x, w, b, r, "silu")
+
+
 @pytest.mark.parametrize("rows", [4, 50])
 def test_every_bit_of_a_row_counts(backend, rows):
     # one nonzero in each row and column: the results are the rows' own values, bit for bit (normal numbers whose least bit

@@ -134,9 +134,8 @@ int yx_matmul_logprobs(yx_ctx *ctx, const void *x_dev, int x_dtype, const void *
     Guard guard(ctx->device);
     Product p = product(x_dev, x_dtype, w_bf16_dev, rows, n, k);
     if (exact_tc_takes(p)) {
-        p.blocks = logprobs_block(p);
         // (the statistics, then the given tokens' logits)
-        const size_t stats = (size_t)rows * p.blocks * 16;
+        const size_t stats = (size_t)rows * most_logprob_blocks(ctx, p) * 16;
         if (int rc = grow(ctx, ctx->lp_stats, stats + (size_t)rows * 4)) return rc;
         p.stats = ctx->lp_stats.dev;
         p.picked = (float *)(ctx->lp_stats.dev + stats);

@@ -199,12 +199,12 @@ __device__ __forceinline__ void stage(const float (&v)[V], int first, float *sta
 }
 __device__ __forceinline__ uint32_t staged_at(uint32_t row, uint32_t column) { return row * 32 + (((column >> 2) ^ (row & 7)) << 2) + (column & 3); }
 
-// Bias, activation and residual of N staged pass rows, t0 and on, by the 32 columns from col0.  All residuals are asked for
-// before the first is used, and what follows is a loop, whose registers move up: unrolled over a thread's up to 128 results
+// Bias, activation and residual of N staged pass rows, t0 and on, by the 32 columns from col0, as far as `end`.  All residuals are asked
+// for before the first is used, and what follows is a loop, whose registers move up: unrolled over a thread's up to 128 results
 // the code does not fit the instruction cache, and out of line every sum still in a register goes through local memory
 // (2048 x [14336, 4096] bf16: 220 us plain, 386 onto a residual with a type looked up for each; out of line 296 and 392).
 template <int N>
-__device__ __forceinline__ void finish_staged(const Epilogue &e, void *out, uint32_t T, uint32_t cols, const float *staged, uint32_t t0, uint32_t col0, int lane) {
+__device__ __forceinline__ void finish_staged(const Epilogue &e, void *out, uint32_t T, uint32_t cols, uint32_t end, const float *staged, uint32_t t0, uint32_t col0, int lane) {
     if (t0 >= T) return;
     const uint32_t rows = min((uint32_t)N, T - t0);
     constexpr int R = N / 4;
@@ -235,7 +235,7 @@ __device__ __forceinline__ void finish_staged(const Epilogue &e, void *out, uint
     if (e.quads) {
         // A turn: four columns a lane, four pass rows a warp.
         const uint32_t q = 4 * (lane & 7), col = col0 + q, r0 = lane >> 3;
-        if (col >= cols) return;
+        if (col >= end) return;
         size_t at = (size_t)(t0 + r0) * cols + col;
         const float4 bias = e.bias ? *(const float4 *)(e.bias + col) : zero;
         ask([&](int dtype, int i) { return r0 + 4 * i < rows ? load4_as_f32(e.residual, dtype, at + (size_t)(4 * i) * cols) : zero; });
@@ -247,7 +247,7 @@ __device__ __forceinline__ void finish_staged(const Epilogue &e, void *out, uint
     } else {
         // A turn: a column a lane, four pass rows.
         const uint32_t col = col0 + lane;
-        if (col >= cols) return;
+        if (col >= end) return;
         size_t at = (size_t)t0 * cols + col;
         const float bias = e.bias ? e.bias[col] : 0.0f;
         ask([&](int dtype, int i) {
@@ -306,16 +306,16 @@ __device__ __forceinline__ RowStats stats_of_16(const float (&v)[N], int first, 
     return RowStats{m, s + __shfl_xor_sync(0xffffffffu, s, 16), t + __shfl_xor_sync(0xffffffffu, t, 16)};
 }
 
-// Of N pass rows from t0 on: this warp's 32 columns, lane i row t0 + i, and the given tokens' logits where they are among them.
+// Of N pass rows from t0 on: this warp's 32 columns as far as `end`, lane i row t0 + i, and the given tokens' logits where they are among them.
 template <int N>
-__device__ __forceinline__ float4 stats_of(const StatsOut &so, uint32_t T, uint32_t cols, const float (&v)[N], uint32_t t0, uint32_t row, const uint32_t *ids,
+__device__ __forceinline__ float4 stats_of(const StatsOut &so, uint32_t T, uint32_t end, const float (&v)[N], uint32_t t0, uint32_t row, const uint32_t *ids,
                                            float *scratch, int lane) {
     const uint32_t t = t0 + lane;
-    const uint32_t want = lane < N && t < T ? ids[t] - (row - lane) : 0xffffffffu;
+    const uint32_t id = lane < N && t < T ? ids[t] : 0xffffffffu, want = id < end ? id - (row - lane) : 0xffffffffu;
     float logit = 0.0f;
-    RowStats st = stats_of_16(v, 0, row < cols, scratch, lane, lane < 16 ? want : 0xffffffffu, logit);
+    RowStats st = stats_of_16(v, 0, row < end, scratch, lane, lane < 16 ? want : 0xffffffffu, logit);
     if constexpr (N > 16) {
-        const RowStats hi = stats_of_16(v, 16, row < cols, scratch, lane, lane < 16 ? 0xffffffffu : want, logit);
+        const RowStats hi = stats_of_16(v, 16, row < end, scratch, lane, lane < 16 ? 0xffffffffu : want, logit);
         if (lane >= 16) st = hi;
     }
     if (want < 32u) so.picked[t] = logit;
@@ -526,7 +526,7 @@ __device__ __forceinline__ void pair_body(const CUtensorMap &w_map, const CUtens
             if constexpr (KIND < EPILOGUE) store_rows<KIND == GLU>(a, v, t, row, lane);
             else if constexpr (KIND == EPILOGUE) {
                 stage<N>(v, 0, scratch, lane);
-                finish_staged<N>(a.e, a.out, a.T, a.cols, scratch, t, row - lane, lane);
+                finish_staged<N>(a.e, a.out, a.T, a.cols, a.cols, scratch, t, row - lane, lane);
             } else {
                 stats_s[chunk][warp][lane] = stats_of(a.so, a.T, a.cols, v, t, row, a.ids, scratch, lane);
             }
@@ -702,7 +702,7 @@ __device__ __forceinline__ void pair_body(const CUtensorMap &w_map, const CUtens
                 }
                 if constexpr (KIND == EPILOGUE) {
                     stage<16>(v, 0, scratch, lane);
-                    finish_staged<16>(a.e, a.out, a.T, a.cols, scratch, t0 + c, row - lane, lane);
+                    finish_staged<16>(a.e, a.out, a.T, a.cols, a.cols, scratch, t0 + c, row - lane, lane);
                 } else {
                     stats_s[0][warp][lane] = stats_of(a.so, a.T, a.cols, v, t0 + c, row, a.ids, scratch, lane);
                     asm volatile("bar.sync %0, 128;" ::"r"(2 + (warp >> 2)) : "memory");
@@ -857,6 +857,7 @@ struct RowsArgs {
     uint32_t T, K, cols, ksteps, units, ctas;
     uint32_t cluster;                 // CTAs that share a tile as one cluster (EPILOGUE, LOGPROBS; 1: none)
     bool whole;                       // every CTA takes whole tiles (EPILOGUE, LOGPROBS)
+    uint32_t wm;                      // weight rows of a tile (a multiple of 4; ROWS_M but for whole tiles)
     uint32_t x_vec16;
     float *out;
     Epilogue e;                       // EPILOGUE (`out` is of its type)
@@ -930,6 +931,7 @@ matmul_rows_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_const
     const uint32_t base = smem_u32(smem);
     const uint32_t b_full = smem_u32(bar_store), b_empty = b_full + 8 * TC_MAX_STAGES;
     const uint32_t b_acc_full = b_empty + 8 * TC_MAX_STAGES, b_acc_empty = b_acc_full + 8 * ROWS_BUFS;
+    const uint32_t wm = KIND < EPILOGUE ? ROWS_M : a.wm;
     volatile int *abortp = &abort_flag;
     uint32_t u0, u1;
     if (KIND >= EPILOGUE && a.cluster > 1) {
@@ -948,7 +950,7 @@ matmul_rows_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_const
     auto weight_rows = [&](uint32_t u, int &x, int &y, int &z) {
         const uint32_t tile = u / a.ksteps;
         x = (int)((u - tile * a.ksteps) * TC_KSTEP);
-        y = GLU_TILES ? 0 : (int)(tile * ROWS_M);
+        y = GLU_TILES ? 0 : (int)(tile * wm);
         z = GLU_TILES ? (int)(tile * (ROWS_M / (2 * GLU_GROUP))) : 0;
     };
     if (warp == 4 && elect()) {
@@ -982,17 +984,17 @@ matmul_rows_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_const
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
-    auto finish = [&](const float (&v)[TP], uint32_t row) {
+    auto finish = [&](const float (&v)[TP], uint32_t tile, uint32_t row) {
         if constexpr (KIND < EPILOGUE) store_few<TP, KIND == GLU>(a, v, row, lane);
         else if constexpr (KIND == EPILOGUE) {
             stage<TP>(v, 0, scratch, lane);
-            finish_staged<TP>(a.e, a.out, a.T, a.cols, scratch, 0, row - lane, lane);
+            finish_staged<TP>(a.e, a.out, a.T, a.cols, min(a.cols, (tile + 1) * wm), scratch, 0, row - lane, lane);
         } else {
-            stats_s[warp][lane] = stats_of(a.so, a.T, a.cols, v, 0, row, a.ids, scratch, lane);
+            stats_s[warp][lane] = stats_of(a.so, a.T, min(a.cols, (tile + 1) * wm), v, 0, row, a.ids, scratch, lane);
             asm volatile("bar.sync 2, 128;" ::: "memory");
             if (warp == 0 && lane < (int)a.T) {
                 const float4 four[4] = {stats_s[0][lane], stats_s[1][lane], stats_s[2][lane], stats_s[3][lane]};
-                a.so.stats[(size_t)lane * a.so.blocks + (row >> 7)] = merge_four(four);
+                a.so.stats[(size_t)lane * a.so.blocks + tile] = merge_four(four);
             }
             asm volatile("bar.sync 2, 128;" ::: "memory");
         }
@@ -1010,13 +1012,13 @@ matmul_rows_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_const
                     mbar_wait_slow(b_empty + 8 * s, phase ^ 1u, abortp, a.status, 511);
                     if (*abortp) break;
                 }
-                mbar_expect_tx(b_full + 8 * s, W_BYTES);
+                mbar_expect_tx(b_full + 8 * s, wm * 128u);
                 tma_load_4d(base + s * STAGE, &w_map, x, y, 0, z, b_full + 8 * s);
                 x += TC_KSTEP;
                 if (x == (int)(a.ksteps * TC_KSTEP)) {   // the next tile
                     x = 0;
                     if (GLU_TILES) z += ROWS_M / (2 * GLU_GROUP);
-                    else y += ROWS_M;
+                    else y += wm;
                 }
                 if (++s == S) {
                     s = 0;
@@ -1129,7 +1131,7 @@ matmul_rows_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_const
         for (uint32_t u = u0; u < u1;) {
             const uint32_t tile = u / a.ksteps, end = min(u1, (tile + 1) * a.ksteps);
             const bool whole = end - u == a.ksteps;
-            const uint32_t wr = warp * 32 + lane, row = tile * ROWS_M + wr;
+            const uint32_t wr = warp * 32 + lane, row = tile * wm + wr;
             // The CTAs that share this tile, found while the tile is being summed (the divisions take a third of a
             // microsecond).  Only the first of them may have begun in a tile before it: then this is its last piece.
             uint32_t q0 = 0, q1 = 0, later = 0;
@@ -1185,7 +1187,7 @@ matmul_rows_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_const
                 if (lane == 0) mbar_arrive(b_acc_empty + 8 * buf);
             }
             if (whole) {
-                finish(v, row);
+                finish(v, tile, row);
                 continue;
             }
             if constexpr (KIND >= EPILOGUE) {
@@ -1227,7 +1229,7 @@ matmul_rows_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_const
 #pragma unroll
                     for (int i = 0; i < TP; i++) v[i] += w[b][i];
             }
-            finish(v, row);
+            finish(v, tile, row);
         }
     }
     __syncwarp();
@@ -1248,7 +1250,7 @@ matmul_rows_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_const
                         if (q < a.cluster) f[0] = make_float4(f[0].x + f[q].x, f[0].y + f[q].y, f[0].z + f[q].z, f[0].w + f[q].w);
                     *(float4 *)(v + i) = f[0];
                 }
-                finish(v, blockIdx.x / a.cluster * ROWS_M + wr);
+                finish(v, blockIdx.x / a.cluster, blockIdx.x / a.cluster * ROWS_M + wr);
             }
             __syncwarp();
             cluster_sync();   // the sums are read
@@ -1286,8 +1288,8 @@ int encode(yx_ctx *ctx, CUtensorMap *map, uint32_t rank, const void *p, const cu
     return r == CUDA_SUCCESS ? YX_OK : fail(ctx, YX_ERR_CUDA, "matmul: cuTensorMapEncodeTiled failed with " + std::to_string((int)r));
 }
 
-// The weights in boxes of 128 rows by 64 k; for a GLU four groups of 16 gate rows and the 16 up rows of the same columns.
-int encode_weights(yx_ctx *ctx, CUtensorMap *map, const void *w, uint32_t N, uint32_t K, bool glu) {
+// The weights in boxes of `rows` rows by 64 k; for a GLU four groups of 16 gate rows and the 16 up rows of the same columns.
+int encode_weights(yx_ctx *ctx, CUtensorMap *map, const void *w, uint32_t N, uint32_t K, bool glu, uint32_t rows = 128) {
     const cuuint64_t row = (cuuint64_t)K * 2;
     if (glu) {
         const cuuint64_t dims[4] = {K, GLU_GROUP, 2, N / 2 / GLU_GROUP};
@@ -1297,7 +1299,7 @@ int encode_weights(yx_ctx *ctx, CUtensorMap *map, const void *w, uint32_t N, uin
     }
     const cuuint64_t dims[4] = {K, N, 1, 1};
     const cuuint64_t strides[3] = {row, N * row, N * row};
-    const cuuint32_t box[4] = {TC_KSTEP, 128, 1, 1};
+    const cuuint32_t box[4] = {TC_KSTEP, rows, 1, 1};
     return encode(ctx, map, 4, w, dims, strides, box);
 }
 
@@ -1510,12 +1512,13 @@ int exact_scratch(yx_ctx *ctx, size_t tiles, float **part, uint32_t **counters) 
 
 // EPILOGUE and LOGPROBS.
 template <int KIND, int CHUNKS>
-int exact_pair_rows(yx_ctx *ctx, const Product &p) {
+int exact_pair_rows(yx_ctx *ctx, Product &p) {
     const size_t n = (size_t)p.T * p.K;
     PairArgs a{};
     if (int rc = plan_pairs<KIND, CHUNKS>(ctx, p, a)) return rc;
     a.out = (float *)p.out;
     a.e = p.e;
+    p.blocks = 2 * ((p.N + TC_M - 1) / TC_M);
     a.so = StatsOut{(float4 *)p.stats, p.blocks, p.picked};
     a.ids = p.ids_dev;
     if (int rc = exact_scratch(ctx, 2 * a.pairs, &a.part, &a.counters)) return rc;
@@ -1546,7 +1549,7 @@ int exact_pair_rows(yx_ctx *ctx, const Product &p) {
 }
 
 template <int TP, int KIND, int PARTS>
-int matmul_few_rows(yx_ctx *ctx, const Product &p) {
+int matmul_few_rows(yx_ctx *ctx, Product &p) {
     constexpr uint32_t stage_bytes = rows_stage_bytes(TP, PARTS), stages = rows_stages(TP, KIND, PARTS);
     auto *kernel = matmul_rows_kernel<TP, KIND, PARTS>;
     bool &configured = ctx->mm_rows_configured[KIND][PARTS - 1][TP / 16];
@@ -1573,7 +1576,8 @@ int matmul_few_rows(yx_ctx *ctx, const Product &p) {
     a.K = K;
     a.cols = KIND == GLU ? N / 2 : N;
     a.ksteps = (K + TC_KSTEP - 1) / TC_KSTEP;
-    const uint32_t tiles = (N + ROWS_M - 1) / ROWS_M;
+    uint32_t tiles = (N + ROWS_M - 1) / ROWS_M;
+    a.wm = ROWS_M;
     a.units = tiles * a.ksteps;
     a.ctas = std::min((uint32_t)ctx->sm_count, std::max(1u, a.units / 2));
     a.cluster = 1;
@@ -1587,17 +1591,23 @@ int matmul_few_rows(yx_ctx *ctx, const Product &p) {
             a.ctas = tiles * c;
             break;
         }
-        // Whole tiles where the last round of them keeps most SMs busy: the idle ones cost less than adding up shares (250 tiles
-        // of 16 k steps 15.1 us, in equal shares 16.3, 393 of 32 37.8 and 42.5; but 224 of 64 45.3 and 43.7, 157 of 32 23.1 and 19.3).
-        const uint32_t last = tiles % a.ctas;
-        if (a.cluster == 1 && (last == 0 || last * 5 >= a.ctas * 3)) {
+        // Whole tiles where there is one round of them or the last keeps half of the SMs busy, and then tiles as low as fill the
+        // rounds: cheaper than adding up shares (us: 88 tiles of 32 k steps, 8 f16 rows, 13.7 in equal shares and 10.8 as 148 lower ones, 79
+        // of 16 steps 9.0 and 6.8, 224 of 64 44.5 and 42.3; but 157 of 32 16.9 and 17.6, 172 of 64 32.4 and 33.1).
+        const uint32_t sms = (uint32_t)ctx->sm_count, last = tiles % sms;
+        if (a.cluster == 1 && (tiles <= sms || last == 0 || last * 2 >= sms)) {
+            const uint32_t most = (tiles + sms - 1) / sms * sms, each = (N + most - 1) / most;
             a.whole = true;
-            a.ctas = std::min(a.ctas, tiles);
+            a.wm = std::clamp((each + 3) / 4 * 4, 32u, ROWS_M);
+            tiles = (N + a.wm - 1) / a.wm;
+            a.units = tiles * a.ksteps;
+            a.ctas = std::min(sms, tiles);
         }
     }
     a.x_vec16 = ((uintptr_t)a.x & 15u) == 0;
     a.out = (float *)p.out;
     a.e = p.e;
+    p.blocks = tiles;
     a.so = StatsOut{(float4 *)p.stats, p.blocks, p.picked};
     if (KIND == LOGPROBS) std::copy(p.ids_host, p.ids_host + T, a.ids);
     a.status = ctx->dev_status;
@@ -1611,13 +1621,13 @@ int matmul_few_rows(yx_ctx *ctx, const Product &p) {
         return rc;
     }
     CUtensorMap w_map;
-    if (int rc = encode_weights(ctx, &w_map, p.w, N, K, KIND == GLU)) return rc;
+    if (int rc = encode_weights(ctx, &w_map, p.w, N, K, KIND == GLU, a.wm)) return rc;
     ctx->last_launch = yx_ctx::LAST_OTHER;
     return launch_cluster(ctx, "matmul kernel launch", kernel, dim3(a.ctas), dim3(ROWS_THREADS), stages * stage_bytes, a.cluster > 1 ? a.cluster : 0, w_map, a);
 }
 
 template <int KIND>
-int matmul_tc(yx_ctx *ctx, const Product &p) {
+int matmul_tc(yx_ctx *ctx, Product &p) {
     if (p.T <= 8) return matmul_few_rows<8, KIND, 2>(ctx, p);
     if (p.T <= 16) return matmul_few_rows<16, KIND, 2>(ctx, p);
     if (p.T <= 32) return matmul_few_rows<32, KIND, 2>(ctx, p);
@@ -1628,7 +1638,7 @@ int matmul_tc(yx_ctx *ctx, const Product &p) {
 }
 
 template <int KIND, int PARTS>
-int exact_few_rows(yx_ctx *ctx, const Product &p) {
+int exact_few_rows(yx_ctx *ctx, Product &p) {
     // (eight columns of one part are fewer than an MMA takes)
     if constexpr (PARTS > 1)
         if (p.T <= 8) return matmul_few_rows<8, KIND, PARTS>(ctx, p);
@@ -1636,15 +1646,14 @@ int exact_few_rows(yx_ctx *ctx, const Product &p) {
     return matmul_few_rows<32, KIND, PARTS>(ctx, p);
 }
 template <int KIND>
-int exact_tc(yx_ctx *ctx, const Product &p) {
+int exact_tc(yx_ctx *ctx, Product &p) {
     if (p.T <= ROWS_MAX)
         return p.parts == 1 ? exact_few_rows<KIND, 1>(ctx, p) : p.parts == 2 ? exact_few_rows<KIND, 2>(ctx, p) : exact_few_rows<KIND, 3>(ctx, p);
-    Product q = p;
-    if (int rc = exact_row_tiles<KIND>(ctx, p, &q.t_tiles)) return rc;
-    const uint32_t rows = rows_of_tiles(p.T, q.t_tiles);
-    if (rows <= 128) return exact_pair_rows<KIND, 2>(ctx, q);
-    if (rows <= 192) return exact_pair_rows<KIND, 3>(ctx, q);
-    return exact_pair_rows<KIND, 4>(ctx, q);
+    if (int rc = exact_row_tiles<KIND>(ctx, p, &p.t_tiles)) return rc;
+    const uint32_t rows = rows_of_tiles(p.T, p.t_tiles);
+    if (rows <= 128) return exact_pair_rows<KIND, 2>(ctx, p);
+    if (rows <= 192) return exact_pair_rows<KIND, 3>(ctx, p);
+    return exact_pair_rows<KIND, 4>(ctx, p);
 }
 
 }  // namespace
@@ -1664,8 +1673,9 @@ int launch_matmul_tc(yx_ctx *ctx, const float *x, const void *w, uint32_t T, uin
 
 bool exact_tc_takes(const Product &p) { return p.K % 8 == 0 && ((uintptr_t)p.w & 15u) == 0; }
 bool exact_tc_reads_rows_late(const Product &p) { return p.T <= ROWS_MAX || p.parts == 1; }
-uint32_t logprobs_block(const Product &p) { return p.T <= ROWS_MAX ? (p.N + ROWS_M - 1) / ROWS_M : 2 * ((p.N + TC_M - 1) / TC_M); }
-int launch_matmul_epilogue_tc(yx_ctx *ctx, const Product &p) { return exact_tc<EPILOGUE>(ctx, p); }
-int launch_matmul_logprobs_tc(yx_ctx *ctx, const Product &p) { return exact_tc<LOGPROBS>(ctx, p); }
+// (lower tiles are at most as many more as complete a round of SMs)
+uint32_t most_logprob_blocks(yx_ctx *ctx, const Product &p) { return 2 * ((p.N + TC_M - 1) / TC_M) + (uint32_t)ctx->sm_count; }
+int launch_matmul_epilogue_tc(yx_ctx *ctx, Product &p) { return exact_tc<EPILOGUE>(ctx, p); }
+int launch_matmul_logprobs_tc(yx_ctx *ctx, Product &p) { return exact_tc<LOGPROBS>(ctx, p); }
 
 }  // namespace yx

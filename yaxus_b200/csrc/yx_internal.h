@@ -411,17 +411,17 @@ struct Product {
     uint32_t t_tiles;        // tiles that more than 32 pass rows are spread over
     void *out;
     Epilogue e;              // yx_matmul_epilogue
-    void *stats;             // yx_matmul_logprobs: float4 [T][blocks], blocks = logprobs_block(p)
-    uint32_t blocks;
+    void *stats;             // yx_matmul_logprobs: float4 [T][blocks], at most most_logprob_blocks of them
+    uint32_t blocks;         // (set by the launch)
     float *picked;           // logits of the given tokens [T]
     const uint32_t *ids_dev, *ids_host;   // for more than 32 rows; for fewer
 };
 bool exact_tc_takes(const Product &p);
 // Whether the kernel that writes the result is also the one that reads the rows.
 bool exact_tc_reads_rows_late(const Product &p);
-uint32_t logprobs_block(const Product &p);
-int launch_matmul_epilogue_tc(yx_ctx *ctx, const Product &p);
-int launch_matmul_logprobs_tc(yx_ctx *ctx, const Product &p);
+uint32_t most_logprob_blocks(yx_ctx *ctx, const Product &p);
+int launch_matmul_epilogue_tc(yx_ctx *ctx, Product &p);
+int launch_matmul_logprobs_tc(yx_ctx *ctx, Product &p);
 
 // The statistics of softmax rows: logprobs.cu.  put_ids brings `n` given tokens to the device (ctx->lp_ids).
 int put_ids(yx_ctx *ctx, const uint32_t *host, size_t n, const uint32_t **out);
