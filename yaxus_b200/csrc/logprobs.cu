@@ -57,7 +57,7 @@ __device__ __forceinline__ RowStats merge_warp(RowStats r) {
 // part into tiles of 16 logits a thread, the next tile's loads in flight while one is worked on.  A thread keeps the
 // statistics (m, s, t) of what it has seen, m any number near its largest logit, and notes the tile that has that.
 //
-// The n best tokens of a part come from that: of 32 groups of threads, the n-th largest of the groups' best is a bound that n
+// The n best tokens of a part come from that: of 32 or 64 groups of threads, the n-th largest of the groups' best is a bound that n
 // tokens reach, and only the n or so threads whose best reaches it can hold others that do.  Their logits are read once
 // more, a warp to a thread's, and what reaches the bound (n to some 4 n tokens) is put in order.  Where too many logits
 // equal it the bound is a key of logit and token, which are all different.  (With a list that grew as the logits went by, and a
@@ -95,22 +95,44 @@ struct Best {
     uint8_t thread[THREADS];
 };
 
-// The n-th largest of 32 groups' largest keys; a group is a lane of every warp.  All threads get it, after two barriers.
+// The n-th largest of the largest keys of 32 groups of threads, lanes of every warp, or of 64 where n is near 32: the least of 32
+// groups is reached by some 130 keys, the 32nd of 64 by 44 (16 rows of 32000 bf16 with 32 tokens 17.6 and 9.8 us, with 20 tokens 8.0 and
+// 8.2).  All threads get it, after two barriers.
 __device__ __forceinline__ uint64_t nth_of_groups(Best &b, uint64_t best, uint32_t n) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     b.group[warp][lane] = best;
     __syncthreads();
     if (warp == 0) {
         uint64_t g = best;
+        if (n <= 20) {
 #pragma unroll
-        for (int w = 1; w < WARPS; w++) g = max(g, b.group[w][lane]);
-        uint32_t larger = 0;
+            for (int w = 1; w < WARPS; w++) g = max(g, b.group[w][lane]);
+            uint32_t above = 0;   // (groups without a token share key 0)
 #pragma unroll
-        for (int i = 0; i < 32; i++) {
-            const uint64_t other = __shfl_sync(0xffffffffu, g, i);
-            larger += other > g || (other == g && i < lane);   // (groups without a token share key 0)
+            for (int i = 0; i < 32; i++) {
+                const uint64_t other = __shfl_sync(0xffffffffu, g, i);
+                above += other > g || (other == g && i < lane);
+            }
+            if (above == n - 1) b.least = g;
+        } else {
+            // (the list has nothing on it yet, and lends its room)
+#pragma unroll
+            for (int w = 2; w < WARPS; w += 2) g = max(g, b.group[w][lane]);
+            b.key[lane] = g;
+            g = b.group[1][lane];
+#pragma unroll
+            for (int w = 3; w < WARPS; w += 2) g = max(g, b.group[w][lane]);
+            b.key[32 + lane] = g;
+            __syncwarp();
+#pragma unroll 1
+            for (int j = lane; j < 64; j += 32) {
+                g = b.key[j];
+                uint32_t above = 0;
+#pragma unroll 8
+                for (int i = 0; i < 64; i++) above += b.key[i] > g || (b.key[i] == g && i < j);
+                if (above == n - 1) b.least = g;
+            }
         }
-        if (larger == n - 1) b.least = g;
     }
     __syncthreads();
     return b.least;
@@ -346,7 +368,9 @@ __global__ void __launch_bounds__(THREADS, 5) logprob_rows_kernel(const __grid_c
 #pragma unroll
                     for (int e = 0; e < T::WIDE; e++) {
                         const uint32_t t = own * T::WIDE + e - shift;
-                        add_to_list(b, own < v1 && t < a.cols && reaches(x[e], t), key_of(x[e], t));
+                        if (!(own < v1 && t < a.cols && reaches(x[e], t))) continue;
+                        const uint32_t at = atomicAdd(&b.count, 1u);   // (few are: a vote for each logit takes longer)
+                        if (at < LIST) b.key[at] = key_of(x[e], t);
                     }
                 }
             }
