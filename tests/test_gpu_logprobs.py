@@ -159,6 +159,28 @@ def test_large_ones_in_a_few_places(backend, dtype, rows, cols):
         check(x[i:i + 100], ids[i:i + 100], 32, type(r)(*(t[i:i + 100] for t in r)))
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,cols", [(1, 60000), (300, 20011)])
+@pytest.mark.parametrize("top", [2, 20, 21, 32])
+def test_the_best_in_one_thread_s_share(backend, dtype, rows, cols, top):
+    # a thread's logits are 16 bytes in every 4096: the best lie in one thread's, in one of its tiles, in two or in all of them
+    wide = 4 if dtype == torch.float32 else 8
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(top)
+    x = torch.randn(rows, cols, generator=gen, device="cuda").clamp(-3, 3)
+    c = torch.arange(cols, device="cuda")
+    own = (c // wide) % 256 == 77
+    tile = c // (256 * 16)
+    for i in range(rows):
+        where = own & (tile == 1) if i % 3 == 0 else own & (tile >= 1) & (tile < 3) if i % 3 == 1 else own
+        x[i, where] = 5 + torch.rand(int(where.sum()), generator=gen, device="cuda")
+    x = x.to(dtype)
+    ids = np.full((rows, 1), 77 * wide)
+    r = backend.logprob_rows(x, ids, top=top, entropy=True)
+    backend.sync()
+    check(x, ids, top, r)
+
+
 def test_large_numbers(backend):
     x = torch.zeros(7, 5000, device="cuda")
     x[0, 17] = INF                      # counts as the largest f32

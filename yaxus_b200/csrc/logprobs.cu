@@ -55,14 +55,16 @@ __device__ __forceinline__ RowStats merge_warp(RowStats r) {
 //
 // One pass over the logits.  A row is cut into parts, a CTA each (one part where there are rows enough to fill the chip), and a
 // part into tiles of 16 logits a thread, the next tile's loads in flight while one is worked on.  A thread keeps the
-// statistics (m, s, t) of what it has seen, m any number near its largest logit, and notes the tile that has that.
+// statistics (m, s, t) of what it has seen, m any number near its largest logit, and notes the tile that has its largest and the
+// largest outside that tile.
 //
 // The n best tokens of a part come from that: of 32 or 64 groups of threads, the n-th largest of the groups' best is a bound that n
-// tokens reach, and only the n or so threads whose best reaches it can hold others that do.  Their logits are read once
-// more, a warp to a thread's, and what reaches the bound (n to some 4 n tokens) is put in order.  Where too many logits
-// equal it the bound is a key of logit and token, which are all different.  (With a list that grew as the logits went by, and a
-// barrier a tile for it, 2048 rows of 50257 took 170 us for five tokens and 82 without.)  The parts' tokens and statistics
-// meet in the row's last CTA.
+// tokens reach, and only the n or so threads whose best reaches it can hold others that do.  Of most of those the best tile alone
+// can, whose logits are read once more; of the few whose others may all are, a warp to a thread's (2048 rows of 50257 f32 with
+// five and 20 tokens 76.2 and 79.4 us; all logits of all of them 76.0 and 94.2, as what is read is 16 bytes in every 4096).  What reaches
+// the bound (n to some 2 n tokens) is put in order.  Where too many logits equal it the bound is a key of logit and
+// token, which are all different.  (With a list that grew as the logits went by, and a barrier a tile for it, five tokens took
+// 170 us.)  The parts' tokens and statistics meet in the row's last CTA.
 constexpr int THREADS = 256, WARPS = THREADS / 32;
 constexpr int PER_THREAD = 16;                              // logits of a tile
 constexpr int TILE = THREADS * PER_THREAD;
@@ -91,8 +93,9 @@ struct Best {
     uint64_t group[WARPS][32];
     uint64_t warp_best[2][WARPS];
     uint64_t least;
-    uint32_t count, threads;
-    uint8_t thread[THREADS];
+    uint32_t count, threads, tiles;
+    uint8_t thread[THREADS];     // whose all have to be looked at
+    uint2 tile[THREADS];         // a tile and a thread
 };
 
 // The n-th largest of the largest keys of 32 groups of threads, lanes of every warp, or of 64 where n is near 32: the least of 32
@@ -283,13 +286,14 @@ struct Tile {
 // first tile hardly any thread's m moves again (with m the largest so far, some lane of a warp moved it in most tiles).
 constexpr float HEADROOM = 8.0f;
 
-// Five CTAs an SM: 48 registers a thread, and two or three of them spilled (2048 rows of 50257 bf16 with five tokens 58 us; four
-// CTAs 64, three 73, six with half the logits in flight each 69).
+// Five CTAs an SM: 48 registers a thread, which is tight (2048 rows of 50257 bf16 with five tokens 58 us; four CTAs 64, three
+// 73, six with half the logits in flight each 69; with the given token's logit in shared memory, which leaves next to no spills, 55).
 template <int DTYPE, bool TOP>
 __global__ void __launch_bounds__(THREADS, 5) logprob_rows_kernel(const __grid_constant__ RowsArgs a) {
     __shared__ Best b;
     __shared__ RowStats scratch[2][WARPS];
     __shared__ bool last;
+    __shared__ float given_s[THREADS];
     using T = Tile<DTYPE>;
     dependent_entry();
     const uint32_t row = blockIdx.x / a.parts, part = blockIdx.x - row * a.parts;
@@ -311,6 +315,7 @@ __global__ void __launch_bounds__(THREADS, 5) logprob_rows_kernel(const __grid_c
     RowStats r = no_stats();
     F2 s2 = f2(0.0f, 0.0f), t2 = s2;
     float best = -INFINITY;
+    float second = -INFINITY;         // the largest outside that tile
     uint32_t best_at = 0xffffffffu;   // the tile of the first of this thread's largest logits
     T next;
     auto load = [&](uint32_t v) {
@@ -318,6 +323,7 @@ __global__ void __launch_bounds__(THREADS, 5) logprob_rows_kernel(const __grid_c
         else next.load(base, shift, a.cols, v + threadIdx.x, THREADS, v1);
     };
     load(v0);
+    if (threadIdx.x < a.n_ids) given_s[threadIdx.x] = given;   // (a register is worth more)
     for (uint32_t v = v0; v < v1; v += STEP) {
         const T tile = next;
         if (v + STEP < v1) load(v + STEP);
@@ -326,9 +332,13 @@ __global__ void __launch_bounds__(THREADS, 5) logprob_rows_kernel(const __grid_c
         float most = x[0];
 #pragma unroll
         for (int j = 1; j < PER_THREAD; j++) most = fmaxf(most, x[j]);
-        if (TOP && clean(most) > best) {
-            best = clean(most);
-            best_at = v;
+        if constexpr (TOP) {
+            const float c = clean(most);
+            second = fmaxf(second, fminf(best, c));
+            if (c > best) {
+                best = c;
+                best_at = v;
+            }
         }
         if (most > r.m + HEADROOM) {
             if (most == INFINITY) {
@@ -353,36 +363,46 @@ __global__ void __launch_bounds__(THREADS, 5) logprob_rows_kernel(const __grid_c
     share_stats(r, scratch[0]);
     if constexpr (TOP) {
         const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-        // Puts on the list what `reaches` of the logits of the threads that are `in`; between barriers.
-        auto look_again = [&](bool in, auto reaches) {
-            if (in) b.thread[atomicAdd(&b.threads, 1u)] = (uint8_t)threadIdx.x;
+        // Puts on the list what `reaches` of the logits of the threads that are `in`, or of their best tile if that is `one`; between
+        // barriers.
+        auto look_again = [&](bool in, bool one, auto reaches) {
+            if (in) {
+                if (one) b.tile[atomicAdd(&b.tiles, 1u)] = make_uint2(best_at, threadIdx.x);
+                else b.thread[atomicAdd(&b.threads, 1u)] = (uint8_t)threadIdx.x;
+            }
             __syncthreads();
+            auto look = [&](uint32_t own) {
+                Tile<DTYPE, T::WIDE> again;
+                again.load(base, shift, a.cols, own, 0, v1);
+                float x[T::WIDE];
+                again.unpack(x);
+#pragma unroll
+                for (int e = 0; e < T::WIDE; e++) {
+                    const uint32_t t = own * T::WIDE + e - shift;
+                    if (!(own < v1 && t < a.cols && reaches(x[e], t))) continue;
+                    const uint32_t at = atomicAdd(&b.count, 1u);   // (few are: a vote for each logit takes longer)
+                    if (at < LIST) b.key[at] = key_of(x[e], t);
+                }
+            };
+            for (uint32_t i = threadIdx.x; i < b.tiles * T::VECS; i += THREADS) {
+                const uint2 at = b.tile[i / T::VECS];
+                look(at.x + at.y + i % T::VECS * THREADS);
+            }
             for (uint32_t i = warp; i < b.threads; i += WARPS) {
                 for (uint32_t v = v0 + b.thread[i]; v < v1; v += 32 * THREADS) {
                     if (__any_sync(0xffffffffu, *(volatile uint32_t *)&b.count > LIST)) break;
-                    const uint32_t own = v + lane * THREADS;
-                    Tile<DTYPE, T::WIDE> again;
-                    again.load(base, shift, a.cols, own, 0, v1);
-                    float x[T::WIDE];
-                    again.unpack(x);
-#pragma unroll
-                    for (int e = 0; e < T::WIDE; e++) {
-                        const uint32_t t = own * T::WIDE + e - shift;
-                        if (!(own < v1 && t < a.cols && reaches(x[e], t))) continue;
-                        const uint32_t at = atomicAdd(&b.count, 1u);   // (few are: a vote for each logit takes longer)
-                        if (at < LIST) b.key[at] = key_of(x[e], t);
-                    }
+                    look(v + lane * THREADS);
                 }
             }
             __syncthreads();
         };
-        if (threadIdx.x == 0) b.count = b.threads = 0;
+        if (threadIdx.x == 0) b.count = b.threads = b.tiles = 0;
         // The bound is a logit; only where too many equal it (or it is the forbidden's) is it a logit and a token.
         const uint64_t bound = nth_of_groups(b, v0 + threadIdx.x < v1 ? key_of(best, 0) : 0, a.n_top);
         const float least = key_logit(bound);
         bool precise = bound == 0 || least == -INFINITY;
         if (!precise) {
-            look_again(best >= least, [&](float x, uint32_t) { return x >= least; });
+            look_again(best >= least, second < least, [&](float x, uint32_t) { return x >= least; });
             precise = b.count > LIST;
             __syncthreads();
         }
@@ -398,10 +418,10 @@ __global__ void __launch_bounds__(THREADS, 5) logprob_rows_kernel(const __grid_c
                     if (clean(x[j]) == best) at = j;
                 token = (best_at + threadIdx.x + at / T::WIDE * THREADS) * T::WIDE + at % T::WIDE - shift;
             }
-            if (threadIdx.x == 0) b.count = b.threads = 0;
+            if (threadIdx.x == 0) b.count = b.threads = b.tiles = 0;
             const uint64_t mine = v0 + threadIdx.x < v1 ? key_of(best, token) : 0;
             const uint64_t reached = nth_of_groups(b, mine, a.n_top);
-            look_again(mine != 0 && mine >= reached, [&](float x, uint32_t t) { return key_of(x, t) >= reached; });
+            look_again(mine != 0 && mine >= reached, false, [&](float x, uint32_t t) { return key_of(x, t) >= reached; });
         }
         const uint32_t t0 = T::first_token(v0, shift), t1 = min(a.cols, v1 * T::WIDE - shift);
         order_list(b, a.n_top, t1 - t0, [&](uint32_t i) { return key_of(load_as_f32(logits, DTYPE, t0 + i), t0 + i); });
@@ -454,7 +474,7 @@ __global__ void __launch_bounds__(THREADS, 5) logprob_rows_kernel(const __grid_c
         r = all_stats(scratch[1]);
     }
     const float log_s = logf(r.s);
-    if (threadIdx.x < a.n_ids) a.logprob[(size_t)row * a.n_ids + threadIdx.x] = log_prob(given, r.m, log_s);
+    if (threadIdx.x < a.n_ids) a.logprob[(size_t)row * a.n_ids + threadIdx.x] = log_prob(given_s[threadIdx.x], r.m, log_s);
     for (uint32_t i = threadIdx.x + THREADS; i < a.n_ids; i += THREADS)
         a.logprob[(size_t)row * a.n_ids + i] = log_prob(load_as_f32(logits, DTYPE, ids[i]), r.m, log_s);
     if (threadIdx.x == 0 && a.entropy) a.entropy[row] = entropy(r);
