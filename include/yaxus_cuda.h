@@ -280,7 +280,11 @@ enum yx_activation {
 
 /* out [rows, n] = act(x [rows, k] . w [n, k]^T + bias) + residual.  x of `x_dtype`, taken exactly (no
  * rounding to w's type); w bf16; bias f32 [n] or null; residual [rows, n] of `out_dtype` or null.  Sums
- * and epilogue are f32, rounded once to `out_dtype`.  out may be the residual itself (x += ...) and may
+ * and epilogue are f32, rounded once to `out_dtype`.  The sums of f32 results are within a millionth (2-norm
+ * of the error over the result's); those of 16-bit results of more than 32 rows stay longer in the tensor
+ * cores' accumulators, which cut off what lies below their last place, and are within 4 to 7 millionths: where K
+ * is some thousands, one result in 400 of bf16 and one in 50 of f16 is the neighbour of the correctly rounded
+ * value (of f32 sums one in 2500 and one in 250).  out may be the residual itself (x += ...) and may
  * lie over x; over w, over the bias or over part of the residual it is refused. */
 int yx_matmul_epilogue(yx_ctx *ctx, const void *x_dev, int x_dtype, const void *w_bf16_dev, const float *bias_dev,
                        int activation, const void *residual_dev, uint32_t rows, uint32_t n, uint32_t k, void *out_dev,
