@@ -1,6 +1,6 @@
 """What the operators between hidden states and log probabilities promise at their edges: how 16-bit results are rounded after long
-sums."""
-import numpy as np  # noqa: F401
+sums, rows in which one token has nearly all the weight."""
+import numpy as np
 import pytest
 import torch
 
@@ -40,3 +40,46 @@ def test_long_sums_of_16_bit_results(backend, dtype, out_dtype, rows, n, k):
     # ... and nothing is further off than that neighbour: half a step, and what 384 whole last places of the terms' sum are
     most = 384 * 2.0 ** -23 * (x.double().abs() @ w.double().abs().T)
     assert ((got.double() - want).abs() <= step / 2 + most).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,cols", [(80, 9000), (3, 9000), (3, 300000)])
+def test_two_tokens_with_all_the_weight(backend, dtype, rows, cols):
+    # the second best is seen first, by the thread that sees the best later; all others weigh exp(-60)
+    d = torch.linspace(0.1, 12.0, rows, device="cuda")
+    x = torch.full((rows, cols), -55.0, device="cuda")
+    x[:, 4099] = 5.0
+    x[:, 3] = 5.0 - d
+    x = x.to(dtype)
+    r = backend.logprob_rows(x, np.tile([4099, 3], (rows, 1)), top=2, entropy=True)
+    backend.sync()
+    d = (x[:, 4099].double() - x[:, 3].double())
+    w = torch.exp(-d)
+    log_s = torch.log1p(w)
+    h = log_s + w * d / (1 + w)
+    # w: its exponent's argument has two roundings (relative, of d) and 2^x is off by two last places at most.  1 + w is rounded
+    # three times on its way (a thread's two sums, their sum; the others' add nothing), the logarithm is off by a last place.
+    w_err = w * (2.0 ** -22 + 1.5 * d * 2.0 ** -24)
+    s_err = w_err + 3 * 2.0 ** -24
+    log_err = s_err + log_s * 2.0 ** -23
+    assert ((r.logprob[:, 0] + log_s).abs() <= log_err + log_s * 2.0 ** -23).all()
+    assert ((r.logprob[:, 1] + d + log_s).abs() <= log_err + (d + log_s) * 2.0 ** -23).all()
+    # t = -w d with w's error and three roundings; t / s with those of s and its own
+    t_err = w_err * d + 3 * w * d * 2.0 ** -24
+    assert ((r.entropy - h).abs() <= log_err + t_err + w * d * s_err + (w * d + h) * 2.0 ** -23).all()
+    assert torch.equal(r.top_logprob, r.logprob)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_no_probability_exceeds_one(backend, dtype):
+    # some token of a row stands 4 to 30 above a bell, anywhere in the row
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(5)
+    for rows, cols in ((3000, 9001), (3, 150001)):
+        for shift in range(4 if rows > 3 else 40):
+            x = torch.randn(rows, cols, generator=gen, device="cuda")
+            at = torch.randint(0, cols, (rows, 1), generator=gen, device="cuda")
+            x.scatter_(1, at, 4 + 26 * torch.rand(rows, 1, generator=gen, device="cuda"))
+            r = backend.logprob_rows(x.to(dtype), at.cpu().numpy(), top=3, entropy=True)
+            backend.sync()
+            assert (r.logprob <= 0).all() and (r.top_logprob <= 0).all() and (r.entropy >= 0).all()

@@ -55,7 +55,7 @@ __device__ __forceinline__ RowStats merge_warp(RowStats r) {
 //
 // One pass over the logits.  A row is cut into parts, a CTA each (one part where there are rows enough to fill the chip), and a
 // part into tiles of 16 logits a thread, the next tile's loads in flight while one is worked on.  A thread keeps the
-// statistics (m, s, t) of what it has seen, m any number near its largest logit, and notes the tile that has its largest and the
+// statistics (m, s, t) of what it has seen, m its warp's largest logit so far, and notes the tile that has its largest and the
 // largest outside that tile.
 //
 // The n best tokens of a part come from that: of 32 or 64 groups of threads, the n-th largest of the groups' best is a bound that n
@@ -282,10 +282,6 @@ struct Tile {
     static __device__ __forceinline__ uint32_t first_token(uint32_t vec, uint32_t shift) { return vec > 0 ? vec * WIDE - shift : 0u; }
 };
 
-// How far a logit may exceed the m of the statistics before m moves: exp(8) of it still adds up without harm, and after the
-// first tile hardly any thread's m moves again (with m the largest so far, some lane of a warp moved it in most tiles).
-constexpr float HEADROOM = 8.0f;
-
 // Five CTAs an SM: 48 registers a thread, which is tight (2048 rows of 50257 bf16 with five tokens 58 us; four CTAs 64, three
 // 73, six with half the logits in flight each 69; with the given token's logit in shared memory, which leaves next to no spills, 55).
 template <int DTYPE, bool TOP>
@@ -340,7 +336,11 @@ __global__ void __launch_bounds__(THREADS, 5) logprob_rows_kernel(const __grid_c
                 best_at = v;
             }
         }
-        if (most > r.m + HEADROOM) {
+        // m is never below a logit that has been added: where one token has nearly all the weight, log s and l - m are then near 0 and
+        // not near 8 and -8 with their last places to lose, s >= 1 and t <= 0, and no probability exceeds 1.  One m for a warp takes
+        // one instruction, and moves in the first tiles and with the few logits that stand out of a row.
+        most = warp_max(most);
+        if (most > r.m) {
             if (most == INFINITY) {
 #pragma unroll
                 for (int j = 0; j < PER_THREAD; j++) x[j] = clean(x[j]);
