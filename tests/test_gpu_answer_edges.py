@@ -1,5 +1,5 @@
 """What the operators between hidden states and log probabilities promise at their edges: how 16-bit results are rounded after long
-sums, rows in which one token has nearly all the weight."""
+sums, activations far below zero, rows in which one token has nearly all the weight."""
 import numpy as np
 import pytest
 import torch
@@ -40,6 +40,31 @@ def test_long_sums_of_16_bit_results(backend, dtype, out_dtype, rows, n, k):
     # ... and nothing is further off than that neighbour: half a step, and what 384 whole last places of the terms' sum are
     most = 384 * 2.0 ** -23 * (x.double().abs() @ w.double().abs().T)
     assert ((got.double() - want).abs() <= step / 2 + most).all()
+
+
+@pytest.mark.parametrize("act", ["gelu", "gelu_tanh", "silu"])
+@pytest.mark.parametrize("rows,k", [(4, 200), (50, 200), (300, 200), (50, 201)])
+def test_activations_near_and_far_from_zero(backend, act, rows, k):
+    # the product is the row's first value itself, so that all that errs is the activation: each result by its own last places
+    y = torch.linspace(-12.0, 12.0, rows, device="cuda")
+    x = torch.zeros(rows, k, device="cuda")
+    x[:, 0] = y
+    w = torch.zeros(24, k, device="cuda").bfloat16()
+    w[:, 0] = 1.0
+    got = backend.matmul_epilogue(x, w, activation=act).double()
+    backend.sync()
+    v = y.double()[:, None].expand(rows, 24)
+    if act == "gelu":
+        want = 0.5 * v * torch.special.erfc(-v * 0.5 ** 0.5)
+        u = v * v           # erfc(z) moves by 2 z^2 + 1 of z's relative error at most, z = -y / sqrt 2
+    else:
+        u = -v if act == "silu" else -2 * (2 / np.pi) ** 0.5 * (v + 0.044715 * v ** 3)
+        want = v / (1 + u.exp())
+    # An argument errs by 8 half units of itself at most (gelu_tanh's polynomial has five operations), the function by four last
+    # places (erfc), what is made of it by three more roundings.  Where 1 + exp(u) passes 2^126 its reciprocal is no normal f32 and
+    # counts as 0: no more than |y| <= 12 times 2^-126 is lost (gelu_tanh is 1.6e-61 at -12).
+    tol = want.abs() * ((u.abs() + 1) * 8 * 2.0 ** -24 + 4 * 2.0 ** -23 + 3 * 2.0 ** -24) + 12 * 2.0 ** -126
+    assert ((got - want).abs() <= tol).all()
 
 
 @pytest.mark.parametrize("dtype", TYPES)
