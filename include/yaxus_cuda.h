@@ -296,7 +296,7 @@ int yx_matmul_epilogue(yx_ctx *ctx, const void *x_dev, int x_dtype, const void *
  *   entropy  [rows]:         -sum p log p, in nats
  *   top_ids, top_logprob [rows, n_top]: the most probable tokens, largest first, equal logits by token
  * Each may be null (logprob with n_ids 0, the top pair with n_top 0); n_top <= YX_TOP_MAX and <= cols.
- * Results over the logits are refused.
+ * Results over the logits or over one another are refused.
  * A logit that is no number counts as -inf, as in yx_argmax_rows, and +inf as the largest f32.  A row
  * with nothing above -inf has log probabilities -inf and entropy 0. */
 #define YX_TOP_MAX 32
@@ -306,7 +306,7 @@ int yx_logprob_rows(yx_ctx *ctx, const void *logits_dev, int dtype, uint32_t row
 
 /* yx_logprob_rows of the logits x [rows, k] . w [n, k]^T, one given token a row, without the logits:
  * logprob [rows] of ids_host [rows], entropy [rows] or null.  x and w as for yx_matmul_epilogue; results over
- * either are refused. */
+ * either or over one another are refused. */
 int yx_matmul_logprobs(yx_ctx *ctx, const void *x_dev, int x_dtype, const void *w_bf16_dev, uint32_t rows, uint32_t n,
                        uint32_t k, const uint32_t *ids_host, float *logprob_dev, float *entropy_dev);
 

@@ -1,8 +1,10 @@
 """What the operators between hidden states and log probabilities promise at their edges: how 16-bit results are rounded after long
-sums, activations far below zero, rows in which one token has nearly all the weight."""
+sums, activations far below zero, rows in which one token has nearly all the weight, results over one another."""
 import numpy as np
 import pytest
 import torch
+
+from yaxus_b200 import _lib
 
 pytestmark = pytest.mark.gpu
 TYPES = [torch.float32, torch.float16, torch.bfloat16]
@@ -108,3 +110,34 @@ def test_no_probability_exceeds_one(backend, dtype):
             r = backend.logprob_rows(x.to(dtype), at.cpu().numpy(), top=3, entropy=True)
             backend.sync()
             assert (r.logprob <= 0).all() and (r.top_logprob <= 0).all() and (r.entropy >= 0).all()
+
+
+def test_results_over_one_another_are_refused(backend):
+    x = torch.randn(3, 50, device="cuda")
+    h, w = torch.randn(3, 64, device="cuda"), torch.randn(50, 64, device="cuda").bfloat16()
+    out = torch.zeros(64, device="cuda")
+    ids = np.zeros((3, 2), np.uint32)
+    L, c, i, o = backend._L, backend._ctx, ids.ctypes.data, out.data_ptr()
+    rows = lambda p, e, t, l: L.yx_logprob_rows(c, x.data_ptr(), 0, 3, 50, 50, i, 2, 4, p, e, t, l)      # noqa: E731
+    # in order: 6 log probabilities, 3 entropies, 12 tokens, 12 of theirs
+    places = [o, o + 24, o + 36, o + 84]
+    for k in range(4):
+        for j in range(4):
+            if j != k:
+                at = list(places)
+                at[k] = places[j]
+                assert rows(*at) == _lib.YX_ERR_INVALID, (k, j)
+                backend.clear_error()
+    for at in ([o, o + 20, o + 36, o + 84], [o, o + 24, o + 32, o + 84], [o, o + 24, o + 36, o + 80], [o + 132, o + 24, o + 36, o + 88]):
+        assert rows(*at) == _lib.YX_ERR_INVALID
+        backend.clear_error()
+    head = lambda p, e: L.yx_matmul_logprobs(c, h.data_ptr(), 0, w.data_ptr(), 3, 50, 64, i, p, e)       # noqa: E731
+    for p, e in ((o, o), (o, o + 8), (o + 8, o)):
+        assert head(p, e) == _lib.YX_ERR_INVALID
+        backend.clear_error()
+    torch.cuda.synchronize()
+    assert (out == 0).all()
+    assert rows(*places) == _lib.YX_OK and head(o + 160, o + 172) == _lib.YX_OK       # side by side they are taken
+    backend.sync()
+    lp = torch.log_softmax(x.double(), 1)
+    assert (out[:6] - lp[:, 0].repeat_interleave(2)).abs().max() <= 1e-5

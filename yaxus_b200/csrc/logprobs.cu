@@ -602,6 +602,15 @@ extern "C" int yx_logprob_rows(yx_ctx *ctx, const void *logits_dev, int dtype, u
     };
     if (over(logprob_dev, n_ids) || over(entropy_dev, 1) || over(top_ids_dev, n_top) || over(top_logprob_dev, n_top))
         return fail(ctx, YX_ERR_INVALID, "logprob_rows: a result lies over the logits");
+    const struct {
+        const void *p;
+        size_t each;
+    } results[] = {{logprob_dev, n_ids}, {entropy_dev, 1}, {top_ids_dev, n_top}, {top_logprob_dev, n_top}};
+    for (int i = 0; i < 4; i++)
+        for (int j = 0; j < i; j++)
+            if (results[i].p && results[j].p && (uintptr_t)results[i].p < (uintptr_t)results[j].p + (size_t)rows * results[j].each * 4 &&
+                (uintptr_t)results[j].p < (uintptr_t)results[i].p + (size_t)rows * results[i].each * 4)
+                return fail(ctx, YX_ERR_INVALID, "logprob_rows: results lie over one another");
     for (size_t i = 0; i < (size_t)rows * n_ids; i++)
         if (ids_host[i] >= cols) return fail(ctx, YX_ERR_INVALID, "logprob_rows: a token id is outside the vocabulary");
     if (n_ids == 0 && n_top == 0 && !entropy_dev) return YX_OK;

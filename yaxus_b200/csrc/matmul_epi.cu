@@ -129,6 +129,7 @@ int yx_matmul_logprobs(yx_ctx *ctx, const void *x_dev, int x_dtype, const void *
     if (overlap(logprob_dev, results, x_dev, x_bytes) || overlap(logprob_dev, results, w_bf16_dev, w_bytes) || overlap(entropy_dev, results, x_dev, x_bytes) ||
         overlap(entropy_dev, results, w_bf16_dev, w_bytes))
         return fail(ctx, YX_ERR_INVALID, "matmul_logprobs: a result lies over the rows or the weight");
+    if (overlap(logprob_dev, results, entropy_dev, results)) return fail(ctx, YX_ERR_INVALID, "matmul_logprobs: the results lie over one another");
     for (uint32_t r = 0; r < rows; r++)
         if (ids_host[r] >= n) return fail(ctx, YX_ERR_INVALID, "matmul_logprobs: a token id is outside the vocabulary");
     Guard guard(ctx->device);
