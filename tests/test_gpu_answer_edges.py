@@ -1,5 +1,6 @@
 """What the operators between hidden states and log probabilities promise at their edges: how 16-bit results are rounded after long
-sums, activations far below zero, rows in which one token has nearly all the weight, results over one another."""
+sums, activations far below zero, rows in which one token has nearly all the weight, results over one another,
+empty batches."""
 import numpy as np
 import pytest
 import torch
@@ -141,3 +142,16 @@ def test_results_over_one_another_are_refused(backend):
     backend.sync()
     lp = torch.log_softmax(x.double(), 1)
     assert (out[:6] - lp[:, 0].repeat_interleave(2)).abs().max() <= 1e-5
+
+
+def test_what_is_asked_for_of_no_rows_and_no_tokens_is_empty(backend):
+    x = torch.randn(3, 50, device="cuda")
+    for shape in ((0,), (0, 2), (0, 0)):
+        r = backend.logprob_rows(x[:0], np.zeros(shape, np.uint32), top=4, entropy=True)
+        assert r.logprob.shape == shape and r.entropy.shape == (0,) and r.top_ids.shape == r.top_logprob.shape == (0, 4)
+    r = backend.logprob_rows(x, np.zeros((3, 0), np.uint32), top=4)
+    backend.sync()
+    assert r.logprob.shape == (3, 0) and torch.equal(r.top_ids.long(), x.topk(4).indices)
+    r = backend.matmul_logprobs(torch.zeros(0, 64, device="cuda"), torch.zeros(50, 64, device="cuda").bfloat16(), [])
+    backend.sync()
+    assert r.logprob.shape == r.entropy.shape == (0,)

@@ -364,10 +364,10 @@ class CudaBackend:
             n_ids = idx.size // max(rows, 1)
         # (allocations are half of a call's time on the host; sizes as plain arguments and no type where it is the logits' are quickest)
         new = logits.new_empty if dtype == F32 else lambda *shape: logits.new_empty(*shape, dtype=torch.float32)   # noqa: E731
-        r = LogProbs(new(*idx.shape) if n_ids else None, new(rows) if entropy else None,
+        r = LogProbs(new(*idx.shape) if ids is not None else None, new(rows) if entropy else None,
                      logits.new_empty(rows, top, dtype=torch.int32) if top else None, new(rows, top) if top else None)
         self._L.yx_logprob_rows(self._ctx, logits.data_ptr(), dtype, rows, cols, stride if rows > 1 else cols, _u32p(idx) if n_ids else None, n_ids,
-                                top, _ptr(r.logprob), _ptr(r.entropy), _ptr(r.top_ids), _ptr(r.top_logprob))
+                                top, _ptr(r.logprob) if n_ids else None, _ptr(r.entropy), _ptr(r.top_ids), _ptr(r.top_logprob))
         return r
 
     def matmul_logprobs(self, x: torch.Tensor, w: torch.Tensor, ids, entropy: bool = True) -> LogProbs:
