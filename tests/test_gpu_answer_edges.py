@@ -1,11 +1,12 @@
 """What the operators between hidden states and log probabilities promise at their edges: how 16-bit results are rounded after long
 sums, activations far below zero, rows in which one token has nearly all the weight, results over one another,
-empty batches."""
+empty batches, a device with little memory left."""
 import numpy as np
 import pytest
 import torch
 
 from yaxus_b200 import _lib
+from yaxus_b200.backend import CudaBackend
 
 pytestmark = pytest.mark.gpu
 TYPES = [torch.float32, torch.float16, torch.bfloat16]
@@ -155,3 +156,32 @@ def test_what_is_asked_for_of_no_rows_and_no_tokens_is_empty(backend):
     r = backend.matmul_logprobs(torch.zeros(0, 64, device="cuda"), torch.zeros(50, 64, device="cuda").bfloat16(), [])
     backend.sync()
     assert r.logprob.shape == r.entropy.shape == (0,)
+
+
+def test_scratch_takes_what_it_needs_where_more_does_not_fit(backend):
+    # an inner size that the tensor cores do not take: the scratch are 2000 rows of 8000 logits, 64 MB
+    stream = torch.cuda.Stream()
+    b = CudaBackend(0, stream)
+    hold = []
+    with torch.cuda.stream(stream):
+        x = torch.randn(2000, 9, device="cuda")
+        w = torch.randn(8000, 9, device="cuda").bfloat16()
+        ids = np.zeros(2000, np.uint32)
+        want = b.matmul_logprobs(x, w, ids)
+        b.close()
+        b = CudaBackend(0, stream)
+        b.matmul_logprobs(x[:40], w, ids[:40])          # the scratch's first size: the next may be half as large again
+        b.sync()
+        torch.cuda.empty_cache()
+        try:
+            # fill the device up to 70 to 82 MiB: 61 fit, 92 do not
+            for size in (1 << 30, 64 << 20, 12 << 20):
+                while torch.cuda.mem_get_info()[0] > (70 << 20) + size:
+                    hold.append(torch.empty(size, dtype=torch.uint8, device="cuda"))
+            got = b.matmul_logprobs(x, w, ids)
+            b.sync()
+            assert torch.equal(got.logprob, want.logprob) and torch.equal(got.entropy, want.entropy)
+        finally:
+            hold.clear()
+            torch.cuda.empty_cache()
+    b.close()

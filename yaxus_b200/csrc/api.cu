@@ -56,9 +56,15 @@ int grow(yx_ctx *ctx, yx_ctx::Grown &buf, size_t bytes) {
     if (int rc = check_cuda(ctx, cudaStreamIsCapturing(ctx->stream, &capture), "cudaStreamIsCapturing")) return rc;
     if (capture != cudaStreamCaptureStatusNone)
         return fail(ctx, YX_ERR_STATE, "scratch would have to grow while the stream is being captured: make a call of this size first");
-    const size_t want = std::max<size_t>(buf.dev ? bytes + bytes / 2 : bytes, 4096);
+    size_t want = std::max<size_t>(buf.dev ? bytes + bytes / 2 : bytes, 4096);
     void *p = nullptr;
-    if (int rc = check_cuda(ctx, cudaMalloc(&p, want), "cudaMalloc (workspace)")) return rc;
+    cudaError_t e = cudaMalloc(&p, want);
+    if (e == cudaErrorMemoryAllocation && want > bytes) {   // (no room to grow into: what this call needs may still fit)
+        cudaGetLastError();
+        want = bytes;
+        e = cudaMalloc(&p, want);
+    }
+    if (int rc = check_cuda(ctx, e, "cudaMalloc (workspace)")) return rc;
     try {
         if (buf.dev) ctx->outgrown.push_back(buf.dev);
     } catch (const std::bad_alloc &) {
