@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from yaxus_b200 import _lib
-from yaxus_b200.backend import CudaBackend
+from yaxus_b200.backend import BackendError, CudaBackend
 
 pytestmark = pytest.mark.gpu
 TYPES = [torch.float32, torch.float16, torch.bfloat16]
@@ -184,4 +184,33 @@ def test_scratch_takes_what_it_needs_where_more_does_not_fit(backend):
         finally:
             hold.clear()
             torch.cuda.empty_cache()
+    b.close()
+
+
+def test_an_error_is_its_own_call_s_alone(backend):
+    # a call that finds no memory: the next one's launch, and its check, know nothing of it
+    stream = torch.cuda.Stream()
+    b = CudaBackend(0, stream)
+    hold = []
+    with torch.cuda.stream(stream):
+        x = torch.randn(2000, 9, device="cuda")
+        w = torch.randn(8000, 9, device="cuda").bfloat16()
+        b.matmul_epilogue(x[:40], w[:8])
+        b.sync()
+        torch.cuda.empty_cache()
+        try:
+            for size in (1 << 30, 64 << 20, 12 << 20):
+                while torch.cuda.mem_get_info()[0] > (34 << 20) + size:
+                    hold.append(torch.empty(size, dtype=torch.uint8, device="cuda"))
+            b.matmul_logprobs(x, w, np.zeros(2000, np.uint32))     # logits of 64 MB
+            assert b.status() == _lib.YX_ERR_OOM
+            with pytest.raises(BackendError):
+                b.sync()
+            b.clear_error()
+            small = b.matmul_epilogue(x[:40], w[:8])
+            b.sync()
+        finally:
+            hold.clear()
+            torch.cuda.empty_cache()
+        assert (small.double() - x[:40].double() @ w[:8].double().T).abs().max() <= 1e-4
     b.close()

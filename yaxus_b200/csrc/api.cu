@@ -20,6 +20,7 @@ int fail(yx_ctx *ctx, int code, const std::string &msg) {
 
 int check_cuda(yx_ctx *ctx, cudaError_t e, const char *what) {
     if (e == cudaSuccess) return YX_OK;
+    cudaGetLastError();   // (recorded here: left with the runtime it would show again at the next launch's check, whoever's that is)
     int code = e == cudaErrorMemoryAllocation ? YX_ERR_OOM : YX_ERR_CUDA;
     return fail(ctx, code, std::string(what) + ": " + cudaGetErrorString(e));
 }
