@@ -268,7 +268,8 @@ int yx_attend_static(yx_ctx *ctx, yx_kv *kv, int layer, const void *q_dev, int q
  * and is never given back before yx_ctx_destroy, so a recorded call stays valid whatever calls
  * follow it; a call that would have to allocate while its stream is being captured is refused (make
  * one of its size before).  Calls of one context, recorded ones included, share that scratch:
- * replay them in the order of one stream. */
+ * replay them in the order of one stream.  Where cut rows or statistics of blocks of columns would take
+ * more than 256 MB, the rows are taken in slices (cut rows of a result that lies over them are not). */
 
 enum yx_activation {
     YX_ACT_NONE = 0,

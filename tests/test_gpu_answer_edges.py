@@ -1,6 +1,7 @@
 """What the operators between hidden states and log probabilities promise at their edges: how 16-bit results are rounded after long
 sums, activations far below zero, rows in which one token has nearly all the weight, results over one another,
-empty batches, a device with little memory left."""
+empty batches, a device with little memory left, more rows than
+are taken at a time."""
 import numpy as np
 import pytest
 import torch
@@ -214,3 +215,48 @@ def test_an_error_is_its_own_call_s_alone(backend):
             torch.cuda.empty_cache()
         assert (small.double() - x[:40].double() @ w[:8].double().T).abs().max() <= 1e-4
     b.close()
+
+
+def used_by(call):
+    """Bytes of device memory a new context has taken for a call."""
+    b = CudaBackend(0, torch.cuda.current_stream())
+    torch.cuda.synchronize()
+    before = torch.cuda.mem_get_info()[0]
+    out = call(b)
+    b.sync()
+    used = before - torch.cuda.mem_get_info()[0]
+    b.close()
+    return out, used
+
+
+def test_scratch_does_not_grow_with_all_rows(backend):
+    # 256 MB for statistics or parts of rows (either would be some 320 and 390 MB here), 40 for shares, and some for small ones
+    most = (256 + 40 + 16) << 20
+    x, w = product(16000, 64, 4096, torch.float32)
+    bias, res, out = torch.randn(64, device="cuda"), torch.randn(16000, 64, device="cuda"), torch.empty(16000, 64, device="cuda")
+    backend.matmul_epilogue(x[:4000], w, bias=bias)                   # (the kernels are on the device before memory is counted)
+    _, used = used_by(lambda b: b.matmul_epilogue(x, w, bias=bias, residual=res, activation="relu", out=out))
+    assert used <= most, used
+    want = (x.double() @ w.double().T + bias.double()).clamp(min=0) + res.double()
+    assert (out - want).norm() <= 1e-6 * want.norm()
+    # rows under the result are all taken before it is written
+    square = x[:, :64].contiguous()
+    wide = (torch.randn(64, 64, device="cuda") / 8).bfloat16()
+    both = backend.matmul_epilogue(square, wide)
+    backend.matmul_epilogue(square, wide, out=square)
+    backend.sync()
+    assert torch.equal(square, both)
+
+    for dtype in (torch.bfloat16, torch.float32):
+        x, w = product(50000, 32000, 64, dtype)
+        w *= 8
+        ids = np.arange(50000) * 7 % 32000
+        backend.matmul_logprobs(x[:4000], w, ids[:4000])
+        r, used = used_by(lambda b: b.matmul_logprobs(x, w, ids))
+        assert used <= most, used
+        for at in (0, 24900, 49700):                                  # ends, and where one slice follows another
+            lp = torch.log_softmax(x[at:at + 300].double() @ w.double().T, 1)
+            want = lp.gather(1, torch.as_tensor(ids[at:at + 300], device="cuda")[:, None])[:, 0]
+            h = torch.special.entr(lp.exp()).sum(1)
+            # (sums of 64 products; log probabilities of some -10 in f32, and the sums of 32000 terms)
+            assert (r.logprob[at:at + 300] - want).norm() <= 2e-6 * want.norm() and (r.entropy[at:at + 300] - h).norm() <= 4e-6 * h.norm()

@@ -61,6 +61,16 @@ int matmul_any(yx_ctx *ctx, const Product &p, int x_dtype) {
     return YX_OK;
 }
 
+// Rows that are taken at a time where a row needs `each` bytes of scratch: all of them within 256 MB (10000 f32 rows of 4096,
+// 14000 rows of 128256 columns' statistics, past which reading the weights once more is nothing), else even slices.
+constexpr size_t MOST_SCRATCH = (size_t)256 << 20;
+uint32_t rows_at_once(uint32_t rows, size_t each) {
+    const size_t most = std::max<size_t>(1, MOST_SCRATCH / std::max<size_t>(each, 1));
+    if (rows <= most) return rows;
+    const uint32_t even = (uint32_t)((rows + ((rows - 1) / most)) / ((rows - 1) / most + 1));
+    return most < 256 ? even : (uint32_t)std::min<size_t>(most / 256 * 256, ((size_t)even + 255) / 256 * 256);
+}
+
 Product product(const void *x, int x_dtype, const void *w, uint32_t T, uint32_t N, uint32_t K) {
     Product p{};
     p.x = x;
@@ -111,7 +121,19 @@ int yx_matmul_epilogue(yx_ctx *ctx, const void *x_dev, int x_dtype, const void *
         ctx->last_launch = yx_ctx::LAST_OTHER;
         p.x = ctx->ep_rows.dev;
     }
-    return tensor ? launch_matmul_epilogue_tc(ctx, p) : matmul_any(ctx, p, x_dtype);
+    if (!tensor) return matmul_any(ctx, p, x_dtype);
+    // (a result over rows that are cut into parts waits for all of them to be)
+    const bool scratch = p.parts > 1 || !aligned(p.x, 16);
+    const uint32_t step = scratch && !overlap(out_dev, out_bytes, x_dev, x_bytes) ? rows_at_once(rows, (size_t)k * 2 * p.parts) : rows;
+    for (uint32_t r = 0; r < rows; r += step) {
+        Product s = p;
+        s.x = (const char *)p.x + (size_t)r * k * size_of(x_dtype);
+        s.T = std::min(step, rows - r);
+        s.out = (char *)out_dev + (size_t)r * n * size_of(out_dtype);
+        if (residual_dev) s.e.residual = (const char *)residual_dev + (size_t)r * n * size_of(out_dtype);
+        if (int rc = launch_matmul_epilogue_tc(ctx, s)) return rc;
+    }
+    return YX_OK;
 }
 
 int yx_matmul_logprobs(yx_ctx *ctx, const void *x_dev, int x_dtype, const void *w_bf16_dev, uint32_t rows, uint32_t n, uint32_t k,
@@ -136,15 +158,25 @@ int yx_matmul_logprobs(yx_ctx *ctx, const void *x_dev, int x_dtype, const void *
     Product p = product(x_dev, x_dtype, w_bf16_dev, rows, n, k);
     if (exact_tc_takes(p)) {
         // (the statistics, then the given tokens' logits)
-        const size_t stats = (size_t)rows * most_logprob_blocks(ctx, p) * 16;
-        if (int rc = grow(ctx, ctx->lp_stats, stats + (size_t)rows * 4)) return rc;
+        const size_t row_stats = (size_t)most_logprob_blocks(ctx, p) * 16;
+        const bool scratch = p.parts > 1 || !aligned(x_dev, 16);
+        const uint32_t step = rows_at_once(rows, std::max(row_stats, scratch ? (size_t)k * 2 * p.parts : (size_t)0));
+        if (int rc = grow(ctx, ctx->lp_stats, step * (row_stats + 4))) return rc;
         p.stats = ctx->lp_stats.dev;
-        p.picked = (float *)(ctx->lp_stats.dev + stats);
-        p.ids_host = ids_host;
+        p.picked = (float *)(ctx->lp_stats.dev + step * row_stats);
+        const uint32_t *ids_dev = nullptr;
         if (rows > 32)
-            if (int rc = put_ids(ctx, ids_host, rows, &p.ids_dev)) return rc;
-        if (int rc = launch_matmul_logprobs_tc(ctx, p)) return rc;
-        return launch_logprob_blocks(ctx, p.stats, p.blocks, p.picked, rows, logprob_dev, entropy_dev);
+            if (int rc = put_ids(ctx, ids_host, rows, &ids_dev)) return rc;
+        for (uint32_t r = 0; r < rows; r += step) {
+            Product s = p;
+            s.x = (const char *)x_dev + (size_t)r * k * size_of(x_dtype);
+            s.T = std::min(step, rows - r);
+            s.ids_host = ids_host + r;
+            s.ids_dev = ids_dev ? ids_dev + r : nullptr;
+            if (int rc = launch_matmul_logprobs_tc(ctx, s)) return rc;
+            if (int rc = launch_logprob_blocks(ctx, s.stats, s.blocks, s.picked, s.T, logprob_dev + r, entropy_dev ? entropy_dev + r : nullptr)) return rc;
+        }
+        return YX_OK;
     }
     // Logits of as many rows as 64 MB hold, then their log probabilities.
     const uint32_t step = (uint32_t)std::max<size_t>(1, std::min<size_t>(rows, ((size_t)64 << 20) / ((size_t)n * 4)));

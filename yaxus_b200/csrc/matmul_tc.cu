@@ -1545,7 +1545,8 @@ int exact_pair_rows(yx_ctx *ctx, Product &p) {
                                       (uint4 *)ctx->ep_rows.dev))
             return rc;
     }
-    // (with LOGPROBS the given tokens' kernel is ahead, which starts this one after its own wait too)
+    // (with LOGPROBS the given tokens' kernel is ahead, or that of the slice of rows before, which start this one after their own
+    // waits too)
     a.early_w = p.parts > 1 || KIND == LOGPROBS;
     return launch_pairs<KIND, CHUNKS>(ctx, w_map, x_map, a);
 }
