@@ -280,7 +280,11 @@ enum yx_activation {
 };
 
 /* out [rows, n] = act(x [rows, k] . w [n, k]^T + bias) + residual.  x of `x_dtype`, taken exactly (no
- * rounding to w's type); w bf16; bias f32 [n] or null; residual [rows, n] of `out_dtype` or null.  Sums
+ * rounding to w's type) down to 2^-133, the least bf16: only f32 values under 2^-110 have bits below that.
+ * w bf16 and finite: f16 and f32 rows go to the tensor cores in parts, of which some are 0, and what an
+ * infinite weight makes of them is an infinity or no number (in its own column; where the value is 1, say,
+ * no number).  K a multiple of 8 and w on 16 bytes take the tensor cores; anything else takes a kernel
+ * that reads the weights once for every row (2048 rows 100 to 200 times as long).  bias f32 [n] or null; residual [rows, n] of `out_dtype` or null.  Sums
  * and epilogue are f32, rounded once to `out_dtype`.  The sums of f32 results are within a millionth (2-norm
  * of the error over the result's); those of 16-bit results of more than 32 rows stay longer in the tensor
  * cores' accumulators, which cut off what lies below their last place, and are within 4 to 7 millionths: where K

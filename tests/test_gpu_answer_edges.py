@@ -1,7 +1,7 @@
 """What the operators between hidden states and log probabilities promise at their edges: how 16-bit results are rounded after long
 sums, activations far below zero, rows in which one token has nearly all the weight, results over one another,
 empty batches, a device with little memory left, more rows than
-are taken at a time."""
+are taken at a time, the least values of rows, infinite weights."""
 import numpy as np
 import pytest
 import torch
@@ -260,3 +260,42 @@ def test_scratch_does_not_grow_with_all_rows(backend):
             h = torch.special.entr(lp.exp()).sum(1)
             # (sums of 64 products; log probabilities of some -10 in f32, and the sums of 32000 terms)
             assert (r.logprob[at:at + 300] - want).norm() <= 2e-6 * want.norm() and (r.entropy[at:at + 300] - h).norm() <= 4e-6 * h.norm()
+
+
+@pytest.mark.parametrize("rows,k", [(16, 128), (64, 128), (64, 129)])
+def test_the_least_values_of_rows(backend, rows, k):
+    # one nonzero in each row and column: results are the rows' own values, whole from 2^-110 on, below that to the least bf16, 2^-133
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(2)
+    at = torch.arange(rows, device="cuda")
+    w = torch.zeros(128, k, device="cuda").bfloat16()
+    w[torch.arange(128), torch.arange(128)] = 1
+    for e in (-60, -100, -110, -112, -120, -126, -132, -140):
+        v = ((torch.randint(1 << 23, 1 << 24, (rows,), generator=gen, device="cuda") | 1).double() * 2.0 ** (e - 23)).float()
+        x = torch.zeros(rows, k, device="cuda")
+        x[at, 2 * at] = v
+        got = backend.matmul_epilogue(x, w)
+        backend.sync()
+        off = (got[at, 2 * at].double() - v.double()).abs().max().item()
+        assert off == 0 if e >= -110 else off < 2.0 ** -133
+        got[at, 2 * at] = 0
+        assert (got == 0).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,k", [(4, 128), (64, 128), (64, 129)])
+def test_an_infinite_weight_stays_in_its_column(backend, dtype, rows, k):
+    x, w = product(rows, 96, k, dtype)
+    want = backend.matmul_epilogue(x, w)
+    x[0, 9] = 1
+    want[0] = backend.matmul_epilogue(x, w)[0]
+    w[17, 9] = float("inf")
+    got = backend.matmul_epilogue(x, w)
+    backend.sync()
+    others = torch.arange(96, device="cuda") != 17
+    assert torch.equal(got[:, others], want[:, others])
+    assert not got[:, 17].isfinite().any()
+    number = ~got[:, 17].isnan()
+    assert torch.equal(got[number, 17], torch.sign(x[number, 9].float()) * float("inf"))
+    if dtype == torch.bfloat16 or k % 8:            # rows that are not cut into parts
+        assert number.all()
