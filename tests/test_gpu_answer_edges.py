@@ -1,13 +1,17 @@
 """What the operators between hidden states and log probabilities promise at their edges: how 16-bit results are rounded after long
 sums, activations far below zero, rows in which one token has nearly all the weight, results over one another,
 empty batches, a device with little memory left, more rows than
-are taken at a time, the least values of rows, infinite weights."""
+are taken at a time, the least values of rows, infinite weights, every way a product is dealt out to the SMs."""
+import ctypes
+
 import numpy as np
 import pytest
 import torch
 
 from yaxus_b200 import _lib
 from yaxus_b200.backend import BackendError, CudaBackend
+
+from .test_gpu_logprobs import tolerances
 
 pytestmark = pytest.mark.gpu
 TYPES = [torch.float32, torch.float16, torch.bfloat16]
@@ -299,3 +303,72 @@ def test_an_infinite_weight_stays_in_its_column(backend, dtype, rows, k):
     assert torch.equal(got[number, 17], torch.sign(x[number, 9].float()) * float("inf"))
     if dtype == torch.bfloat16 or k % 8:            # rows that are not cut into parts
         assert number.all()
+
+
+# (rows, columns, inner size, how it is dealt out on 148 SMs): tiles' sums added up in clusters, whole tiles, shares that meet in scratch;
+# of the pair kernel shares of the tiles behind whole rounds, and shares that run over a tile's end where there is no whole round.
+DEALT = [
+    (1, 4096, 2048, "few, clusters"), (8, 18000, 1024, "few, whole"), (8, 20000, 4096, "few, shares"), (1, 25600, 1024, "few, shares"),
+    (32, 40000, 512, "few, shares"), (17, 38001, 768, "few, shares"), (64, 4096, 2048, "pairs, clusters"), (300, 9400, 512, "pairs, whole"),
+    (80, 40000, 2048, "pairs, rest shared"), (64, 19200, 4096, "pairs, rest shared"), (300, 20000, 2048, "pairs, rest shared"),
+    (600, 13000, 1024, "pairs, rest shared"), (100, 12000, 4096, "pairs, shares"), (250, 11000, 4096, "pairs, shares"), (130, 11500, 4104, "pairs, shares")]
+
+
+def dealt_out(backend):
+    out = np.zeros(6, np.uint32)
+    assert backend._L.yx_hook_last_product(backend._ctx, out.ctypes.data_as(ctypes.POINTER(ctypes.c_uint32))) == _lib.YX_OK
+    kind, cluster, rounds, rest, shares, _ = out.tolist()
+    if cluster > 1:
+        return ("few, " if kind == 1 else "pairs, ") + "clusters"
+    if kind == 1:
+        return "few, whole" if rounds else "few, shares"
+    return "pairs, whole" if shares == rest else "pairs, rest shared" if rounds else "pairs, shares"
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,n,k,dealt", DEALT)
+def test_products_however_they_are_dealt_out(backend, dtype, rows, n, k, dealt):
+    x, w = product(rows, n, k, dtype)
+    res = torch.randn(rows, n, device="cuda")
+    got = backend.matmul_epilogue(x, w, residual=res)
+    assert dealt_out(backend) == dealt
+    for _ in range(6):
+        again = backend.matmul_epilogue(x, w, residual=res)
+        backend.sync()
+        assert torch.equal(got, again)
+    # (sums within a millionth of the result, and the residual's rounding)
+    want = x.double() @ w.double().T
+    assert (got.double() - res.double() - want).norm() <= 1e-6 * want.norm() + 2.0 ** -24 * (want + res.double()).norm()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,n,k,dealt", DEALT)
+def test_heads_however_they_are_dealt_out(backend, dtype, rows, n, k, dealt):
+    x, w = product(rows, n, k, dtype)
+    w *= 2
+    xd, wd = x.double(), w.double().T
+    logits = xd @ wd
+    lp = torch.log_softmax(logits, 1)
+    h = torch.special.entr(lp.exp()).sum(1)
+    # A logit's chains and shares are at most 512 f32 additions one after the other, a last place each; a log probability moves by no more
+    # than its own logit and the largest move of any, the entropy by that times 1 + its spread.
+    move = 512 * 2.0 ** -23 * (xd.abs() @ wd.abs()).amax(1)
+    spread = logits.amax(1) - logits.amin(1)
+    for turn in range(4):
+        # tokens of every column tile, the ends of tiles among them
+        ids = ((np.arange(rows) * 127 + 128 * turn * 37 + 127) % n).astype(np.uint32) if turn else np.full(rows, n - 1, np.uint32)
+        r = backend.matmul_logprobs(x, w, ids)
+        assert dealt_out(backend) == dealt
+        for _ in range(6):
+            again = backend.matmul_logprobs(x, w, ids)
+            backend.sync()
+            assert torch.equal(r.logprob, again.logprob) and torch.equal(r.entropy, again.entropy)
+        at = torch.as_tensor(ids.astype(np.int64), device="cuda")[:, None]
+        lp_tol, h_tol = tolerances(n, lp, h)
+        want = lp.gather(1, at)[:, 0]
+        assert ((r.logprob - want).abs() <= 2 * move + lp_tol.gather(1, at)[:, 0]).all()
+        assert ((r.entropy - h).abs() <= 2 * move * (1 + spread) + h_tol).all()
+        assert (r.logprob - want).norm() <= 2e-6 * want.norm() + 1e-7 * rows ** 0.5
+        # The entropy's error is that of independent errors of logits, a millionth of their size each, weighted with p (|log p| + h) and
+        # added up as squares, and of its sums of n terms: a place or two of log n.
+        assert (r.entropy - h).norm() <= 4e-6 * h.norm()

@@ -139,6 +139,12 @@ extern "C" int yx_hook_skip_merge(yx_ctx *ctx, int on) {
     return YX_OK;
 }
 
+extern "C" int yx_hook_last_product(yx_ctx *ctx, uint32_t *out6) {
+    if (!ctx || !out6) return YX_ERR_INVALID;
+    memcpy(out6, ctx->mm_last, sizeof ctx->mm_last);
+    return YX_OK;
+}
+
 namespace {
 
 // One CTA, one mbarrier that nobody arrives on, the same bounded wait the attention kernels use

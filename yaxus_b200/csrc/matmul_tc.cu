@@ -1459,7 +1459,9 @@ int plan_pairs(yx_ctx *ctx, const Product &p, PairArgs &a) {
 
 template <int KIND, int CHUNKS>
 int launch_pairs(yx_ctx *ctx, const CUtensorMap &w_map, const CUtensorMap &x_map, const PairArgs &a) {
-    const uint32_t shares = a.cluster > 1 ? a.rest_units / a.ksteps * a.cluster : a.rest_pairs;
+    const uint32_t rest = a.rest_units / a.ksteps, shares = a.cluster > 1 ? rest * a.cluster : a.rest_pairs;
+    const uint32_t dealt[6] = {2, a.cluster, a.rounds, rest, shares, a.chain};
+    std::copy(dealt, dealt + 6, ctx->mm_last);
     const dim3 grid(2 * (a.rounds > 0 ? a.pairs : shares)), block(TC_THREADS);
     const size_t smem = a.stages * (W_BYTES + a.parts * a.bt * 64u);
     if constexpr (KIND < EPILOGUE) return launch_dependent(ctx, "matmul kernel launch", pair_kernel<KIND, CHUNKS>(), grid, block, smem, w_map, x_map, a);
@@ -1625,6 +1627,8 @@ int matmul_few_rows(yx_ctx *ctx, Product &p) {
     }
     CUtensorMap w_map;
     if (int rc = encode_weights(ctx, &w_map, p.w, N, K, KIND == GLU, a.wm)) return rc;
+    const uint32_t dealt[6] = {1, a.cluster, a.whole, tiles, a.ctas, ROWS_CHAIN};
+    std::copy(dealt, dealt + 6, ctx->mm_last);
     ctx->last_launch = yx_ctx::LAST_OTHER;
     return launch_cluster(ctx, "matmul kernel launch", kernel, dim3(a.ctas), dim3(ROWS_THREADS), stages * stage_bytes, a.cluster > 1 ? a.cluster : 0, w_map, a);
 }

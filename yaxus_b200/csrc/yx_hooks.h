@@ -59,6 +59,12 @@ int yx_hook_set_trace(yx_ctx *ctx, void *dev_buf);
  * Measured only by a library built with -DYX_TRACE; otherwise YX_ERR_UNSUPPORTED. */
 int yx_hook_host_times(yx_ctx *ctx, double *out8, int reset);
 
+/* How the context's last product on the tensor cores was dealt out, as six words: 1 for the kernel of few rows
+ * and 2 for pairs of CTAs; CTAs (pairs) that share a tile as one cluster, 1 for none; whole rounds of tiles
+ * (few rows: 1 where every CTA takes whole tiles); tiles left over, and the CTAs (pairs) that share
+ * those (of few rows all tiles and CTAs); k steps that are summed in tensor memory at a time. */
+int yx_hook_last_product(yx_ctx *ctx, uint32_t *out6);
+
 #ifdef __cplusplus
 }
 #endif

@@ -353,6 +353,7 @@ struct yx_ctx {
     bool mm_rows_configured[4][3][3] = {}; // opt-in to large shared memory of the few-row matmul kernels
     int mm_rows_clusters[4][3][3][8] = {}; // clusters of them that fit the chip together
     int mm_clusters[4][3][4] = {};         // clusters of the matmul kernel (by its kind, the tile's size, CTA pairs) that fit the chip together
+    uint32_t mm_last[6] = {};              // how the last product was dealt out (yx_hook_last_product)
     uint32_t *idx_dev = nullptr;           // token ids / row indices / argmax parts of the model operators
     size_t idx_cap = 0;
     uint32_t *pick_counters = nullptr;     // argmax: arrivals per row, zero between launches
