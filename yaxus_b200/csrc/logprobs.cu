@@ -282,7 +282,7 @@ struct Tile {
     static __device__ __forceinline__ uint32_t first_token(uint32_t vec, uint32_t shift) { return vec > 0 ? vec * WIDE - shift : 0u; }
 };
 
-// Five CTAs an SM: 48 registers a thread, which is tight (2048 rows of 50257 bf16 with five tokens 58 us; four CTAs 64, three
+// Five CTAs an SM: 48 registers a thread, which is tight (2048 rows of 50257 bf16 with five tokens then 58 us; four CTAs 64, three
 // 73, six with half the logits in flight each 69; with the given token's logit in shared memory, which leaves next to no spills, 55).
 template <int DTYPE, bool TOP>
 __global__ void __launch_bounds__(THREADS, 5) logprob_rows_kernel(const __grid_constant__ RowsArgs a) {

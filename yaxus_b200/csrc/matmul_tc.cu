@@ -61,14 +61,14 @@ constexpr uint32_t TC_SMEM_BUDGET = 220 * 1024;
 // 80 rows pays 19 us of 399 for chains of eight in place of 16.
 constexpr uint32_t TC_CHAIN = 16, TC_FIRST_CHAIN = 32, TC_SHORT_CHAIN = 8, TC_CUT_CHAIN = 6, TC_LEAST_CHAIN = 4;
 constexpr int TC_MAX_BUFS = 4;
+constexpr uint32_t MAX_CLUSTER = 4;         // pairs of a cluster (eight CTAs: the most that any chip of this kind places)
 // The same for rows taken exactly (EPILOGUE, LOGPROBS), by their parts: what keeps the result well within a millionth (2-norm
-// of the error over the result's, 2048 x [14336, 4096]: one part in chains of 8, 12 and 16 steps 4.7, 7.1 and 9.9e-7 and 235, 225 and
-// 216 us, two of 4, 6 and 8 4.7, 7.2 and 10.1e-7 and 369, 356 and 348 us, three of 2, 3 and 4 3.4, 5.5 and 7.7e-7 and 547, 514 and 505 us; a library's
+// of the error over the result's, 2048 x [14336, 4096]: one part in chains of 8, 12 and 16 steps 4.7, 7.1 and 9.9e-7 and in short runs 235, 225
+// and 216 us, two of 4, 6 and 8 4.7, 7.2 and 10.1e-7 and 369, 356 and 348 us, three of 2, 3 and 4 3.4, 5.5 and 7.7e-7 and 547, 514 and 505 us; a library's
 // f32 products 6 to 12e-7, yx_matmul 27e-7).  Results of 16 bits take chains that lose 4 to 7e-6: half a step of bf16 is 500
 // times that.  2048 bf16 rows x [14336, 4096], call after call, in chains of 64 steps (a whole tile's), 32, 16 and 12: 206, 219, 249 and
 // 256 us, and 0.23, 0.13, 0.07 and 0.05 % of the results are not the correctly rounded value but its neighbour (of a library's f32
 // sums 0.04 %); the same of f16 rows and results, in chains of 48, 24, 12 and 6, 359, 366, 381 and 412 us and 2.2, 1.2, 0.7 and 0.35 % (0.41 %).
-constexpr uint32_t MAX_CLUSTER = 4;         // pairs of a cluster (eight CTAs: the most that any chip of this kind places)
 constexpr uint32_t EXACT_CHAIN[3] = {12, 6, 4}, NARROW_CHAIN[3] = {64, 48, 32};
 constexpr uint32_t GLU_GROUP = 16;          // gate and up rows alternate in a tile sixteen by sixteen: a warp holds both
 
@@ -1379,7 +1379,7 @@ int cluster_for(yx_ctx *ctx, uint32_t tiles, uint32_t ksteps, uint32_t *out) {
 
 // Tiles that pass rows taken exactly are spread over.  More than hold them where that leaves fewer pairs idle: a k step takes
 // a CTA what its 16 KiB of weights and 64 bytes a pass row and part take at some 60 bytes a nanosecond, and pairs of a
-// cluster share it (300 f32 rows x [5633, 2040]: 46 tiles of 160 rows 34.6 us, 69 of 128 29.7; 600 bf16 x [4096, 4096] 40.3 and 27.7).
+// cluster share it (on the device, 300 f32 rows x [5633, 2040]: 46 tiles of 160 rows 34.6 us, 69 of 128 29.7; 600 bf16 x [4096, 4096] 40.3 and 27.7).
 template <int KIND>
 int exact_row_tiles(yx_ctx *ctx, const Product &p, uint32_t *out) {
     const uint32_t columns = (p.N + TC_M - 1) / TC_M, least = (p.T + TC_MAX_BT - 1) / TC_MAX_BT, ksteps = (p.K + TC_KSTEP - 1) / TC_KSTEP;
