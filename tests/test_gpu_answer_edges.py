@@ -372,3 +372,15 @@ def test_heads_however_they_are_dealt_out(backend, dtype, rows, n, k, dealt):
         # The entropy's error is that of independent errors of logits, a millionth of their size each, weighted with p (|log p| + h) and
         # added up as squares, and of its sums of n terms: a place or two of log n.
         assert (r.entropy - h).norm() <= 4e-6 * h.norm()
+
+
+def test_few_long_rows_are_one_launch(backend):
+    # (rows that the kernel cuts itself need no scratch, however long they are)
+    x, w = product(32, 8, 1500000, torch.float32)
+    before = backend.launch_count()
+    got = backend.matmul_epilogue(x, w)
+    assert backend.launch_count() - before == 1
+    backend.sync()
+    want = x.double() @ w.double().T
+    # 23438 k steps, eight at a time, in shares of some 160: sums of 2930 chains' f32 at most, half a last place each in the mean
+    assert (got - want).norm() <= 2930 ** 0.5 * 2.0 ** -23 * want.norm()

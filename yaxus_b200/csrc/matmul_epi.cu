@@ -123,7 +123,7 @@ int yx_matmul_epilogue(yx_ctx *ctx, const void *x_dev, int x_dtype, const void *
     }
     if (!tensor) return matmul_any(ctx, p, x_dtype);
     // (a result over rows that are cut into parts waits for all of them to be)
-    const bool scratch = p.parts > 1 || !aligned(p.x, 16);
+    const bool scratch = exact_tc_copies_rows(p);
     const uint32_t step = scratch && !overlap(out_dev, out_bytes, x_dev, x_bytes) ? rows_at_once(rows, (size_t)k * 2 * p.parts) : rows;
     for (uint32_t r = 0; r < rows; r += step) {
         Product s = p;
@@ -159,8 +159,7 @@ int yx_matmul_logprobs(yx_ctx *ctx, const void *x_dev, int x_dtype, const void *
     if (exact_tc_takes(p)) {
         // (the statistics, then the given tokens' logits)
         const size_t row_stats = (size_t)most_logprob_blocks(ctx, p) * 16;
-        const bool scratch = p.parts > 1 || !aligned(x_dev, 16);
-        const uint32_t step = rows_at_once(rows, std::max(row_stats, scratch ? (size_t)k * 2 * p.parts : (size_t)0));
+        const uint32_t step = rows_at_once(rows, std::max(row_stats, exact_tc_copies_rows(p) ? (size_t)k * 2 * p.parts : (size_t)0));
         if (int rc = grow(ctx, ctx->lp_stats, step * (row_stats + 4))) return rc;
         p.stats = ctx->lp_stats.dev;
         p.picked = (float *)(ctx->lp_stats.dev + step * row_stats);

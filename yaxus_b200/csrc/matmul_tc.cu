@@ -1679,6 +1679,7 @@ int launch_matmul_tc(yx_ctx *ctx, const float *x, const void *w, uint32_t T, uin
 }
 
 bool exact_tc_takes(const Product &p) { return p.K % 8 == 0 && ((uintptr_t)p.w & 15u) == 0; }
+bool exact_tc_copies_rows(const Product &p) { return p.T > ROWS_MAX && (p.parts > 1 || ((uintptr_t)p.x & 15u) != 0); }
 bool exact_tc_reads_rows_late(const Product &p) { return p.T <= ROWS_MAX || p.parts == 1; }
 // (lower tiles are at most as many more as complete a round of SMs)
 uint32_t most_logprob_blocks(yx_ctx *ctx, const Product &p) { return 2 * ((p.N + TC_M - 1) / TC_M) + (uint32_t)ctx->sm_count; }

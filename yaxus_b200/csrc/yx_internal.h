@@ -418,6 +418,8 @@ struct Product {
     const uint32_t *ids_dev, *ids_host;   // for more than 32 rows; for fewer
 };
 bool exact_tc_takes(const Product &p);
+// Whether the rows reach the kernel through scratch: in parts, or moved to 16 bytes.
+bool exact_tc_copies_rows(const Product &p);
 // Whether the kernel that writes the result is also the one that reads the rows.
 bool exact_tc_reads_rows_late(const Product &p);
 uint32_t most_logprob_blocks(yx_ctx *ctx, const Product &p);
